@@ -75,7 +75,8 @@ size_t b200k_attention_workspace_bytes(int batch, int num_q_heads, int num_kv_he
 /* The first word of every workspace is a status word that kernels OR bits into and never clear:
  *   bit 0 (1)  a bounded device-side wait gave up (attention pipeline);
  *   bit 1 (2)  a bounded wait of the tensor-core GEMM pipeline gave up;
- *   bit 2 (4)  a sequence length or cache position outside [0, max_len) was clamped / its row skipped.
+ *   bit 2 (4)  a sequence length or cache position outside [0, max_len) was clamped / its row skipped;
+ *   bit 3 (8)  a block table of a 4-bit cache named a block outside [0, num_blocks): its positions were skipped.
  * b200k_workspace_status copies it to the host for a caller-owned workspace (the `_ws` entry points;
  * synchronises the stream; allocates nothing); b200k_device_status (below) does the same for the
  * default workspace; b200k_workspace_clear_status sets it back to 0. */
@@ -505,6 +506,149 @@ int rope_kv_append_hm_f16(const b200k_half *qkv, const float *cos_table,
                           b200k_half *q_out, b200k_half *k_cache, b200k_half *v_cache,
                           int num_q_heads, int num_kv_heads, int head_dim, int max_len,
                           int batch, b200k_stream stream);
+
+/* ------------------------------------------------------------------------- */
+/* 4-bit KV cache                                                              */
+/* ------------------------------------------------------------------------- */
+/* No counterpart in the reference, whose caches hold the activations' own type.  A cache row is one (position, kv head):
+ * head_dim codes of 4 bits and, for every group_size consecutive dims, a (scale, base) pair of fp16:
+ *   x' = clamp(x, -65440, 65440)   base = fp16(min x')   scale = fp16((max x' - base) / 15)
+ *   code = clamp(round_half_even((x' - base) / scale), 0, 15), 0 where scale = 0     value = code * scale + base
+ * so infinities saturate, and a NaN makes its group read back as NaN.  head_dim is a multiple of 32 up to 256, group_size 32,
+ * 64 or 128 and divides it.  The row's head_dim/4 units of four codes (unit u = 8 j + r holds dims 4u .. 4u+3) stand at place
+ * r * (head_dim/32) + j, a unit in 16 bits and dim 4u in its lowest four.
+ *   head-major   codes [batch, heads, max_len, head_dim/8] int32, params [batch, heads, max_len, head_dim/group_size, 2] fp16
+ *   paged pool   codes [num_blocks, heads, block_size, head_dim/8], params [num_blocks, heads, block_size, head_dim/group_size, 2];
+ *                position p of sequence b is slot p % block_size of block block_table[b, p / block_size], block_table
+ *                [batch, max_blocks_per_seq]: a sequence holds up to max_blocks_per_seq * block_size positions (below 2^31)
+ * At head_dim 128 and group_size 64 a row takes 72 bytes where fp16 takes 256.  All tensors are contiguous, 16-byte aligned, and
+ * live on the current device; batch up to 65535.  Activations are fp16 or bf16, params fp16 with either.  Positions outside the
+ * cache and blocks outside the pool are skipped and reported in the status word (bits 2 and 3). */
+
+/* Appends rows [batch, tokens, num_heads, head_dim]: token t of sequence b goes to position cache_idx[b] + t.  stride_kt and
+ * stride_vt are the elements from one token to the next (num_heads * head_dim for a contiguous tensor, more for the k and v
+ * parts of a fused QKV tensor; multiples of 8).  new_lens [batch] says how many of a sequence's `tokens` rows are new, the rest
+ * being padding that is not stored; NULL: all.  tokens = 1 is the decode step.  Two sequences whose tables share the block that
+ * an append writes to race for the row. */
+int kv_cache_append_hm_int4_f16(const b200k_half *new_keys, const b200k_half *new_values, int32_t *k_codes,
+                                b200k_half *k_params, int32_t *v_codes, b200k_half *v_params,
+                                const int32_t *cache_idx, const int32_t *new_lens, int num_heads,
+                                int head_dim, int group_size, int max_len, int batch, int tokens,
+                                int stride_kt, int stride_vt, b200k_stream stream);
+int kv_cache_append_paged_int4_f16(const b200k_half *new_keys, const b200k_half *new_values, int32_t *k_codes,
+                                   b200k_half *k_params, int32_t *v_codes, b200k_half *v_params,
+                                   const int32_t *block_table, const int32_t *cache_idx,
+                                   const int32_t *new_lens, int num_heads, int head_dim, int group_size,
+                                   int block_size, int num_blocks, int max_blocks_per_seq, int batch,
+                                   int tokens, int stride_kt, int stride_vt, b200k_stream stream);
+/* rope_kv_append_hm_f16 for a 4-bit cache: q rotated into q_out, k rotated, rounded to its type and quantised, v quantised, both
+ * stored at positions[b].  qkv [batch, (num_q_heads + 2 num_kv_heads) * head_dim], tables [>= max_len, head_dim/2]. */
+int rope_kv_append_hm_int4_f16(const b200k_half *qkv, const float *cos_table, const float *sin_table,
+                               const int32_t *positions, b200k_half *q_out, int32_t *k_codes,
+                               b200k_half *k_params, int32_t *v_codes, b200k_half *v_params,
+                               int num_q_heads, int num_kv_heads, int head_dim, int group_size,
+                               int max_len, int batch, b200k_stream stream);
+/* Reads positions first[b] .. min(first[b] + out_len, context_lens[b]) - 1 back into k_out and v_out [batch, num_heads, out_len,
+ * head_dim] (the layout flash_attn_full_* takes), rows behind them left as they were.  first NULL: from position 0. */
+int kv_cache_read_hm_int4_f16(const int32_t *k_codes, const b200k_half *k_params, const int32_t *v_codes,
+                              const b200k_half *v_params, const int32_t *first, const int32_t *context_lens,
+                              b200k_half *k_out, b200k_half *v_out, int num_heads, int head_dim,
+                              int group_size, int max_len, int batch, int out_len, b200k_stream stream);
+int kv_cache_read_paged_int4_f16(const int32_t *k_codes, const b200k_half *k_params, const int32_t *v_codes,
+                                 const b200k_half *v_params, const int32_t *block_table,
+                                 const int32_t *first, const int32_t *context_lens, b200k_half *k_out,
+                                 b200k_half *v_out, int num_heads, int head_dim, int group_size,
+                                 int block_size, int num_blocks, int max_blocks_per_seq, int batch,
+                                 int out_len, b200k_stream stream);
+/* batched_decode_attention_hm_f16 over a 4-bit cache: q / output [batch, num_q_heads, head_dim], context_lens [batch] int32
+ * (0 or less: a zero output row), any GQA group size.  Scores, softmax and output are computed from the values in fp32; they
+ * are never written out in 16 bits.  The `_ws` editions take a workspace of b200k_attention_int4_workspace_bytes whose first
+ * 128 KiB are zero before the first call and then left to the kernels (b200k_workspace_status reads its status word); calls
+ * that may run at the same time need one each. */
+size_t b200k_attention_int4_workspace_bytes(int batch, int num_q_heads, int num_kv_heads, int head_dim);
+int batched_decode_attention_hm_int4_f16(const b200k_half *q, const int32_t *k_codes, const b200k_half *k_params,
+                                         const int32_t *v_codes, const b200k_half *v_params,
+                                         const int32_t *context_lens, b200k_half *output, int batch_size,
+                                         int num_q_heads, int num_kv_heads, int head_dim, int group_size,
+                                         int max_len, float scale, b200k_stream stream);
+int batched_decode_attention_hm_int4_f16_ws(const b200k_half *q, const int32_t *k_codes,
+                                            const b200k_half *k_params, const int32_t *v_codes,
+                                            const b200k_half *v_params, const int32_t *context_lens,
+                                            b200k_half *output, int batch_size, int num_q_heads,
+                                            int num_kv_heads, int head_dim, int group_size, int max_len,
+                                            float scale, void *workspace, size_t workspace_bytes,
+                                            b200k_stream stream);
+int batched_decode_attention_paged_int4_f16(const b200k_half *q, const int32_t *k_codes,
+                                            const b200k_half *k_params, const int32_t *v_codes,
+                                            const b200k_half *v_params, const int32_t *block_table,
+                                            const int32_t *context_lens, b200k_half *output, int batch_size,
+                                            int num_q_heads, int num_kv_heads, int head_dim, int group_size,
+                                            int block_size, int num_blocks, int max_blocks_per_seq,
+                                            float scale, b200k_stream stream);
+int batched_decode_attention_paged_int4_f16_ws(const b200k_half *q, const int32_t *k_codes,
+                                               const b200k_half *k_params, const int32_t *v_codes,
+                                               const b200k_half *v_params, const int32_t *block_table,
+                                               const int32_t *context_lens, b200k_half *output,
+                                               int batch_size, int num_q_heads, int num_kv_heads,
+                                               int head_dim, int group_size, int block_size,
+                                               int num_blocks, int max_blocks_per_seq, float scale,
+                                               void *workspace, size_t workspace_bytes,
+                                               b200k_stream stream);
+/* The same with bf16 activations (params stay fp16; |x| beyond 65440 saturates). */
+int kv_cache_append_hm_int4_bf16(const b200k_bf16 *new_keys, const b200k_bf16 *new_values, int32_t *k_codes,
+                                b200k_half *k_params, int32_t *v_codes, b200k_half *v_params,
+                                const int32_t *cache_idx, const int32_t *new_lens, int num_heads,
+                                int head_dim, int group_size, int max_len, int batch, int tokens,
+                                int stride_kt, int stride_vt, b200k_stream stream);
+int kv_cache_append_paged_int4_bf16(const b200k_bf16 *new_keys, const b200k_bf16 *new_values, int32_t *k_codes,
+                                   b200k_half *k_params, int32_t *v_codes, b200k_half *v_params,
+                                   const int32_t *block_table, const int32_t *cache_idx,
+                                   const int32_t *new_lens, int num_heads, int head_dim, int group_size,
+                                   int block_size, int num_blocks, int max_blocks_per_seq, int batch,
+                                   int tokens, int stride_kt, int stride_vt, b200k_stream stream);
+int rope_kv_append_hm_int4_bf16(const b200k_bf16 *qkv, const float *cos_table, const float *sin_table,
+                               const int32_t *positions, b200k_bf16 *q_out, int32_t *k_codes,
+                               b200k_half *k_params, int32_t *v_codes, b200k_half *v_params,
+                               int num_q_heads, int num_kv_heads, int head_dim, int group_size,
+                               int max_len, int batch, b200k_stream stream);
+int kv_cache_read_hm_int4_bf16(const int32_t *k_codes, const b200k_half *k_params, const int32_t *v_codes,
+                              const b200k_half *v_params, const int32_t *first, const int32_t *context_lens,
+                              b200k_bf16 *k_out, b200k_bf16 *v_out, int num_heads, int head_dim,
+                              int group_size, int max_len, int batch, int out_len, b200k_stream stream);
+int kv_cache_read_paged_int4_bf16(const int32_t *k_codes, const b200k_half *k_params, const int32_t *v_codes,
+                                 const b200k_half *v_params, const int32_t *block_table,
+                                 const int32_t *first, const int32_t *context_lens, b200k_bf16 *k_out,
+                                 b200k_bf16 *v_out, int num_heads, int head_dim, int group_size,
+                                 int block_size, int num_blocks, int max_blocks_per_seq, int batch,
+                                 int out_len, b200k_stream stream);
+int batched_decode_attention_hm_int4_bf16(const b200k_bf16 *q, const int32_t *k_codes, const b200k_half *k_params,
+                                         const int32_t *v_codes, const b200k_half *v_params,
+                                         const int32_t *context_lens, b200k_bf16 *output, int batch_size,
+                                         int num_q_heads, int num_kv_heads, int head_dim, int group_size,
+                                         int max_len, float scale, b200k_stream stream);
+int batched_decode_attention_hm_int4_bf16_ws(const b200k_bf16 *q, const int32_t *k_codes,
+                                            const b200k_half *k_params, const int32_t *v_codes,
+                                            const b200k_half *v_params, const int32_t *context_lens,
+                                            b200k_bf16 *output, int batch_size, int num_q_heads,
+                                            int num_kv_heads, int head_dim, int group_size, int max_len,
+                                            float scale, void *workspace, size_t workspace_bytes,
+                                            b200k_stream stream);
+int batched_decode_attention_paged_int4_bf16(const b200k_bf16 *q, const int32_t *k_codes,
+                                            const b200k_half *k_params, const int32_t *v_codes,
+                                            const b200k_half *v_params, const int32_t *block_table,
+                                            const int32_t *context_lens, b200k_bf16 *output, int batch_size,
+                                            int num_q_heads, int num_kv_heads, int head_dim, int group_size,
+                                            int block_size, int num_blocks, int max_blocks_per_seq,
+                                            float scale, b200k_stream stream);
+int batched_decode_attention_paged_int4_bf16_ws(const b200k_bf16 *q, const int32_t *k_codes,
+                                               const b200k_half *k_params, const int32_t *v_codes,
+                                               const b200k_half *v_params, const int32_t *block_table,
+                                               const int32_t *context_lens, b200k_bf16 *output,
+                                               int batch_size, int num_q_heads, int num_kv_heads,
+                                               int head_dim, int group_size, int block_size,
+                                               int num_blocks, int max_blocks_per_seq, float scale,
+                                               void *workspace, size_t workspace_bytes,
+                                               b200k_stream stream);
 
 /* ------------------------------------------------------------------------- */
 /* bf16 editions                                                               */

@@ -556,3 +556,74 @@ def decode_layer(hidden, p, k_cache, v_cache, positions, round_fp16=True, faithf
     if stages is not None:
         stages.update(n1=n1, qkv=qkv, q=q, att=attn, o=o, h1=h1, n2=n2, gate_up=gu, act=act, down=dn)
     return residual_add(h1, dn)
+
+
+# ---------------------------------------------------------------------------
+# 4-bit KV cache (no counterpart in the reference; in 64 bits, from the format's definition in b200_kernels.h)
+# ---------------------------------------------------------------------------
+KV4_LIMIT = 65440.0
+
+
+def kv4_places(d):
+    """[d] -> (word, shift): where the code of every dim stands in a row of d / 8 words."""
+    e = np.arange(d)
+    u = e // 4
+    place = (u % 8) * (d // 32) + u // 8
+    return place // 2, 16 * (place % 2) + 4 * (e % 4)
+
+
+def kv4_pack(codes):
+    """codes [..., d] 0..15 -> [..., d / 8] int32."""
+    d = codes.shape[-1]
+    word, shift = kv4_places(d)
+    out = np.zeros(codes.shape[:-1] + (d // 8,), dtype=np.uint32)
+    for e in range(d):
+        out[..., word[e]] |= codes[..., e].astype(np.uint32) << np.uint32(shift[e])
+    return out.view(np.int32)
+
+
+def kv4_unpack(words):
+    d = words.shape[-1] * 8
+    word, shift = kv4_places(d)
+    return ((words.view(np.uint32)[..., word] >> shift.astype(np.uint32)) & 15).astype(np.int32)
+
+
+def kv4_quantise(x, group):
+    """x [..., d] (values of a 16-bit type, any float dtype) -> (words, params [..., d / group, 2] fp16).  The difference and the
+    quotient that give the scale are fp32 operations, the quotient that gives a code is exact up to 2^-53."""
+    x = np.clip(np.asarray(x, dtype=np.float64), -KV4_LIMIT, KV4_LIMIT)
+    g = x.reshape(x.shape[:-1] + (x.shape[-1] // group, group))
+    with np.errstate(invalid="ignore"):
+        base = g.min(-1).astype(np.float16)
+        scale = ((g.max(-1).astype(np.float32) - base.astype(np.float32)) / np.float32(15)).astype(np.float16)
+        s, b = scale.astype(np.float64)[..., None], base.astype(np.float64)[..., None]
+        q = np.rint((g - b) / np.where(s > 0, s, 1.0))
+    codes = np.where(s > 0, np.clip(q, 0, 15), 0).astype(np.int32)
+    return kv4_pack(codes.reshape(x.shape)), np.stack([scale, base], -1)
+
+
+def kv4_values(words, params):
+    """The rows that a cache holds, in 64 bits: words [..., d / 8], params [..., d / group, 2] -> [..., d]."""
+    codes = kv4_unpack(words).astype(np.float64)
+    c = codes.reshape(params.shape[:-1] + (codes.shape[-1] // params.shape[-2],))
+    p = params.astype(np.float64)
+    return (c * p[..., 0:1] + p[..., 1:2]).reshape(codes.shape)
+
+
+def kv4_decode_attention(q, k_words, k_params, v_words, v_params, scale):
+    """q [hq, d], caches [hkv, len, ...] -> (output [hq, d], bound [hq, d]) in 64 bits.  `bound` is what rounding errors of the
+    probabilities (relative delta) and of the scores may add to an output, in units to be scaled by the caller:
+    (sum_p w_p (code scale + |base|), largest sum_d |q_d| (code scale + |base|) * |softmax scale|)."""
+    hq, d = q.shape
+    hkv, n = k_words.shape[:2]
+    out, mag, smag = np.zeros((hq, d)), np.zeros((hq, d)), np.zeros(hq)
+    for h in range(hq if n else 0):
+        kv = h // (hq // hkv)
+        k, v = kv4_values(k_words[kv], k_params[kv]), kv4_values(v_words[kv], v_params[kv])
+        ka, va = (kv4_values(w[kv], np.abs(p[kv])) for w, p in ((k_words, k_params), (v_words, v_params)))
+        z = k @ q[h].astype(np.float64) * scale
+        w = np.exp(z - z.max())
+        w /= w.sum()
+        out[h], mag[h] = w @ v, w @ va
+        smag[h] = np.max(ka @ np.abs(q[h].astype(np.float64))) * abs(scale)
+    return out, mag, smag[:, None]

@@ -331,6 +331,123 @@ extern "C" {
         q_out: *mut b200k_half, k_cache: *mut b200k_half, v_cache: *mut b200k_half, num_q_heads: c_int,
         num_kv_heads: c_int, head_dim: c_int, max_len: c_int, batch: c_int, stream: b200k_stream
     ) -> c_int;
+    pub fn kv_cache_append_hm_int4_f16(
+        new_keys: *const b200k_half, new_values: *const b200k_half, k_codes: *mut i32,
+        k_params: *mut b200k_half, v_codes: *mut i32, v_params: *mut b200k_half, cache_idx: *const i32,
+        new_lens: *const i32, num_heads: c_int, head_dim: c_int, group_size: c_int, max_len: c_int,
+        batch: c_int, tokens: c_int, stride_kt: c_int, stride_vt: c_int, stream: b200k_stream
+    ) -> c_int;
+    pub fn kv_cache_append_paged_int4_f16(
+        new_keys: *const b200k_half, new_values: *const b200k_half, k_codes: *mut i32,
+        k_params: *mut b200k_half, v_codes: *mut i32, v_params: *mut b200k_half, block_table: *const i32,
+        cache_idx: *const i32, new_lens: *const i32, num_heads: c_int, head_dim: c_int, group_size: c_int,
+        block_size: c_int, num_blocks: c_int, max_blocks_per_seq: c_int, batch: c_int, tokens: c_int,
+        stride_kt: c_int, stride_vt: c_int, stream: b200k_stream
+    ) -> c_int;
+    pub fn rope_kv_append_hm_int4_f16(
+        qkv: *const b200k_half, cos_table: *const f32, sin_table: *const f32, positions: *const i32,
+        q_out: *mut b200k_half, k_codes: *mut i32, k_params: *mut b200k_half, v_codes: *mut i32,
+        v_params: *mut b200k_half, num_q_heads: c_int, num_kv_heads: c_int, head_dim: c_int,
+        group_size: c_int, max_len: c_int, batch: c_int, stream: b200k_stream
+    ) -> c_int;
+    pub fn kv_cache_read_hm_int4_f16(
+        k_codes: *const i32, k_params: *const b200k_half, v_codes: *const i32, v_params: *const b200k_half,
+        first: *const i32, context_lens: *const i32, k_out: *mut b200k_half, v_out: *mut b200k_half,
+        num_heads: c_int, head_dim: c_int, group_size: c_int, max_len: c_int, batch: c_int, out_len: c_int,
+        stream: b200k_stream
+    ) -> c_int;
+    pub fn kv_cache_read_paged_int4_f16(
+        k_codes: *const i32, k_params: *const b200k_half, v_codes: *const i32, v_params: *const b200k_half,
+        block_table: *const i32, first: *const i32, context_lens: *const i32, k_out: *mut b200k_half,
+        v_out: *mut b200k_half, num_heads: c_int, head_dim: c_int, group_size: c_int, block_size: c_int,
+        num_blocks: c_int, max_blocks_per_seq: c_int, batch: c_int, out_len: c_int, stream: b200k_stream
+    ) -> c_int;
+    pub fn b200k_attention_int4_workspace_bytes(
+        batch: c_int, num_q_heads: c_int, num_kv_heads: c_int, head_dim: c_int
+    ) -> usize;
+    pub fn batched_decode_attention_hm_int4_f16(
+        q: *const b200k_half, k_codes: *const i32, k_params: *const b200k_half, v_codes: *const i32,
+        v_params: *const b200k_half, context_lens: *const i32, output: *mut b200k_half, batch_size: c_int,
+        num_q_heads: c_int, num_kv_heads: c_int, head_dim: c_int, group_size: c_int, max_len: c_int,
+        scale: f32, stream: b200k_stream
+    ) -> c_int;
+    pub fn batched_decode_attention_hm_int4_f16_ws(
+        q: *const b200k_half, k_codes: *const i32, k_params: *const b200k_half, v_codes: *const i32,
+        v_params: *const b200k_half, context_lens: *const i32, output: *mut b200k_half, batch_size: c_int,
+        num_q_heads: c_int, num_kv_heads: c_int, head_dim: c_int, group_size: c_int, max_len: c_int,
+        scale: f32, workspace: *mut c_void, workspace_bytes: usize, stream: b200k_stream
+    ) -> c_int;
+    pub fn batched_decode_attention_paged_int4_f16(
+        q: *const b200k_half, k_codes: *const i32, k_params: *const b200k_half, v_codes: *const i32,
+        v_params: *const b200k_half, block_table: *const i32, context_lens: *const i32,
+        output: *mut b200k_half, batch_size: c_int, num_q_heads: c_int, num_kv_heads: c_int, head_dim: c_int,
+        group_size: c_int, block_size: c_int, num_blocks: c_int, max_blocks_per_seq: c_int, scale: f32,
+        stream: b200k_stream
+    ) -> c_int;
+    pub fn batched_decode_attention_paged_int4_f16_ws(
+        q: *const b200k_half, k_codes: *const i32, k_params: *const b200k_half, v_codes: *const i32,
+        v_params: *const b200k_half, block_table: *const i32, context_lens: *const i32,
+        output: *mut b200k_half, batch_size: c_int, num_q_heads: c_int, num_kv_heads: c_int, head_dim: c_int,
+        group_size: c_int, block_size: c_int, num_blocks: c_int, max_blocks_per_seq: c_int, scale: f32,
+        workspace: *mut c_void, workspace_bytes: usize, stream: b200k_stream
+    ) -> c_int;
+    pub fn kv_cache_append_hm_int4_bf16(
+        new_keys: *const b200k_bf16, new_values: *const b200k_bf16, k_codes: *mut i32,
+        k_params: *mut b200k_half, v_codes: *mut i32, v_params: *mut b200k_half, cache_idx: *const i32,
+        new_lens: *const i32, num_heads: c_int, head_dim: c_int, group_size: c_int, max_len: c_int,
+        batch: c_int, tokens: c_int, stride_kt: c_int, stride_vt: c_int, stream: b200k_stream
+    ) -> c_int;
+    pub fn kv_cache_append_paged_int4_bf16(
+        new_keys: *const b200k_bf16, new_values: *const b200k_bf16, k_codes: *mut i32,
+        k_params: *mut b200k_half, v_codes: *mut i32, v_params: *mut b200k_half, block_table: *const i32,
+        cache_idx: *const i32, new_lens: *const i32, num_heads: c_int, head_dim: c_int, group_size: c_int,
+        block_size: c_int, num_blocks: c_int, max_blocks_per_seq: c_int, batch: c_int, tokens: c_int,
+        stride_kt: c_int, stride_vt: c_int, stream: b200k_stream
+    ) -> c_int;
+    pub fn rope_kv_append_hm_int4_bf16(
+        qkv: *const b200k_bf16, cos_table: *const f32, sin_table: *const f32, positions: *const i32,
+        q_out: *mut b200k_bf16, k_codes: *mut i32, k_params: *mut b200k_half, v_codes: *mut i32,
+        v_params: *mut b200k_half, num_q_heads: c_int, num_kv_heads: c_int, head_dim: c_int,
+        group_size: c_int, max_len: c_int, batch: c_int, stream: b200k_stream
+    ) -> c_int;
+    pub fn kv_cache_read_hm_int4_bf16(
+        k_codes: *const i32, k_params: *const b200k_half, v_codes: *const i32, v_params: *const b200k_half,
+        first: *const i32, context_lens: *const i32, k_out: *mut b200k_bf16, v_out: *mut b200k_bf16,
+        num_heads: c_int, head_dim: c_int, group_size: c_int, max_len: c_int, batch: c_int, out_len: c_int,
+        stream: b200k_stream
+    ) -> c_int;
+    pub fn kv_cache_read_paged_int4_bf16(
+        k_codes: *const i32, k_params: *const b200k_half, v_codes: *const i32, v_params: *const b200k_half,
+        block_table: *const i32, first: *const i32, context_lens: *const i32, k_out: *mut b200k_bf16,
+        v_out: *mut b200k_bf16, num_heads: c_int, head_dim: c_int, group_size: c_int, block_size: c_int,
+        num_blocks: c_int, max_blocks_per_seq: c_int, batch: c_int, out_len: c_int, stream: b200k_stream
+    ) -> c_int;
+    pub fn batched_decode_attention_hm_int4_bf16(
+        q: *const b200k_bf16, k_codes: *const i32, k_params: *const b200k_half, v_codes: *const i32,
+        v_params: *const b200k_half, context_lens: *const i32, output: *mut b200k_bf16, batch_size: c_int,
+        num_q_heads: c_int, num_kv_heads: c_int, head_dim: c_int, group_size: c_int, max_len: c_int,
+        scale: f32, stream: b200k_stream
+    ) -> c_int;
+    pub fn batched_decode_attention_hm_int4_bf16_ws(
+        q: *const b200k_bf16, k_codes: *const i32, k_params: *const b200k_half, v_codes: *const i32,
+        v_params: *const b200k_half, context_lens: *const i32, output: *mut b200k_bf16, batch_size: c_int,
+        num_q_heads: c_int, num_kv_heads: c_int, head_dim: c_int, group_size: c_int, max_len: c_int,
+        scale: f32, workspace: *mut c_void, workspace_bytes: usize, stream: b200k_stream
+    ) -> c_int;
+    pub fn batched_decode_attention_paged_int4_bf16(
+        q: *const b200k_bf16, k_codes: *const i32, k_params: *const b200k_half, v_codes: *const i32,
+        v_params: *const b200k_half, block_table: *const i32, context_lens: *const i32,
+        output: *mut b200k_bf16, batch_size: c_int, num_q_heads: c_int, num_kv_heads: c_int, head_dim: c_int,
+        group_size: c_int, block_size: c_int, num_blocks: c_int, max_blocks_per_seq: c_int, scale: f32,
+        stream: b200k_stream
+    ) -> c_int;
+    pub fn batched_decode_attention_paged_int4_bf16_ws(
+        q: *const b200k_bf16, k_codes: *const i32, k_params: *const b200k_half, v_codes: *const i32,
+        v_params: *const b200k_half, block_table: *const i32, context_lens: *const i32,
+        output: *mut b200k_bf16, batch_size: c_int, num_q_heads: c_int, num_kv_heads: c_int, head_dim: c_int,
+        group_size: c_int, block_size: c_int, num_blocks: c_int, max_blocks_per_seq: c_int, scale: f32,
+        workspace: *mut c_void, workspace_bytes: usize, stream: b200k_stream
+    ) -> c_int;
     pub fn w4a16_gptq_gemm_bf16(
         a: *const b200k_bf16, qweight: *const i32, scales: *const b200k_bf16, qzeros: *const i32,
         c: *mut b200k_bf16, m_size: c_int, n_size: c_int, k_size: c_int, group_size: c_int, stride_am: c_int,
