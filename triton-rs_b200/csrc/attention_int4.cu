@@ -1,113 +1,577 @@
 // GQA decode attention over the 4-bit KV cache (format: kv_int4.cuh).
 //
-// One CTA per (sequence, q head); warp w takes positions w, w + 4, ...; lanes stride over the units of a row.  Online
-// softmax per warp in fp32, merged across the warps at the end.
+// The codes never become values.  With a row's scale s and base z per group,
+//   q . K[p]        = sum_g s_pg (sum_{d in g} q_d c_pd) + z_pg (sum_{d in g} q_d)
+//   sum_p w_p V[p]  = sum_p (w_p s_pg) c_pd + sum_p w_p z_pg
+// so the matrix instructions multiply by the codes themselves and the scales go to the sums (K) and the probabilities (V).
+// A masked nibble is already an fp16 number: bits 0-3 of a half are the subnormal c 2^-24, bits 4-7 are c 2^-20, both exact,
+// so eight codes cost one shift and four ANDs (and one byte permute where two positions have to share a register).  The
+// factors of two go to q (K side) and to the output (V side).  Dequantising to fp16 first would take two more
+// instructions for every pair of codes and round every value.
+//
+// mma.sync m16n8k16 in transposed form, as in the 16-bit kernel: positions (K) or dims (V) fill the 16 rows, up to 8 q heads
+// of a GQA group the 8 columns; one query token a sequence cannot fill a 128-row tcgen05 tile, and the kernel is bound by
+// memory and by the issue of the integer instructions above, not by the tensor pipe.
+//
+// Work is cut evenly, not by sequence: the units of 64 positions of all (sequence, kv head, block of 8 q heads) are numbered
+// through, and every CTA of one wave takes the same number of consecutive units, whatever the lengths are; it works that out
+// from the lengths on the device, so a captured graph follows them.  A (sequence, head) that more than one CTA works on
+// is joined by the last of them to finish, in CTA order.  Each warp streams its 16-position tiles through a ring of
+// cp.async stages of its own, without any barrier between warps; rows behind the context are filled with zeros and never read.
 #include "kv_int4.cuh"
+#include "tma.cuh"
 
 namespace b200k {
+
+constexpr int A4_WARPS = 4, A4_THREADS = 32 * A4_WARPS, A4_STAGES = 4;
+constexpr int A4_TILE = 16, A4_UNIT = A4_WARPS * A4_TILE;      // positions of a warp's tile, of a unit of work
+constexpr int A4_HEADS = 8;                                    // columns of one MMA
+constexpr float A4_LAZY = 6.f;        // the running maximum moves when a score passes it by 2^6: probabilities stay below 2^6
+constexpr float A4_TOP = 512.f;       // 2^e times the largest value scale is set to [2^2, 2^3) and set again when it passes 2^9
 
 struct Attn4Args {
     const void *q;                // [B, Hq, D]
     void *out;                    // [B, Hq, D]
     const int32_t *lens;
     Kv4Cache C;
-    int hq;
-    float scale;
+    unsigned long long block_magic;   // floor(2^64 / block_size) + 1: pos / block_size = umul64hi(pos, magic) for pos < 2^32
+    int batch, hq, head_blocks;   // head_blocks: blocks of 8 q heads a kv head has
+    int bf16, out_kperm;
+    float scale_log2e;
     int *status;
+    int *counters;                // one per CTA, zero between launches
+    float *parts;                 // [CTA][2][D * 8 + 16]
 };
 
-template <typename T>
-__global__ void __launch_bounds__(128)
-attn4_kernel(Attn4Args A) {
-    __shared__ float sm_acc[4][256], sm_m[4], sm_l[4];
-    const Kv4Cache &C = A.C;
-    const int h = blockIdx.x, b = blockIdx.y, kvh = h / (A.hq / C.heads);
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int units = C.d / 4, nb = C.d / 32, groups = C.d / C.g;
-    pdl_wait();
-    pdl_launch_dependents();
-    int len = A.lens[b];
-    if (len > C.capacity) {
-        len = C.capacity;
-        if (threadIdx.x == 0 && h == 0) atomicOr(A.status, KV4_BAD_POSITION);
-    }
-    const T *q = (const T *)A.q + ((long)b * A.hq + h) * C.d;
-    float qr[2][4], acc[2][4];
+// ---- what a (head_dim, group) pair fixes -------------------------------------------------------------------------------
+template <int NB_, int NG_>
+struct A4 {
+    static constexpr int NB = NB_, NG = NG_;                  // blocks of 32 dims, groups
+    static constexpr int D = 32 * NB, G = D / NG;
+    static constexpr int ROW = 16 * NB, PROW = 4 * NG;        // bytes of a row's codes, of its params
+    static constexpr int PCOPY = NG % 4 == 0 ? 16 : NG % 2 == 0 ? 8 : 4;      // as wide as a row of params is aligned
+    static constexpr int STAGE = 2 * A4_TILE * (ROW + PROW) + 16;
+    static constexpr int KSTEPS = 2 * NB, MTILES = 2 * NB;
+    static constexpr bool PURE = G == 32;                     // a group is one block: see kword()
+    static constexpr int PART = D * A4_HEADS + 16;            // floats of a partial result
+    static constexpr int CTAS = NB <= 4 ? 4 : NB <= 6 ? 3 : 2;
+    static constexpr int RING = A4_WARPS * A4_STAGES * STAGE;
+    static constexpr int JOIN = A4_WARPS * D * A4_HEADS * 4;  // the warps' results, over the ring
+    static constexpr int SMEM = (RING > JOIN ? RING : JOIN) + 16;
+    // 16-byte chunk of a row in shared memory is chunk ^ swizzle(position): the K loads of a quarter warp (two rows of
+    // opposite parity) and the V loads of a half warp (positions 0-3 or 4-7) then meet no bank twice
+    __device__ static int swizzle(int pos) { return NB == 4 ? pos & 2 : NB == 8 ? ((pos & 3) << 1) | (pos & 1) : 0; }
+};
+
+__device__ __forceinline__ int a4_pos(int k) { return (k & 8) + ((k & 1) ? 4 + (((k & 7) >> 1) ^ 1) : (k & 7) >> 1); }   // position of MMA index k
+
+__device__ __forceinline__ void a4_mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t a4_transpose(uint32_t a) {
+    uint32_t d;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+    return d;
+}
+__device__ __forceinline__ float a4_exp2(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+template <int BYTES>
+__device__ __forceinline__ void a4_copy(uint32_t dst, const void *src, int bytes) {   // bytes = BYTES, or 0: zeros
+    if constexpr (BYTES == 16)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+    else
+        asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(BYTES), "r"(bytes) : "memory");
+}
+template <int N>
+__device__ __forceinline__ void a4_lds(uint32_t (&w)[N], const unsigned char *p) {    // N words, as aligned as their number allows
+    if constexpr (N % 4 == 0) {
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const int place = lane + 32 * i, u = (place % nb) * 8 + place / nb;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) qr[i][e] = acc[i][e] = 0.f;
-        if (place < units) Kv4Elem<T>::load(q + 4 * u, qr[i]);
-    }
-    float m = -INFINITY, l = 0.f;
-    for (int pos = warp; pos < len; pos += 4) {
-        const long row = kv4_row(C, b, kvh, pos);
-        if (row < 0) {      // a block that the pool does not have: its positions are left out
-            if (lane == 0) atomicOr(A.status, KV4_BAD_BLOCK);
-            continue;
+        for (int i = 0; i < N; i += 4) {
+            const uint4 u = *reinterpret_cast<const uint4 *>(p + 4 * i);
+            w[i] = u.x; w[i + 1] = u.y; w[i + 2] = u.z; w[i + 3] = u.w;
         }
-        float dot = 0.f, v[2][4];
+    } else if constexpr (N % 2 == 0) {
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const int place = lane + 32 * i, gi = 4 * ((place % nb) * 8 + place / nb) / C.g;
-            if (place >= units) continue;
-            const uint32_t kb = reinterpret_cast<const uint16_t *>(C.k_codes)[row * units + place];
-            const uint32_t vb = reinterpret_cast<const uint16_t *>(C.v_codes)[row * units + place];
-            const float2 kp = __half22float2(reinterpret_cast<const __half2 *>(C.k_params)[row * groups + gi]);
-            const float2 vp = __half22float2(reinterpret_cast<const __half2 *>(C.v_params)[row * groups + gi]);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                dot += qr[i][e] * fmaf((float)((kb >> (4 * e)) & 15u), kp.x, kp.y);
-                v[i][e] = fmaf((float)((vb >> (4 * e)) & 15u), vp.x, vp.y);
-            }
+        for (int i = 0; i < N; i += 2) {
+            const uint2 u = *reinterpret_cast<const uint2 *>(p + 4 * i);
+            w[i] = u.x; w[i + 1] = u.y;
         }
-        const float s = warp_sum(dot) * A.scale;
-        const float mn = fmaxf(m, s), alpha = expf(m - mn), p = expf(s - mn);
-        l = l * alpha + p;
+    } else {
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-                if (lane + 32 * i < units) acc[i][e] = acc[i][e] * alpha + p * v[i][e];
-        m = mn;
+        for (int i = 0; i < N; ++i) w[i] = *reinterpret_cast<const uint32_t *>(p + 4 * i);
     }
+}
+template <int NG>
+__device__ __forceinline__ void a4_params(float (&s)[NG], float (&z)[NG], const unsigned char *p) {
+    uint32_t w[NG];
+    a4_lds<NG>(w, p);
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const int place = lane + 32 * i, u = (place % nb) * 8 + place / nb;
-        if (place < units)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) sm_acc[warp][4 * u + e] = acc[i][e];
-    }
-    if (lane == 0) {
-        sm_m[warp] = m;
-        sm_l[warp] = l;
-    }
-    __syncthreads();
-    const float M = fmaxf(fmaxf(sm_m[0], sm_m[1]), fmaxf(sm_m[2], sm_m[3]));
-    float w[4], L = 0.f;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        w[j] = sm_l[j] == 0.f ? 0.f : expf(sm_m[j] - M);
-        L += sm_l[j] * w[j];
-    }
-    for (int i = 2 * threadIdx.x; i < C.d; i += 256) {
-        float o[2] = {0.f, 0.f};
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            o[0] += sm_acc[j][i] * w[j];
-            o[1] += sm_acc[j][i + 1] * w[j];
-        }
-        // no keys: a zero output row
-        reinterpret_cast<uint32_t *>((T *)A.out + ((long)b * A.hq + h) * C.d)[i / 2] = L == 0.f ? 0u : Kv4Elem<T>::pack(o[0] / L, o[1] / L);
+    for (int g = 0; g < NG; ++g) {
+        const float2 f = h2_to_f2(w[g]);
+        s[g] = f.x; z[g] = f.y;
     }
 }
 
-constexpr size_t ATTN4_WS_BYTES = 128 * 1024;
+// Lane t of a K row holds units (2t, j) and (2t + 1, j), j = 0 .. NB-1, in this order, in NB words.  Word i of its operand: where
+// a group spans several blocks, the two blocks of a word share a register (word i as loaded); where a group is one block,
+// the two units of block i do.  Either way all products of one MMA belong to one group.
+template <int NB, bool PURE>
+__device__ __forceinline__ uint32_t a4_kword(const uint32_t (&w)[NB], int i) {
+    if constexpr (!PURE) return w[i];
+    const int a = i, b = NB + i;
+    return __byte_perm(w[a >> 1], w[b >> 1], (a & 1 ? 0x32 : 0x10) | ((b & 1 ? 0x76 : 0x54) << 8));
+}
+// dims of the low and high half of nibble n of operand word i, for lane t
+template <int NB, bool PURE>
+__device__ __forceinline__ void a4_kdims(int i, int n, int t, int &lo, int &hi) {
+    if constexpr (PURE) {
+        lo = 32 * i + 8 * t + n;
+        hi = lo + 4;
+    } else {
+        const int rho = 2 * t + (i >= NB / 2), jp = i % (NB / 2);
+        lo = 64 * jp + 4 * rho + n;
+        hi = lo + 32;
+    }
+}
+template <int NB, int NG, bool PURE>
+__device__ __forceinline__ constexpr int a4_kgroup(int i) { return PURE ? i : (i % (NB / 2)) * 2 * NG / NB; }
 
-template <typename T>
+template <int NB, int NG>
+__global__ void __launch_bounds__(A4_THREADS, A4<NB, NG>::CTAS)
+attn4_kernel(const Attn4Args A) {
+    using X = A4<NB, NG>;
+    extern __shared__ __align__(16) unsigned char smem[];
+    __shared__ float sm_ref[A4_WARPS][A4_HEADS], sm_l[A4_WARPS][A4_HEADS], sm_w[A4_WARPS][A4_HEADS], sm_top[A4_HEADS], sm_sum[A4_HEADS];
+    __shared__ int sm_last;
+    const Kv4Cache &C = A.C;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, r = lane >> 2, t = lane & 3;
+    const int cta = blockIdx.x, gqa = A.hq / C.heads, per_seq = C.heads * A.head_blocks;
+    pdl_wait();
+    pdl_launch_dependents();
+
+    // ---- the share of this CTA: units [begin, end) of all ------------------------------------------------------------------
+    auto length = [&](int b) { return min(A.lens[b], C.capacity); };
+    auto units_of = [&](int b) { return (max(length(b), 0) + A4_UNIT - 1) / A4_UNIT; };
+    long total = 0;
+    for (int b = lane; b < A.batch; b += 32) total += units_of(b);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+    total *= per_seq;
+    const long share = max((total + gridDim.x - 1) / (long)gridDim.x, 1l);
+    const long begin = share * cta, end = min(begin + share, total);
+    for (int b = cta; b < A.batch; b += gridDim.x) {
+        const int len = A.lens[b];
+        if (len > C.capacity && tid == 0) atomicOr(A.status, KV4_BAD_POSITION);
+        if (len <= 0)       // no keys: a zero output row
+            for (int i = tid; i < A.hq * X::D / 2; i += A4_THREADS) reinterpret_cast<uint32_t *>(A.out)[(long)b * A.hq * X::D / 2 + i] = 0u;
+    }
+    if (begin >= end) return;
+    int b = 0;
+    long start = 0;         // units before sequence b
+    for (int b0 = 0; b0 < A.batch; b0 += 32) {
+        const long mine = b0 + lane < A.batch ? (long)units_of(b0 + lane) * per_seq : 0;
+        long upto = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const long x = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += x;
+        }
+        const unsigned past = __ballot_sync(0xffffffffu, start + upto > begin);
+        if (past) {
+            const int at = __ffs(past) - 1;
+            b = b0 + at;
+            start += __shfl_sync(0xffffffffu, upto - mine, at);
+            break;
+        }
+        start += __shfl_sync(0xffffffffu, upto, 31);
+    }
+
+    unsigned char *ring = smem + warp * A4_STAGES * X::STAGE;
+    const int kpos0 = a4_pos(r);                               // this lane's K rows: kpos0 and kpos0 + 8
+    const int vpos0 = t, vpos1 = 4 + (t ^ 1);                  // its V rows: these and + 8
+
+    for (long at = begin; at < end;) {
+        // ---- one segment: units [u0, u1) of (sequence b, kv head, block of q heads) -------------------------------------------
+        int n = units_of(b);
+        while (at >= start + (long)n * per_seq) {
+            start += (long)n * per_seq;
+            n = units_of(++b);
+        }
+        const int len = length(b);
+        const int item = (int)((at - start) / n);
+        const long item_start = start + (long)item * n;
+        const int u0 = (int)(at - item_start), u1 = (int)min((long)n, end - item_start);
+        const int kvh = item / A.head_blocks, h0 = kvh * gqa + (item % A.head_blocks) * A4_HEADS;
+        const int heads = min(A4_HEADS, (kvh + 1) * gqa - h0);
+        at = item_start + u1;
+
+        // tile i of this warp -> stage i % STAGES
+        auto issue = [&](int i) {
+            const int p0 = (u0 + i) * A4_UNIT + warp * A4_TILE;
+            unsigned char *st = ring + (i % A4_STAGES) * X::STAGE;
+            const bool one = !C.block_table || C.block_size % A4_TILE == 0;      // the tile lies in one block: its rows are neighbours
+            long first = 0;
+            if (!C.block_table) {
+                first = ((long)b * C.heads + kvh) * C.capacity + p0;
+            } else if (one && p0 < len) {
+                const int lb = (int)__umul64hi((unsigned long long)p0, A.block_magic);
+                const int blk = C.block_table[(long)b * C.max_blocks + lb];
+                first = (unsigned)blk < (unsigned)C.num_blocks ? ((long)blk * C.heads + kvh) * C.block_size + (p0 - lb * C.block_size) : -1;
+            }
+            auto row_of = [&](int row) {           // -1: behind the context, or in a block that the pool does not have
+                if (p0 + row >= len) return -1l;
+                if (one) return first < 0 ? -1l : first + row;
+                return kv4_row(C, b, kvh, p0 + row);
+            };
+#pragma unroll
+            for (int c = lane; c < A4_TILE * NB; c += 32) {
+                const int row = c / NB, part = c % NB;
+                const long rr = row_of(row);
+                const uint32_t dst = smem_u32(st + row * X::ROW + (part ^ X::swizzle(row)) * 16);
+                const long off = max(rr, 0l) * X::ROW + part * 16;
+                a4_copy<16>(dst, (const unsigned char *)C.k_codes + off, rr < 0 ? 0 : 16);
+                a4_copy<16>(dst + A4_TILE * X::ROW, (const unsigned char *)C.v_codes + off, rr < 0 ? 0 : 16);
+            }
+            const int row = lane & 15;
+            const long rr = row_of(row);
+#pragma unroll
+            for (int c = 0; c < X::PROW; c += X::PCOPY)
+                a4_copy<X::PCOPY>(smem_u32(st + 2 * A4_TILE * X::ROW + lane * X::PROW + c),
+                                  (const unsigned char *)(lane < 16 ? C.k_params : C.v_params) + max(rr, 0l) * X::PROW + c, rr < 0 ? 0 : X::PCOPY);
+            const unsigned valid = __ballot_sync(0xffffffffu, rr >= 0);
+            if (lane == 0) {
+                *reinterpret_cast<uint32_t *>(st + X::STAGE - 16) = valid;
+                const int rows = min(A4_TILE, len - p0);
+                if (rows > 0 && __popc(valid & 0xffffu) != rows) atomicOr(A.status, KV4_BAD_BLOCK);
+            }
+            asm volatile("cp.async.commit_group;" ::: "memory");
+        };
+        const int tiles = u1 - u0;
+#pragma unroll
+        for (int i = 0; i < A4_STAGES - 1; ++i) {
+            if (i < tiles) issue(i);
+            else asm volatile("cp.async.commit_group;" ::: "memory");
+        }
+
+        // ---- q as the B operand: head r, lane t's dims; scaled by a power of two to [2^14, 2^15) ----------------------------------
+        // (any 16-bit type then fits fp16 with all its bits, down to 2^-25 of the head's largest element; nibbles 1 and 3 carry
+        // 2^4 more than 0 and 2, so their q is divided by 16)
+        uint32_t qf[4 * NB];
+        float qsum[NG][2], fac[2];             // of heads 2t and 2t + 1: sum of q over a group, and what a score is multiplied by
+        {
+            const uint16_t *qrow = (const uint16_t *)A.q + ((long)b * A.hq + h0 + r) * X::D;
+            auto ld = [&](int d) {
+                const uint16_t x = r < heads ? qrow[d] : (uint16_t)0;
+                return A.bf16 ? __uint_as_float((uint32_t)x << 16) : __half2float(__ushort_as_half(x));
+            };
+            float big = 0.f;
+#pragma unroll
+            for (int i = 0; i < NB; ++i)
+#pragma unroll
+                for (int nn = 0; nn < 4; ++nn) {
+                    int lo, hi;
+                    a4_kdims<NB, X::PURE>(i, nn, t, lo, hi);
+                    big = fmaxf(big, fmaxf(fabsf(ld(lo)), fabsf(ld(hi))));
+                }
+            big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
+            big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
+            const int k = min(14 - ((int)(__float_as_uint(big) >> 23) - 127), 126);
+            const float up = copysignf(__uint_as_float((uint32_t)(k + 127) << 23), A.scale_log2e);
+            float sum[NG] = {};
+#pragma unroll
+            for (int i = 0; i < NB; ++i)
+#pragma unroll
+                for (int nn = 0; nn < 4; ++nn) {
+                    int lo, hi;
+                    a4_kdims<NB, X::PURE>(i, nn, t, lo, hi);
+                    const float a = ld(lo) * up, c = ld(hi) * up;
+                    sum[a4_kgroup<NB, NG, X::PURE>(i)] += a + c;
+                    qf[4 * i + nn] = (nn & 1) ? f2_to_h2(a * 0.0625f, c * 0.0625f) : f2_to_h2(a, c);
+                }
+            // an infinite q has no finite score: NaN, as inf - inf gives
+            const float f = big < INFINITY ? fabsf(A.scale_log2e) / fabsf(up) * 16777216.f : NAN;
+#pragma unroll
+            for (int g = 0; g < NG; ++g) {
+                sum[g] += __shfl_xor_sync(0xffffffffu, sum[g], 1);
+                sum[g] += __shfl_xor_sync(0xffffffffu, sum[g], 2);
+                sum[g] *= 1.f / 16777216.f;
+                qsum[g][0] = __shfl_sync(0xffffffffu, sum[g], 8 * t);
+                qsum[g][1] = __shfl_sync(0xffffffffu, sum[g], 8 * t + 4);
+            }
+            fac[0] = __shfl_sync(0xffffffffu, r < heads ? f : 0.f, 8 * t);
+            fac[1] = __shfl_sync(0xffffffffu, r < heads ? f : 0.f, 8 * t + 4);
+        }
+
+        float oacc[X::MTILES][4], zacc[NG][2], l[2] = {0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < X::MTILES; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) oacc[i][j] = 0.f;
+#pragma unroll
+        for (int g = 0; g < NG; ++g) zacc[g][0] = zacc[g][1] = 0.f;
+        // top: the running maximum of the raw scores; a probability is 2^(score fac - ref), ref = top fac - e: the factor 2^e,
+        // the same for all heads, keeps probability times value scale inside fp16 and cancels in the end
+        float top[2] = {-1e30f, -1e30f}, ref[2] = {0.f, 0.f}, bar[2] = {-1e30f, -1e30f}, e = 0.f, most = -1.f;
+        if (!(fac[0] > 0.f)) { top[0] = 0.f; bar[0] = INFINITY; ref[0] = 0.f; }
+        if (!(fac[1] > 0.f)) { top[1] = 0.f; bar[1] = INFINITY; ref[1] = 0.f; }
+
+        for (int i = 0; i < tiles; ++i) {
+            asm volatile("cp.async.wait_group %0;" ::"n"(A4_STAGES - 2) : "memory");
+            __syncwarp();
+            if (i + A4_STAGES - 1 < tiles) issue(i + A4_STAGES - 1);
+            else asm volatile("cp.async.commit_group;" ::: "memory");
+            const unsigned char *st = ring + (i % A4_STAGES) * X::STAGE;
+            const unsigned char *sk = st, *sv = st + A4_TILE * X::ROW, *pk = sv + A4_TILE * X::ROW, *pv = pk + A4_TILE * X::PROW;
+            const uint32_t valid = *reinterpret_cast<const uint32_t *>(st + X::STAGE - 16) & 0xffffu;
+
+            // scores: rows r and r + 8 are positions kpos0 and kpos0 + 8, columns heads 2t and 2t + 1
+            float s[4] = {0.f, 0.f, 0.f, 0.f};
+            {
+                uint32_t w0[NB], w1[NB];
+                if constexpr (NB == 8) {
+                    const int sw = X::swizzle(kpos0);         // the same for + 8
+                    a4_lds<4>(*reinterpret_cast<uint32_t (*)[4]>(&w0[0]), sk + kpos0 * X::ROW + ((2 * t) ^ sw) * 16);
+                    a4_lds<4>(*reinterpret_cast<uint32_t (*)[4]>(&w0[4]), sk + kpos0 * X::ROW + ((2 * t + 1) ^ sw) * 16);
+                    a4_lds<4>(*reinterpret_cast<uint32_t (*)[4]>(&w1[0]), sk + (kpos0 + 8) * X::ROW + ((2 * t) ^ sw) * 16);
+                    a4_lds<4>(*reinterpret_cast<uint32_t (*)[4]>(&w1[4]), sk + (kpos0 + 8) * X::ROW + ((2 * t + 1) ^ sw) * 16);
+                } else {
+                    const int off = NB == 4 ? (t ^ X::swizzle(kpos0)) * 16 : t * 4 * NB;
+                    a4_lds<NB>(w0, sk + kpos0 * X::ROW + off);
+                    a4_lds<NB>(w1, sk + (kpos0 + 8) * X::ROW + off);
+                }
+                float s0[NG], z0[NG], s1[NG], z1[NG];
+                a4_params<NG>(s0, z0, pk + kpos0 * X::PROW);
+                a4_params<NG>(s1, z1, pk + (kpos0 + 8) * X::PROW);
+#pragma unroll
+                for (int g = 0; g < NG; ++g) {
+                    float acc[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int j = 0; j < NB; ++j) {
+                        if (a4_kgroup<NB, NG, X::PURE>(j) != g) continue;
+                        const uint32_t x = a4_kword<NB, X::PURE>(w0, j), y = a4_kword<NB, X::PURE>(w1, j);
+                        const uint32_t x8 = x >> 8, y8 = y >> 8;
+                        a4_mma(acc, x & 0x000f000fu, y & 0x000f000fu, x & 0x00f000f0u, y & 0x00f000f0u, qf[4 * j], qf[4 * j + 1]);
+                        a4_mma(acc, x8 & 0x000f000fu, y8 & 0x000f000fu, x8 & 0x00f000f0u, y8 & 0x00f000f0u, qf[4 * j + 2], qf[4 * j + 3]);
+                    }
+                    s[0] = fmaf(s0[g], acc[0], fmaf(z0[g], qsum[g][0], s[0]));
+                    s[1] = fmaf(s0[g], acc[1], fmaf(z0[g], qsum[g][1], s[1]));
+                    s[2] = fmaf(s1[g], acc[2], fmaf(z1[g], qsum[g][0], s[2]));
+                    s[3] = fmaf(s1[g], acc[3], fmaf(z1[g], qsum[g][1], s[3]));
+                }
+            }
+            float vs0[NG], vz0[NG], vs1[NG], vz1[NG];
+            a4_params<NG>(vs0, vz0, pv + kpos0 * X::PROW);
+            a4_params<NG>(vs1, vz1, pv + (kpos0 + 8) * X::PROW);
+            const bool ok0 = (valid >> kpos0) & 1, ok1 = (valid >> (kpos0 + 8)) & 1;
+            if (valid != 0xffffu) {
+                if (!ok0) s[0] = s[1] = -1e30f;
+                if (!ok1) s[2] = s[3] = -1e30f;
+            }
+            float vmax = 0.f;
+#pragma unroll
+            for (int g = 0; g < NG; ++g) vmax = fmaxf(vmax, fmaxf(vs0[g], vs1[g]));
+            if (__any_sync(0xffffffffu, fmaxf(s[0], s[2]) > bar[0] || fmaxf(s[1], s[3]) > bar[1] || vmax > most)) {
+                // a score or a value scale has outgrown what the probabilities are held against
+                float n0 = fmaxf(top[0], fmaxf(s[0], s[2])), n1 = fmaxf(top[1], fmaxf(s[1], s[3]));
+#pragma unroll
+                for (int o = 4; o <= 16; o <<= 1) {
+                    n0 = fmaxf(n0, __shfl_xor_sync(0xffffffffu, n0, o));
+                    n1 = fmaxf(n1, __shfl_xor_sync(0xffffffffu, n1, o));
+                    vmax = fmaxf(vmax, __shfl_xor_sync(0xffffffffu, vmax, o));
+                }
+                if (vmax > most) {
+                    // 2^e vmax in [2^2, 2^3): vmax is a positive fp16 number, so its exponent lies in -24 .. 15
+                    const int ex = (int)(__float_as_uint(vmax) >> 23) - 127;
+                    e = vmax > 0.f ? 2.f - (float)ex : 0.f;
+                    most = vmax > 0.f ? A4_TOP * a4_exp2(-e) : 0.f;
+                }
+                const float f0 = fac[0], f1 = fac[1];
+                const float r0 = f0 > 0.f ? n0 * f0 - e : -e, r1 = f1 > 0.f ? n1 * f1 - e : -e;
+                const float a0 = top[0] <= -1e30f ? 0.f : a4_exp2(ref[0] - r0), a1 = top[1] <= -1e30f ? 0.f : a4_exp2(ref[1] - r1);
+                if (f0 > 0.f) { top[0] = n0; bar[0] = n0 + A4_LAZY / f0; }
+                if (f1 > 0.f) { top[1] = n1; bar[1] = n1 + A4_LAZY / f1; }
+                ref[0] = r0;
+                ref[1] = r1;
+                l[0] *= a0;
+                l[1] *= a1;
+#pragma unroll
+                for (int g = 0; g < NG; ++g) { zacc[g][0] *= a0; zacc[g][1] *= a1; }
+#pragma unroll
+                for (int m = 0; m < X::MTILES; ++m) { oacc[m][0] *= a0; oacc[m][1] *= a1; oacc[m][2] *= a0; oacc[m][3] *= a1; }
+            }
+            float p[4];
+            p[0] = a4_exp2(fmaf(s[0], fac[0], -ref[0]));
+            p[1] = a4_exp2(fmaf(s[1], fac[1], -ref[1]));
+            p[2] = a4_exp2(fmaf(s[2], fac[0], -ref[0]));
+            p[3] = a4_exp2(fmaf(s[3], fac[1], -ref[1]));
+            if (valid != 0xffffu) {
+                if (!ok0) p[0] = p[1] = 0.f;
+                if (!ok1) p[2] = p[3] = 0.f;
+            }
+            l[0] += p[0] + p[2];
+            l[1] += p[1] + p[3];
+            uint32_t pb[NG][2];            // (probability x value scale)^T as the B operand; the one rounding to fp16 on the way
+#pragma unroll
+            for (int g = 0; g < NG; ++g) {
+                pb[g][0] = a4_transpose(f2_to_h2(p[0] * vs0[g], p[1] * vs0[g]));
+                pb[g][1] = a4_transpose(f2_to_h2(p[2] * vs1[g], p[3] * vs1[g]));
+                zacc[g][0] = fmaf(p[0], vz0[g], fmaf(p[2], vz1[g], zacc[g][0]));
+                zacc[g][1] = fmaf(p[1], vz0[g], fmaf(p[3], vz1[g], zacc[g][1]));
+            }
+            // output: rows r and r + 8 of m-tile 2 j + h are dims 32 j + 4 r + 2 h and + 1
+            auto out_tiles = [&](int j, uint32_t x, uint32_t y) {
+                const int g = j * NG / NB;
+                a4_mma(oacc[2 * j], x & 0x000f000fu, x & 0x00f000f0u, y & 0x000f000fu, y & 0x00f000f0u, pb[g][0], pb[g][1]);
+                x >>= 8;
+                y >>= 8;
+                a4_mma(oacc[2 * j + 1], x & 0x000f000fu, x & 0x00f000f0u, y & 0x000f000fu, y & 0x00f000f0u, pb[g][0], pb[g][1]);
+            };
+            if constexpr (NB % 2 == 0) {
+                uint32_t va[NB / 2], vb[NB / 2], vc[NB / 2], vd[NB / 2];
+                // lane r's piece of a row: 2 NB bytes at 2 NB r
+                auto piece = [&](int pos) {
+                    const int byte = 2 * NB * r;
+                    return sv + pos * X::ROW + (((byte >> 4) ^ X::swizzle(pos)) << 4) + (byte & 15);
+                };
+                a4_lds<NB / 2>(va, piece(vpos0));
+                a4_lds<NB / 2>(vb, piece(vpos1));
+                a4_lds<NB / 2>(vc, piece(vpos0 + 8));
+                a4_lds<NB / 2>(vd, piece(vpos1 + 8));
+#pragma unroll
+                for (int j = 0; j < NB; ++j) {
+                    const int sel = j & 1 ? 0x7632 : 0x5410;
+                    out_tiles(j, __byte_perm(va[j >> 1], vb[j >> 1], sel), __byte_perm(vc[j >> 1], vd[j >> 1], sel));
+                }
+            } else {
+                auto unit = [&](int pos, int j) { return (uint32_t) * reinterpret_cast<const uint16_t *>(sv + pos * X::ROW + 2 * (NB * r + j)); };
+#pragma unroll
+                for (int j = 0; j < NB; ++j)
+                    out_tiles(j, unit(vpos0, j) | unit(vpos1, j) << 16, unit(vpos0 + 8, j) | unit(vpos1 + 8, j) << 16);
+            }
+        }
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+
+        // ---- join the warps ----------------------------------------------------------------------------------------------
+#pragma unroll
+        for (int o = 4; o <= 16; o <<= 1) {
+            l[0] += __shfl_xor_sync(0xffffffffu, l[0], o);
+            l[1] += __shfl_xor_sync(0xffffffffu, l[1], o);
+#pragma unroll
+            for (int g = 0; g < NG; ++g) {
+                zacc[g][0] += __shfl_xor_sync(0xffffffffu, zacc[g][0], o);
+                zacc[g][1] += __shfl_xor_sync(0xffffffffu, zacc[g][1], o);
+            }
+        }
+        __syncthreads();                   // every warp is done with its ring
+        float *so = reinterpret_cast<float *>(smem);       // [warp][m-tile row][head]
+#pragma unroll
+        for (int m = 0; m < X::MTILES; ++m) {
+            const int g = (m / 2) * NG / NB;
+            float *o0 = so + ((warp * X::D) + m * 16 + r) * A4_HEADS + 2 * t;
+            *reinterpret_cast<float2 *>(o0) = make_float2(fmaf(oacc[m][0], 16777216.f, zacc[g][0]), fmaf(oacc[m][1], 16777216.f, zacc[g][1]));
+            *reinterpret_cast<float2 *>(o0 + 8 * A4_HEADS) = make_float2(fmaf(oacc[m][2], 1048576.f, zacc[g][0]), fmaf(oacc[m][3], 1048576.f, zacc[g][1]));
+        }
+        if (lane < 4) {
+            const bool some0 = l[0] != 0.f, some1 = l[1] != 0.f;    // a warp without positions has no say in the maximum
+            sm_ref[warp][2 * t] = some0 ? ref[0] : -INFINITY;
+            sm_ref[warp][2 * t + 1] = some1 ? ref[1] : -INFINITY;
+            sm_l[warp][2 * t] = l[0];
+            sm_l[warp][2 * t + 1] = l[1];
+        }
+        __syncthreads();
+        if (tid < A4_HEADS) {
+            float M = -INFINITY, L = 0.f;
+            for (int w = 0; w < A4_WARPS; ++w) M = fmaxf(M, sm_ref[w][tid]);
+            for (int w = 0; w < A4_WARPS; ++w) {
+                const float x = sm_l[w][tid] == 0.f ? 0.f : exp2f(sm_ref[w][tid] - M);
+                sm_w[w][tid] = x;
+                L += sm_l[w][tid] * x;
+            }
+            sm_top[tid] = M;
+            sm_sum[tid] = L;
+        }
+        __syncthreads();
+        auto joined = [&](int idx, int h) {
+            float o = 0.f;
+#pragma unroll
+            for (int w = 0; w < A4_WARPS; ++w) {
+                const float x = sm_w[w][h];
+                o += x == 0.f ? 0.f : so[(w * X::D + idx) * A4_HEADS + h] * x;
+            }
+            return o;
+        };
+        auto index_of = [](int d) { return (2 * (d >> 5) + ((d >> 1) & 1)) * 16 + ((d & 31) >> 2) + 8 * (d & 1); };   // dim -> m-tile row
+        auto store = [&](int h, int d, float v) {
+            const long at_out = ((long)b * A.hq + h0 + h) * X::D;
+            const int e7 = d & 7, dd = A.out_kperm ? (d & ~7) | (e7 < 4 ? 2 * e7 : 2 * e7 - 7) : d;
+            if (A.bf16) reinterpret_cast<__nv_bfloat16 *>(A.out)[at_out + dd] = __float2bfloat16_rn(v);
+            else reinterpret_cast<__half *>(A.out)[at_out + dd] = __float2half_rn(v);
+        };
+        if (u0 == 0 && u1 == n) {          // the whole context was here
+            for (int i = tid; i < heads * X::D; i += A4_THREADS) {
+                const int h = i / X::D, d = i % X::D;
+                store(h, d, sm_sum[h] == 0.f ? 0.f : joined(index_of(d), h) / sm_sum[h]);
+            }
+            __syncthreads();
+            continue;
+        }
+        // ---- join the CTAs: partial results through the workspace, the last to arrive adds them up in CTA order ------------------
+        const int c0 = (int)(item_start / share), c1 = (int)((item_start + n - 1) / share);
+        float *part = A.parts + ((long)cta * 2 + (u0 == 0)) * X::PART;
+        for (int i = tid; i < X::D * A4_HEADS; i += A4_THREADS) part[i] = joined(i / A4_HEADS, i % A4_HEADS);
+        if (tid < A4_HEADS) {
+            part[X::D * A4_HEADS + 2 * tid] = sm_top[tid];
+            part[X::D * A4_HEADS + 2 * tid + 1] = sm_sum[tid];
+        }
+        __threadfence();
+        __syncthreads();
+        if (tid == 0) sm_last = atomicAdd(&A.counters[c0], 1) == c1 - c0;
+        __syncthreads();
+        if (sm_last) {
+            __threadfence();
+            auto part_of = [&](int c) { return A.parts + ((long)c * 2 + (c == c0)) * X::PART; };
+            for (int i = tid; i < heads * X::D; i += A4_THREADS) {
+                const int h = i / X::D, d = i % X::D, idx = index_of(d) * A4_HEADS + h, ml = X::D * A4_HEADS + 2 * h;
+                float M = -INFINITY, L = 0.f, o = 0.f;
+                for (int c = c0; c <= c1; ++c) M = fmaxf(M, __ldcg(part_of(c) + ml));
+                for (int c = c0; c <= c1; ++c) {
+                    const float lc = __ldcg(part_of(c) + ml + 1);
+                    if (lc == 0.f) continue;
+                    const float x = exp2f(__ldcg(part_of(c) + ml) - M);
+                    L += lc * x;
+                    o += __ldcg(part_of(c) + idx) * x;
+                }
+                store(h, d, L == 0.f ? 0.f : o / L);
+            }
+            if (tid == 0) A.counters[c0] = 0;      // ready for the next launch
+        }
+        __syncthreads();
+    }
+}
+
+// Workspace: the status word, the arrival counters (one per CTA) from byte 256, and from 128 KiB the partial results.
+constexpr size_t A4_COUNTERS_OFF = 256, A4_PARTS_OFF = 128 * 1024;
+static int attn4_max_ctas() { return sm_count() * 4; }
+static size_t attn4_ws_bytes(int d) { return A4_PARTS_OFF + (size_t)attn4_max_ctas() * 2 * (d * A4_HEADS + 16) * sizeof(float); }
+
+template <int NB, int NG>
+static int attn4_launch_as(const char *name, const Attn4Args &A, long max_units, cudaStream_t st) {
+    using X = A4<NB, NG>;
+    static OncePerDevice once;
+    cudaError_t e = once.run([&] { return cudaFuncSetAttribute(attn4_kernel<NB, NG>, cudaFuncAttributeMaxDynamicSharedMemorySize, X::SMEM); });
+    if (e != cudaSuccess) return fail((int)e, "%s: shared memory %d: %s", name, X::SMEM, cudaGetErrorString(e));
+    const long wave = (long)sm_count() * X::CTAS;
+    launch_kernel(attn4_kernel<NB, NG>, dim3((unsigned)(max_units < wave ? max_units : wave)), dim3(A4_THREADS), X::SMEM, st, A);
+    return launch_status(name);
+}
+
 static int attn4_launch(const char *name, const void *q, const Kv4Cache &C, bool paged, const int32_t *lens, void *out, int batch, int hq,
-                        float scale, void *ws, size_t ws_bytes, bool own_ws, b200k_stream stream) {
+                        float scale, bool bf16, bool out_kperm, void *ws, size_t ws_bytes, bool own_ws, b200k_stream stream) {
     B200K_REQUIRE(q && lens && out, B200K_E_NULL, "%s: NULL pointer", name);
     int rc = kv4_check(name, C, batch, paged);
     if (rc) return rc;
@@ -118,11 +582,36 @@ static int attn4_launch(const char *name, const void *q, const Kv4Cache &C, bool
         rc = default_workspace(&ws, &ws_bytes);
         if (rc) return rc;
     }
-    B200K_REQUIRE(ws && aligned16(ws) && ws_bytes >= ATTN4_WS_BYTES, B200K_E_WORKSPACE, "%s: workspace %zu bytes, need %zu", name, ws_bytes, ATTN4_WS_BYTES);
+    B200K_REQUIRE(ws && aligned16(ws) && ws_bytes >= attn4_ws_bytes(C.d), B200K_E_WORKSPACE, "%s: workspace %zu bytes, need %zu (16-byte aligned)", name,
+                  ws_bytes, attn4_ws_bytes(C.d));
     Attn4Args A = {};
-    A.q = q; A.out = out; A.lens = lens; A.C = C; A.hq = hq; A.scale = scale; A.status = (int *)ws;
-    launch_kernel(attn4_kernel<T>, dim3(hq, batch), dim3(128), 0, to_stream(stream), A);
-    return launch_status(name);
+    A.q = q; A.out = out; A.lens = lens; A.C = C;
+    A.block_magic = ~0ull / (unsigned)C.block_size + 1;      // used for multiples of 16 only
+    A.batch = batch; A.hq = hq; A.head_blocks = ceil_div(hq / C.heads, A4_HEADS);
+    A.bf16 = bf16; A.out_kperm = out_kperm;
+    A.scale_log2e = scale * 1.4426950408889634f;
+    A.status = (int *)ws;
+    A.counters = (int *)((unsigned char *)ws + A4_COUNTERS_OFF);
+    A.parts = (float *)((unsigned char *)ws + A4_PARTS_OFF);
+    const long max_units = (long)batch * C.heads * A.head_blocks * (((long)C.capacity + A4_UNIT - 1) / A4_UNIT);
+    cudaStream_t st = to_stream(stream);
+    switch (C.d / 32 * 1000 + C.d / C.g) {
+        case 1001: return attn4_launch_as<1, 1>(name, A, max_units, st);
+        case 2001: return attn4_launch_as<2, 1>(name, A, max_units, st);
+        case 2002: return attn4_launch_as<2, 2>(name, A, max_units, st);
+        case 3003: return attn4_launch_as<3, 3>(name, A, max_units, st);
+        case 4001: return attn4_launch_as<4, 1>(name, A, max_units, st);
+        case 4002: return attn4_launch_as<4, 2>(name, A, max_units, st);
+        case 4004: return attn4_launch_as<4, 4>(name, A, max_units, st);
+        case 5005: return attn4_launch_as<5, 5>(name, A, max_units, st);
+        case 6003: return attn4_launch_as<6, 3>(name, A, max_units, st);
+        case 6006: return attn4_launch_as<6, 6>(name, A, max_units, st);
+        case 7007: return attn4_launch_as<7, 7>(name, A, max_units, st);
+        case 8002: return attn4_launch_as<8, 2>(name, A, max_units, st);
+        case 8004: return attn4_launch_as<8, 4>(name, A, max_units, st);
+        case 8008: return attn4_launch_as<8, 8>(name, A, max_units, st);
+    }
+    return fail(B200K_E_SHAPE, "%s: head_dim %d, group_size %d", name, C.d, C.g);
 }
 
 }  // namespace b200k
@@ -131,18 +620,18 @@ using namespace b200k;
 
 extern "C" size_t b200k_attention_int4_workspace_bytes(int batch, int num_q_heads, int num_kv_heads, int head_dim) {
     if (batch <= 0 || num_q_heads <= 0 || num_kv_heads <= 0 || num_q_heads % num_kv_heads || head_dim <= 0) return 0;
-    return ATTN4_WS_BYTES;
+    return attn4_ws_bytes(head_dim);
 }
 
-#define ATTN4_ENTRIES(SUF, ABI, T)                                                                                                          \
+#define ATTN4_ENTRIES(SUF, ABI, IS_BF16)                                                                                                         \
     extern "C" int batched_decode_attention_hm_int4_##SUF##_ws(const ABI *q, const int32_t *k_codes, const b200k_half *k_params,             \
                                                                const int32_t *v_codes, const b200k_half *v_params,                          \
                                                                const int32_t *context_lens, ABI *output, int batch_size, int num_q_heads,   \
                                                                int num_kv_heads, int head_dim, int group_size, int max_len, float scale,    \
                                                                void *workspace, size_t workspace_bytes, b200k_stream stream) {              \
-        return attn4_launch<T>("batched_decode_attention_hm_int4_" #SUF, q,                                                                 \
+        return attn4_launch("batched_decode_attention_hm_int4_" #SUF, q,                                                                 \
                                kv4_cache(k_codes, k_params, v_codes, v_params, num_kv_heads, head_dim, group_size, max_len), false,         \
-                               context_lens, output, batch_size, num_q_heads, scale, workspace, workspace_bytes, workspace == nullptr, stream); \
+                               context_lens, output, batch_size, num_q_heads, scale, IS_BF16, false, workspace, workspace_bytes, workspace == nullptr, stream); \
     }                                                                                                                                       \
     extern "C" int batched_decode_attention_hm_int4_##SUF(const ABI *q, const int32_t *k_codes, const b200k_half *k_params,                  \
                                                           const int32_t *v_codes, const b200k_half *v_params, const int32_t *context_lens,  \
@@ -156,10 +645,10 @@ extern "C" size_t b200k_attention_int4_workspace_bytes(int batch, int num_q_head
         const int32_t *block_table, const int32_t *context_lens, ABI *output, int batch_size, int num_q_heads, int num_kv_heads,            \
         int head_dim, int group_size, int block_size, int num_blocks, int max_blocks_per_seq, float scale, void *workspace,                 \
         size_t workspace_bytes, b200k_stream stream) {                                                                                      \
-        return attn4_launch<T>("batched_decode_attention_paged_int4_" #SUF, q,                                                              \
+        return attn4_launch("batched_decode_attention_paged_int4_" #SUF, q,                                                              \
                                kv4_pool(k_codes, k_params, v_codes, v_params, block_table, num_kv_heads, head_dim, group_size, block_size,  \
                                         num_blocks, max_blocks_per_seq), true, context_lens, output, batch_size, num_q_heads, scale,        \
-                               workspace, workspace_bytes, workspace == nullptr, stream);                                                   \
+                               IS_BF16, false, workspace, workspace_bytes, workspace == nullptr, stream);                                                   \
     }                                                                                                                                       \
     extern "C" int batched_decode_attention_paged_int4_##SUF(                                                                               \
         const ABI *q, const int32_t *k_codes, const b200k_half *k_params, const int32_t *v_codes, const b200k_half *v_params,               \
@@ -170,5 +659,5 @@ extern "C" size_t b200k_attention_int4_workspace_bytes(int batch, int num_q_head
                                                               num_blocks, max_blocks_per_seq, scale, nullptr, 0, stream);                   \
     }
 
-ATTN4_ENTRIES(f16, b200k_half, __half)
-ATTN4_ENTRIES(bf16, b200k_bf16, __nv_bfloat16)
+ATTN4_ENTRIES(f16, b200k_half, false)
+ATTN4_ENTRIES(bf16, b200k_bf16, true)
