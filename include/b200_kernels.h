@@ -520,7 +520,7 @@ int rope_kv_append_hm_f16(const b200k_half *qkv, const float *cos_table,
  *   head-major   codes [batch, heads, max_len, head_dim/8] int32, params [batch, heads, max_len, head_dim/group_size, 2] fp16
  *   paged pool   codes [num_blocks, heads, block_size, head_dim/8], params [num_blocks, heads, block_size, head_dim/group_size, 2];
  *                position p of sequence b is slot p % block_size of block block_table[b, p / block_size], block_table
- *                [batch, max_blocks_per_seq]: a sequence holds up to max_blocks_per_seq * block_size positions (below 2^31)
+ *                [batch, max_blocks_per_seq]: a sequence holds up to max_blocks_per_seq * block_size positions (at most 2^30, as max_len)
  * At head_dim 128 and group_size 64 a row takes 72 bytes where fp16 takes 256.  All tensors are contiguous, 16-byte aligned, and
  * live on the current device; batch up to 65535.  Activations are fp16 or bf16, params fp16 with either.  Positions outside the
  * cache and blocks outside the pool are skipped and reported in the status word (bits 2 and 3). */

@@ -86,7 +86,7 @@ NULL, SHAPE, ALIGN, WORKSPACE = -1, -2, -3, -4
         (dict(kc=None), NULL), (dict(kp=None), NULL), (dict(vc=None), NULL), (dict(vp=None), NULL), (dict(heads=0), SHAPE), (dict(d=0), SHAPE),
         (dict(d=48), SHAPE), (dict(d=288), SHAPE), (dict(d=96), SHAPE), (dict(g=16), SHAPE), (dict(g=0), SHAPE), (dict(g=256, d=256), SHAPE),
         (dict(b=-1), SHAPE), (dict(b=65536), SHAPE), (dict(kc=PTR + 4), ALIGN), (dict(vp=PTR + 8), ALIGN)]],
-    *[(f, kw, SHAPE) for f in (_append, _rope, _read, _attn) for kw in (dict(ml=0), dict(ml=-5))],
+    *[(f, kw, SHAPE) for f in (_append, _rope, _read, _attn) for kw in (dict(ml=0), dict(ml=-5), dict(ml=2 ** 30 + 1))],
     *[(f, kw, code) for f in (_append_paged, _attn_paged) for kw, code in [
         (dict(table=None), NULL), (dict(bs=0), SHAPE), (dict(nb=0), SHAPE), (dict(mb=0), SHAPE), (dict(bs=1 << 16, mb=1 << 15), SHAPE)]],
     *[(f, kw, code) for f in (_append, _append_paged) for kw, code in [

@@ -25,6 +25,7 @@ namespace b200k {
 
 constexpr int A4_WARPS = 4, A4_THREADS = 32 * A4_WARPS, A4_STAGES = 4;
 constexpr int A4_TILE = 16, A4_UNIT = A4_WARPS * A4_TILE;      // positions of a warp's tile, of a unit of work
+constexpr int A4_MAX_CTAS = 640;                               // more than four CTAs on every SM
 constexpr int A4_HEADS = 8;                                    // columns of one MMA
 constexpr float A4_LAZY = 6.f;        // the running maximum moves when a score passes it by 2^6: probabilities stay below 2^6
 constexpr float A4_TOP = 512.f;       // 2^e times the largest value scale is set to [2^2, 2^3) and set again when it passes 2^9
@@ -57,7 +58,8 @@ struct A4 {
     static constexpr int CTAS = NB <= 4 ? 4 : NB <= 6 ? 3 : 2;
     static constexpr int RING = A4_WARPS * A4_STAGES * STAGE;
     static constexpr int JOIN = A4_WARPS * D * A4_HEADS * 4;  // the warps' results, over the ring
-    static constexpr int SMEM = (RING > JOIN ? RING : JOIN) + 16;
+    static constexpr int JOIN2 = JOIN + A4_MAX_CTAS * A4_HEADS * 4;      // and the weights of the CTAs' results behind them
+    static constexpr int SMEM = RING > JOIN2 ? RING : JOIN2;
     // 16-byte chunk of a row in shared memory is chunk ^ swizzle(position): the K loads of a quarter warp (two rows of
     // opposite parity) and the V loads of a half warp (positions 0-3 or 4-7) then meet no bank twice
     __device__ static int swizzle(int pos) { return NB == 4 ? pos & 2 : NB == 8 ? ((pos & 3) << 1) | (pos & 1) : 0; }
@@ -192,6 +194,11 @@ attn4_kernel(const Attn4Args A) {
     }
 
     unsigned char *ring = smem + warp * A4_STAGES * X::STAGE;
+    const uint32_t ring32 = smem_u32(ring);
+    // where this lane's first 16-byte piece and its row of params go in a stage; lanes 0-15 copy K params, 16-31 V params
+    const uint32_t dst_codes = (lane / NB) * X::ROW + ((lane % NB) ^ X::swizzle(lane / NB)) * 16;
+    const uint32_t dst_params = 2 * A4_TILE * X::ROW + lane * X::PROW;
+    const unsigned char *params = (const unsigned char *)(lane < 16 ? C.k_params : C.v_params) + (lane & 15) * X::PROW;
     const int kpos0 = a4_pos(r);                               // this lane's K rows: kpos0 and kpos0 + 8
     const int vpos0 = t, vpos1 = 4 + (t ^ 1);                  // its V rows: these and + 8
 
@@ -210,44 +217,58 @@ attn4_kernel(const Attn4Args A) {
         const int heads = min(A4_HEADS, (kvh + 1) * gqa - h0);
         at = item_start + u1;
 
-        // tile i of this warp -> stage i % STAGES
+        // tile i of this warp -> stage i % STAGES: 16 neighbouring rows are one linear piece of the cache, so a tile that is
+        // whole and lies in one block takes nothing but copies at fixed distances
+        const bool one = !C.block_table || C.block_size % A4_TILE == 0;
+        long next = ((long)b * C.heads + kvh) * C.capacity + u0 * A4_UNIT + warp * A4_TILE;      // head-major: row of the next tile
         auto issue = [&](int i) {
             const int p0 = (u0 + i) * A4_UNIT + warp * A4_TILE;
-            unsigned char *st = ring + (i % A4_STAGES) * X::STAGE;
-            const bool one = !C.block_table || C.block_size % A4_TILE == 0;      // the tile lies in one block: its rows are neighbours
-            long first = 0;
-            if (!C.block_table) {
-                first = ((long)b * C.heads + kvh) * C.capacity + p0;
-            } else if (one && p0 < len) {
+            const uint32_t st = ring32 + (i % A4_STAGES) * X::STAGE;
+            long first = next;
+            next += A4_UNIT;
+            if (C.block_table && one && p0 < len) {
                 const int lb = (int)__umul64hi((unsigned long long)p0, A.block_magic);
                 const int blk = C.block_table[(long)b * C.max_blocks + lb];
                 first = (unsigned)blk < (unsigned)C.num_blocks ? ((long)blk * C.heads + kvh) * C.block_size + (p0 - lb * C.block_size) : -1;
             }
-            auto row_of = [&](int row) {           // -1: behind the context, or in a block that the pool does not have
-                if (p0 + row >= len) return -1l;
-                if (one) return first < 0 ? -1l : first + row;
-                return kv4_row(C, b, kvh, p0 + row);
-            };
+            if (one && p0 + A4_TILE <= len && first >= 0) {
+                const unsigned char *k = (const unsigned char *)C.k_codes + first * X::ROW + lane * 16;
+                const unsigned char *v = (const unsigned char *)C.v_codes + first * X::ROW + lane * 16;
 #pragma unroll
-            for (int c = lane; c < A4_TILE * NB; c += 32) {
-                const int row = c / NB, part = c % NB;
-                const long rr = row_of(row);
-                const uint32_t dst = smem_u32(st + row * X::ROW + (part ^ X::swizzle(row)) * 16);
-                const long off = max(rr, 0l) * X::ROW + part * 16;
-                a4_copy<16>(dst, (const unsigned char *)C.k_codes + off, rr < 0 ? 0 : 16);
-                a4_copy<16>(dst + A4_TILE * X::ROW, (const unsigned char *)C.v_codes + off, rr < 0 ? 0 : 16);
-            }
-            const int row = lane & 15;
-            const long rr = row_of(row);
+                for (int c = 0; c < NB; c += 2)
+                    if (c + 1 < NB || lane < 16) {
+                        a4_copy<16>(st + dst_codes + c * 256, k + c * 256, 16);
+                        a4_copy<16>(st + dst_codes + A4_TILE * X::ROW + c * 256, v + c * 256, 16);
+                    }
+                const unsigned char *p = params + first * X::PROW;
 #pragma unroll
-            for (int c = 0; c < X::PROW; c += X::PCOPY)
-                a4_copy<X::PCOPY>(smem_u32(st + 2 * A4_TILE * X::ROW + lane * X::PROW + c),
-                                  (const unsigned char *)(lane < 16 ? C.k_params : C.v_params) + max(rr, 0l) * X::PROW + c, rr < 0 ? 0 : X::PCOPY);
-            const unsigned valid = __ballot_sync(0xffffffffu, rr >= 0);
-            if (lane == 0) {
-                *reinterpret_cast<uint32_t *>(st + X::STAGE - 16) = valid;
-                const int rows = min(A4_TILE, len - p0);
-                if (rows > 0 && __popc(valid & 0xffffu) != rows) atomicOr(A.status, KV4_BAD_BLOCK);
+                for (int c = 0; c < X::PROW; c += X::PCOPY) a4_copy<X::PCOPY>(st + dst_params + c, p + c, X::PCOPY);
+                if (C.block_table && lane == 0) *reinterpret_cast<uint32_t *>(ring + (i % A4_STAGES) * X::STAGE + X::STAGE - 16) = 0xffffu;
+            } else {
+                auto row_of = [&](int row) {           // -1: behind the context, or in a block that the pool does not have
+                    if (p0 + row >= len) return -1l;
+                    if (one) return first < 0 ? -1l : first + row;
+                    return kv4_row(C, b, kvh, p0 + row);
+                };
+#pragma unroll 1
+                for (int c = lane; c < A4_TILE * NB; c += 32) {
+                    const long row = row_of(c / NB);
+                    const long off = max(row, 0l) * X::ROW + (c % NB) * 16;
+                    const uint32_t dst = st + dst_codes + (c - lane) * 16;
+                    a4_copy<16>(dst, (const unsigned char *)C.k_codes + off, row < 0 ? 0 : 16);
+                    a4_copy<16>(dst + A4_TILE * X::ROW, (const unsigned char *)C.v_codes + off, row < 0 ? 0 : 16);
+                }
+                const long row = row_of(lane & 15);
+#pragma unroll
+                for (int c = 0; c < X::PROW; c += X::PCOPY)
+                    a4_copy<X::PCOPY>(st + dst_params + c, (const unsigned char *)(lane < 16 ? C.k_params : C.v_params) + max(row, 0l) * X::PROW + c,
+                                      row < 0 ? 0 : X::PCOPY);
+                const unsigned valid = __ballot_sync(0xffffffffu, row >= 0) & 0xffffu;
+                if (lane == 0) {
+                    *reinterpret_cast<uint32_t *>(ring + (i % A4_STAGES) * X::STAGE + X::STAGE - 16) = valid;
+                    const int rows = min(A4_TILE, len - p0);
+                    if (rows > 0 && __popc(valid) != rows) atomicOr(A.status, KV4_BAD_BLOCK);
+                }
             }
             asm volatile("cp.async.commit_group;" ::: "memory");
         };
@@ -264,20 +285,32 @@ attn4_kernel(const Attn4Args A) {
         uint32_t qf[4 * NB];
         float qsum[NG][2], fac[2];             // of heads 2t and 2t + 1: sum of q over a group, and what a score is multiplied by
         {
-            const uint16_t *qrow = (const uint16_t *)A.q + ((long)b * A.hq + h0 + r) * X::D;
-            auto ld = [&](int d) {
-                const uint16_t x = r < heads ? qrow[d] : (uint16_t)0;
-                return A.bf16 ? __uint_as_float((uint32_t)x << 16) : __half2float(__ushort_as_half(x));
+            // word i's dims: 4 + 4 (two blocks), or 8 in a row (one block)
+            uint32_t raw[NB][4];
+            const uint16_t *qrow = (const uint16_t *)A.q + ((long)b * A.hq + h0 + (r < heads ? r : 0)) * X::D;
+#pragma unroll
+            for (int i = 0; i < NB; ++i) {
+                int lo, hi;
+                a4_kdims<NB, X::PURE>(i, 0, t, lo, hi);
+                if constexpr (X::PURE) {
+                    const uint4 u = *reinterpret_cast<const uint4 *>(qrow + lo);
+                    raw[i][0] = u.x; raw[i][1] = u.y; raw[i][2] = u.z; raw[i][3] = u.w;
+                } else {
+                    const uint2 u = *reinterpret_cast<const uint2 *>(qrow + lo), w = *reinterpret_cast<const uint2 *>(qrow + hi);
+                    raw[i][0] = u.x; raw[i][1] = u.y; raw[i][2] = w.x; raw[i][3] = w.y;
+                }
+            }
+            auto pick = [&](int i, int n) {      // n 0-3: the low half's dims, 4-7: the high half's
+                const uint32_t x = r < heads ? raw[i][n >> 1] : 0u;
+                if (A.bf16) return __uint_as_float(n & 1 ? x & 0xffff0000u : x << 16);
+                const float2 f = h2_to_f2(x);
+                return n & 1 ? f.y : f.x;
             };
             float big = 0.f;
 #pragma unroll
             for (int i = 0; i < NB; ++i)
 #pragma unroll
-                for (int nn = 0; nn < 4; ++nn) {
-                    int lo, hi;
-                    a4_kdims<NB, X::PURE>(i, nn, t, lo, hi);
-                    big = fmaxf(big, fmaxf(fabsf(ld(lo)), fabsf(ld(hi))));
-                }
+                for (int nn = 0; nn < 8; ++nn) big = fmaxf(big, fabsf(pick(i, nn)));
             big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
             big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
             const int k = min(14 - ((int)(__float_as_uint(big) >> 23) - 127), 126);
@@ -287,9 +320,7 @@ attn4_kernel(const Attn4Args A) {
             for (int i = 0; i < NB; ++i)
 #pragma unroll
                 for (int nn = 0; nn < 4; ++nn) {
-                    int lo, hi;
-                    a4_kdims<NB, X::PURE>(i, nn, t, lo, hi);
-                    const float a = ld(lo) * up, c = ld(hi) * up;
+                    const float a = pick(i, nn) * up, c = pick(i, nn + 4) * up;
                     sum[a4_kgroup<NB, NG, X::PURE>(i)] += a + c;
                     qf[4 * i + nn] = (nn & 1) ? f2_to_h2(a * 0.0625f, c * 0.0625f) : f2_to_h2(a, c);
                 }
@@ -327,7 +358,8 @@ attn4_kernel(const Attn4Args A) {
             else asm volatile("cp.async.commit_group;" ::: "memory");
             const unsigned char *st = ring + (i % A4_STAGES) * X::STAGE;
             const unsigned char *sk = st, *sv = st + A4_TILE * X::ROW, *pk = sv + A4_TILE * X::ROW, *pv = pk + A4_TILE * X::PROW;
-            const uint32_t valid = *reinterpret_cast<const uint32_t *>(st + X::STAGE - 16) & 0xffffu;
+            uint32_t valid = 0xffffu;
+            if (C.block_table || (u0 + i) * A4_UNIT + (warp + 1) * A4_TILE > len) valid = *reinterpret_cast<const uint32_t *>(st + X::STAGE - 16);
 
             // scores: rows r and r + 8 are positions kpos0 and kpos0 + 8, columns heads 2t and 2t + 1
             float s[4] = {0.f, 0.f, 0.f, 0.f};
@@ -534,19 +566,56 @@ attn4_kernel(const Attn4Args A) {
         __syncthreads();
         if (sm_last) {
             __threadfence();
-            auto part_of = [&](int c) { return A.parts + ((long)c * 2 + (c == c0)) * X::PART; };
-            for (int i = tid; i < heads * X::D; i += A4_THREADS) {
-                const int h = i / X::D, d = i % X::D, idx = index_of(d) * A4_HEADS + h, ml = X::D * A4_HEADS + 2 * h;
-                float M = -INFINITY, L = 0.f, o = 0.f;
-                for (int c = c0; c <= c1; ++c) M = fmaxf(M, __ldcg(part_of(c) + ml));
-                for (int c = c0; c <= c1; ++c) {
-                    const float lc = __ldcg(part_of(c) + ml + 1);
-                    if (lc == 0.f) continue;
-                    const float x = exp2f(__ldcg(part_of(c) + ml) - M);
-                    L += lc * x;
-                    o += __ldcg(part_of(c) + idx) * x;
+            // weights 2^(m_c - M) of the parts to shared memory (over the ring), then the parts dealt out to the warps, each lane
+            // with several loads in flight, then the warps' sums in order
+            const int parts = c1 - c0 + 1;
+            float *wt = reinterpret_cast<float *>(smem) + A4_WARPS * X::D * A4_HEADS;      // [part][head]
+            auto part_of = [&](int c) { return A.parts + ((long)(c0 + c) * 2 + (c == 0)) * X::PART; };
+            const int h = tid & 7;
+            float M = -INFINITY, L = 0.f;
+            for (int c = tid >> 3; c < parts; c += A4_THREADS / 8) {
+                const float2 ml = __ldcg(reinterpret_cast<const float2 *>(part_of(c) + X::D * A4_HEADS) + h);
+                if (ml.y != 0.f) M = fmaxf(M, ml.x);
+            }
+            M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, 8));
+            M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, 16));
+            if (lane < 8) sm_ref[warp][lane] = M;
+            __syncthreads();
+#pragma unroll
+            for (int w = 0; w < A4_WARPS; ++w) M = fmaxf(M, sm_ref[w][h]);
+            for (int c = tid >> 3; c < parts; c += A4_THREADS / 8) {
+                const float2 ml = __ldcg(reinterpret_cast<const float2 *>(part_of(c) + X::D * A4_HEADS) + h);
+                const float x = ml.y == 0.f ? 0.f : exp2f(ml.x - M);
+                wt[c * A4_HEADS + h] = x;
+                L += ml.y * x;
+            }
+            L += __shfl_xor_sync(0xffffffffu, L, 8);
+            L += __shfl_xor_sync(0xffffffffu, L, 16);
+            if (lane < 8) sm_l[warp][lane] = L;
+            __syncthreads();
+            if (tid < A4_HEADS) sm_sum[tid] = sm_l[0][tid] + sm_l[1][tid] + sm_l[2][tid] + sm_l[3][tid];
+            const int quads = heads <= 4 ? 1 : 2;            // groups of four heads that exist
+            for (int i = lane; i < X::D * quads; i += 32) {
+                const int at4 = (i / quads) * 2 + i % quads;  // float4 of a part: (m-tile row, four heads)
+                float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+                for (int c = warp; c < parts; c += A4_WARPS) {
+                    const float4 x = __ldcg(reinterpret_cast<const float4 *>(part_of(c)) + at4);
+                    const float4 w = *reinterpret_cast<const float4 *>(wt + c * A4_HEADS + 4 * (at4 & 1));
+                    o.x += w.x == 0.f ? 0.f : w.x * x.x;
+                    o.y += w.y == 0.f ? 0.f : w.y * x.y;
+                    o.z += w.z == 0.f ? 0.f : w.z * x.z;
+                    o.w += w.w == 0.f ? 0.f : w.w * x.w;
                 }
-                store(h, d, L == 0.f ? 0.f : o / L);
+                reinterpret_cast<float4 *>(so + warp * X::D * A4_HEADS)[at4] = o;
+            }
+            __syncthreads();
+            for (int i = tid; i < heads * X::D; i += A4_THREADS) {
+                const int hh = i / X::D, d = i % X::D, idx = index_of(d) * A4_HEADS + hh;
+                float o = 0.f;
+#pragma unroll
+                for (int w = 0; w < A4_WARPS; ++w) o += so[w * X::D * A4_HEADS + idx];
+                store(hh, d, sm_sum[hh] == 0.f ? 0.f : o / sm_sum[hh]);
             }
             if (tid == 0) A.counters[c0] = 0;      // ready for the next launch
         }
@@ -556,8 +625,7 @@ attn4_kernel(const Attn4Args A) {
 
 // Workspace: the status word, the arrival counters (one per CTA) from byte 256, and from 128 KiB the partial results.
 constexpr size_t A4_COUNTERS_OFF = 256, A4_PARTS_OFF = 128 * 1024;
-static int attn4_max_ctas() { return sm_count() * 4; }
-static size_t attn4_ws_bytes(int d) { return A4_PARTS_OFF + (size_t)attn4_max_ctas() * 2 * (d * A4_HEADS + 16) * sizeof(float); }
+static size_t attn4_ws_bytes(int d) { return A4_PARTS_OFF + (size_t)A4_MAX_CTAS * 2 * (d * A4_HEADS + 16) * sizeof(float); }
 
 template <int NB, int NG>
 static int attn4_launch_as(const char *name, const Attn4Args &A, long max_units, cudaStream_t st) {
@@ -565,7 +633,7 @@ static int attn4_launch_as(const char *name, const Attn4Args &A, long max_units,
     static OncePerDevice once;
     cudaError_t e = once.run([&] { return cudaFuncSetAttribute(attn4_kernel<NB, NG>, cudaFuncAttributeMaxDynamicSharedMemorySize, X::SMEM); });
     if (e != cudaSuccess) return fail((int)e, "%s: shared memory %d: %s", name, X::SMEM, cudaGetErrorString(e));
-    const long wave = (long)sm_count() * X::CTAS;
+    const long wave = min((long)sm_count() * X::CTAS, (long)A4_MAX_CTAS);
     launch_kernel(attn4_kernel<NB, NG>, dim3((unsigned)(max_units < wave ? max_units : wave)), dim3(A4_THREADS), X::SMEM, st, A);
     return launch_status(name);
 }

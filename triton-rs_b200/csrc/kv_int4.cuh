@@ -21,6 +21,7 @@
 namespace b200k {
 
 constexpr float KV4_LIMIT = 65440.f;
+constexpr long KV4_MAX_LEN = 1l << 30;      // positions of a sequence: sums of two of them stay in 32 bits
 constexpr int KV4_BAD_POSITION = 4, KV4_BAD_BLOCK = 8;   // bits of the status word
 
 struct Kv4Cache {
@@ -49,10 +50,10 @@ static inline int kv4_check(const char *name, const Kv4Cache &C, int batch, bool
     B200K_REQUIRE((C.g == 32 || C.g == 64 || C.g == 128) && C.d % C.g == 0, B200K_E_SHAPE,
                   "%s: group_size %d (32, 64 or 128, dividing head_dim %d)", name, C.g, C.d);
     if (paged)
-        B200K_REQUIRE(C.block_size > 0 && C.num_blocks > 0 && C.max_blocks > 0 && (long)C.block_size * C.max_blocks < (1l << 31), B200K_E_SHAPE,
+        B200K_REQUIRE(C.block_size > 0 && C.num_blocks > 0 && C.max_blocks > 0 && (long)C.block_size * C.max_blocks <= KV4_MAX_LEN, B200K_E_SHAPE,
                       "%s: block_size %d, num_blocks %d, max_blocks_per_seq %d", name, C.block_size, C.num_blocks, C.max_blocks);
     else
-        B200K_REQUIRE(C.capacity > 0, B200K_E_SHAPE, "%s: max_len %d", name, C.capacity);
+        B200K_REQUIRE(C.capacity > 0 && C.capacity <= KV4_MAX_LEN, B200K_E_SHAPE, "%s: max_len %d", name, C.capacity);
     B200K_REQUIRE(aligned16(C.k_codes) && aligned16(C.v_codes) && aligned16(C.k_params) && aligned16(C.v_params), B200K_E_ALIGN,
                   "%s: codes and params must be 16-byte aligned", name);
     return 0;
@@ -69,7 +70,7 @@ static inline Kv4Cache kv4_pool(const int32_t *kc, const b200k_half *kp, const i
                                 int g, int block_size, int num_blocks, int max_blocks) {
     Kv4Cache C = kv4_cache(kc, kp, vc, vp, heads, d, g, 0);
     C.block_table = table; C.block_size = block_size; C.num_blocks = num_blocks; C.max_blocks = max_blocks;
-    C.capacity = (int)min((long)block_size * max_blocks, (1l << 31) - 1);
+    C.capacity = (int)min((long)block_size * max_blocks, KV4_MAX_LEN);
     return C;
 }
 
