@@ -72,6 +72,11 @@ __device__ __forceinline__ void a4_mma(float (&d)[4], uint32_t a0, uint32_t a1, 
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+__device__ __forceinline__ void a4_mma0(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {   // sum from 0
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+                 : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
 __device__ __forceinline__ uint32_t a4_transpose(uint32_t a) {
     uint32_t d;
     asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
@@ -90,33 +95,48 @@ __device__ __forceinline__ void a4_copy(uint32_t dst, const void *src, int bytes
         asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(BYTES), "r"(bytes) : "memory");
 }
 template <int N>
-__device__ __forceinline__ void a4_lds(uint32_t (&w)[N], const unsigned char *p) {    // N words, as aligned as their number allows
+__device__ __forceinline__ void a4_lds(uint32_t *w, uint32_t at) {    // N words of shared memory, as aligned as their number allows
     if constexpr (N % 4 == 0) {
 #pragma unroll
-        for (int i = 0; i < N; i += 4) {
-            const uint4 u = *reinterpret_cast<const uint4 *>(p + 4 * i);
-            w[i] = u.x; w[i + 1] = u.y; w[i + 2] = u.z; w[i + 3] = u.w;
-        }
+        for (int i = 0; i < N; i += 4)
+            asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(w[i]), "=r"(w[i + 1]), "=r"(w[i + 2]), "=r"(w[i + 3]) : "r"(at + 4 * i) : "memory");
     } else if constexpr (N % 2 == 0) {
 #pragma unroll
-        for (int i = 0; i < N; i += 2) {
-            const uint2 u = *reinterpret_cast<const uint2 *>(p + 4 * i);
-            w[i] = u.x; w[i + 1] = u.y;
-        }
+        for (int i = 0; i < N; i += 2) asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(w[i]), "=r"(w[i + 1]) : "r"(at + 4 * i) : "memory");
     } else {
 #pragma unroll
-        for (int i = 0; i < N; ++i) w[i] = *reinterpret_cast<const uint32_t *>(p + 4 * i);
+        for (int i = 0; i < N; ++i) asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w[i]) : "r"(at + 4 * i) : "memory");
     }
 }
+__device__ __forceinline__ uint32_t a4_lds16(uint32_t at) {
+    uint16_t h;
+    asm volatile("ld.shared.u16 %0, [%1];" : "=h"(h) : "r"(at) : "memory");
+    return h;
+}
 template <int NG>
-__device__ __forceinline__ void a4_params(float (&s)[NG], float (&z)[NG], const unsigned char *p) {
+__device__ __forceinline__ void a4_params(float (&s)[NG], float (&z)[NG], uint32_t at) {
     uint32_t w[NG];
-    a4_lds<NG>(w, p);
+    a4_lds<NG>(w, at);
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
         const float2 f = h2_to_f2(w[g]);
         s[g] = f.x; z[g] = f.y;
     }
+}
+// a value that is to be kept in its register: not to be worked out again wherever it is used
+__device__ __forceinline__ uint32_t a4_keep(uint32_t x) {
+    asm volatile("" : "+r"(x));
+    return x;
+}
+
+// The eight codes of a word as four operand registers: nibbles 0 and 2 of both halves as c 2^-24, 1 and 3 as c 2^-20.  Four
+// integer instructions and a subtraction (exact) on the other pipe: the integer one runs at half rate and is the busiest here.
+__device__ __forceinline__ void a4_codes(uint32_t x, uint32_t &n0, uint32_t &n1, uint32_t &n2, uint32_t &n3) {
+    const uint32_t y = __byte_perm(x, 0, 0x4341);
+    n0 = x & 0x000f000fu;
+    n1 = x & 0x00f000f0u;
+    n3 = y & 0x00f000f0u;
+    asm("sub.f16x2 %0, %1, %2;" : "=r"(n2) : "r"(y), "r"(n3));
 }
 
 // Lane t of a K row holds units (2t, j) and (2t + 1, j), j = 0 .. NB-1, in this order, in NB words.  Word i of its operand: where
@@ -145,10 +165,10 @@ __device__ __forceinline__ constexpr int a4_kgroup(int i) { return PURE ? i : (i
 
 template <int NB, int NG>
 __global__ void __launch_bounds__(A4_THREADS, A4<NB, NG>::CTAS)
-attn4_kernel(const Attn4Args A) {
+attn4_kernel(const __grid_constant__ Attn4Args A) {
     using X = A4<NB, NG>;
-    extern __shared__ __align__(16) unsigned char smem[];
-    __shared__ float sm_ref[A4_WARPS][A4_HEADS], sm_l[A4_WARPS][A4_HEADS], sm_w[A4_WARPS][A4_HEADS], sm_top[A4_HEADS], sm_sum[A4_HEADS];
+    extern __shared__ __align__(128) unsigned char smem[];
+    __shared__ float sm_ref[A4_WARPS][A4_HEADS], sm_l[A4_WARPS][A4_HEADS], sm_top[A4_HEADS], sm_sum[A4_HEADS];
     __shared__ int sm_last;
     const Kv4Cache &C = A.C;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, r = lane >> 2, t = lane & 3;
@@ -193,14 +213,18 @@ attn4_kernel(const Attn4Args A) {
         start += __shfl_sync(0xffffffffu, upto, 31);
     }
 
-    unsigned char *ring = smem + warp * A4_STAGES * X::STAGE;
-    const uint32_t ring32 = smem_u32(ring);
-    // where this lane's first 16-byte piece and its row of params go in a stage; lanes 0-15 copy K params, 16-31 V params
-    const uint32_t dst_codes = (lane / NB) * X::ROW + ((lane % NB) ^ X::swizzle(lane / NB)) * 16;
-    const uint32_t dst_params = 2 * A4_TILE * X::ROW + lane * X::PROW;
+    const uint32_t ring = smem_u32(smem) + warp * A4_STAGES * X::STAGE;
+    // where this lane's first 16-byte piece goes in a stage, and its row of params; lanes 0-15 copy K params, 16-31 V params
+    const uint32_t dst_codes = a4_keep(ring + (lane / NB) * X::ROW + ((lane % NB) ^ X::swizzle(lane / NB)) * 16);
+    const uint32_t dst_params = a4_keep(ring + 2 * A4_TILE * X::ROW + lane * X::PROW);
     const unsigned char *params = (const unsigned char *)(lane < 16 ? C.k_params : C.v_params) + (lane & 15) * X::PROW;
-    const int kpos0 = a4_pos(r);                               // this lane's K rows: kpos0 and kpos0 + 8
-    const int vpos0 = t, vpos1 = 4 + (t ^ 1);                  // its V rows: these and + 8
+    // where it reads: K rows kpos and kpos + 8 (chunk t of a row; two chunks at head_dim 256), their params, and its eighth of V
+    // rows t, 4 + (t ^ 1) and these + 8
+    const int kpos = a4_pos(r);
+    const uint32_t at_k = a4_keep(ring + kpos * X::ROW + (NB == 4 ? (t ^ X::swizzle(kpos)) * 16 : NB == 8 ? ((2 * t) ^ X::swizzle(kpos)) * 16 : t * 4 * NB));
+    const uint32_t at_p = a4_keep(ring + 2 * A4_TILE * X::ROW + kpos * X::PROW);
+    auto piece = [&](int pos) { return ring + (A4_TILE + pos) * X::ROW + (((2 * NB * r >> 4) ^ X::swizzle(pos)) << 4) + (2 * NB * r & 15); };
+    const uint32_t at_v0 = a4_keep(piece(t)), at_v1 = a4_keep(piece(4 + (t ^ 1)));
 
     for (long at = begin; at < end;) {
         // ---- one segment: units [u0, u1) of (sequence b, kv head, block of q heads) -------------------------------------------
@@ -217,67 +241,74 @@ attn4_kernel(const Attn4Args A) {
         const int heads = min(A4_HEADS, (kvh + 1) * gqa - h0);
         at = item_start + u1;
 
-        // tile i of this warp -> stage i % STAGES: 16 neighbouring rows are one linear piece of the cache, so a tile that is
-        // whole and lies in one block takes nothing but copies at fixed distances
-        const bool one = !C.block_table || C.block_size % A4_TILE == 0;
-        long next = ((long)b * C.heads + kvh) * C.capacity + u0 * A4_UNIT + warp * A4_TILE;      // head-major: row of the next tile
-        auto issue = [&](int i) {
-            const int p0 = (u0 + i) * A4_UNIT + warp * A4_TILE;
-            const uint32_t st = ring32 + (i % A4_STAGES) * X::STAGE;
-            long first = next;
-            next += A4_UNIT;
-            if (C.block_table && one && p0 < len) {
-                const int lb = (int)__umul64hi((unsigned long long)p0, A.block_magic);
-                const int blk = C.block_table[(long)b * C.max_blocks + lb];
-                first = (unsigned)blk < (unsigned)C.num_blocks ? ((long)blk * C.heads + kvh) * C.block_size + (p0 - lb * C.block_size) : -1;
-            }
-            if (one && p0 + A4_TILE <= len && first >= 0) {
-                const unsigned char *k = (const unsigned char *)C.k_codes + first * X::ROW + lane * 16;
-                const unsigned char *v = (const unsigned char *)C.v_codes + first * X::ROW + lane * 16;
+        // Tile i of this warp goes to stage i % STAGES.  16 neighbouring rows are one linear piece of the cache, so a tile that is
+        // whole and lies in one block takes nothing but copies at fixed distances; the loops below are unrolled over the stages,
+        // which makes the distances of a head-major cache constants (`ahead` tiles from the pointers).
+        const int tiles = u1 - u0;
+        const bool paged = C.block_table != nullptr, one = !paged || C.block_size % A4_TILE == 0;
+        // head-major: this many tiles are whole
+        const int whole = paged ? 0 : min(max((len - (warp + 1) * A4_TILE + A4_UNIT) / A4_UNIT - u0, 0), tiles);
+        const long row0 = ((long)b * C.heads + kvh) * C.capacity + u0 * A4_UNIT + warp * A4_TILE;
+        const unsigned char *src_k = (const unsigned char *)C.k_codes + row0 * X::ROW + lane * 16;
+        const unsigned char *src_v = (const unsigned char *)C.v_codes + row0 * X::ROW + lane * 16;
+        const unsigned char *src_p = params + row0 * X::PROW;
+        auto copy_whole = [&](uint32_t stage, const unsigned char *k, const unsigned char *v, const unsigned char *p) {
 #pragma unroll
-                for (int c = 0; c < NB; c += 2)
-                    if (c + 1 < NB || lane < 16) {
-                        a4_copy<16>(st + dst_codes + c * 256, k + c * 256, 16);
-                        a4_copy<16>(st + dst_codes + A4_TILE * X::ROW + c * 256, v + c * 256, 16);
-                    }
-                const unsigned char *p = params + first * X::PROW;
-#pragma unroll
-                for (int c = 0; c < X::PROW; c += X::PCOPY) a4_copy<X::PCOPY>(st + dst_params + c, p + c, X::PCOPY);
-                if (C.block_table && lane == 0) *reinterpret_cast<uint32_t *>(ring + (i % A4_STAGES) * X::STAGE + X::STAGE - 16) = 0xffffu;
-            } else {
-                auto row_of = [&](int row) {           // -1: behind the context, or in a block that the pool does not have
-                    if (p0 + row >= len) return -1l;
-                    if (one) return first < 0 ? -1l : first + row;
-                    return kv4_row(C, b, kvh, p0 + row);
-                };
-#pragma unroll 1
-                for (int c = lane; c < A4_TILE * NB; c += 32) {
-                    const long row = row_of(c / NB);
-                    const long off = max(row, 0l) * X::ROW + (c % NB) * 16;
-                    const uint32_t dst = st + dst_codes + (c - lane) * 16;
-                    a4_copy<16>(dst, (const unsigned char *)C.k_codes + off, row < 0 ? 0 : 16);
-                    a4_copy<16>(dst + A4_TILE * X::ROW, (const unsigned char *)C.v_codes + off, row < 0 ? 0 : 16);
+            for (int c = 0; c < NB; c += 2)
+                if (c + 1 < NB || lane < 16) {
+                    a4_copy<16>(dst_codes + stage + c * 256, k + c * 256, 16);
+                    a4_copy<16>(dst_codes + stage + A4_TILE * X::ROW + c * 256, v + c * 256, 16);
                 }
-                const long row = row_of(lane & 15);
 #pragma unroll
-                for (int c = 0; c < X::PROW; c += X::PCOPY)
-                    a4_copy<X::PCOPY>(st + dst_params + c, (const unsigned char *)(lane < 16 ? C.k_params : C.v_params) + max(row, 0l) * X::PROW + c,
-                                      row < 0 ? 0 : X::PCOPY);
-                const unsigned valid = __ballot_sync(0xffffffffu, row >= 0) & 0xffffu;
-                if (lane == 0) {
-                    *reinterpret_cast<uint32_t *>(ring + (i % A4_STAGES) * X::STAGE + X::STAGE - 16) = valid;
-                    const int rows = min(A4_TILE, len - p0);
-                    if (rows > 0 && __popc(valid) != rows) atomicOr(A.status, KV4_BAD_BLOCK);
+            for (int c = 0; c < X::PROW; c += X::PCOPY) a4_copy<X::PCOPY>(dst_params + stage + c, p + c, X::PCOPY);
+        };
+        auto issue = [&](int i, int stage, int ahead) {
+            const uint32_t st = stage * X::STAGE;
+            if (i < whole) {
+                copy_whole(st, src_k + ahead * A4_UNIT * X::ROW, src_v + ahead * A4_UNIT * X::ROW, src_p + ahead * A4_UNIT * X::PROW);
+            } else if (i < tiles) {
+                const int p0 = (u0 + i) * A4_UNIT + warp * A4_TILE;
+                long first = row0 + (long)i * A4_UNIT;
+                if (paged && one && p0 < len) {
+                    const int lb = (int)__umul64hi((unsigned long long)p0, A.block_magic);
+                    const int blk = C.block_table[(long)b * C.max_blocks + lb];
+                    first = (unsigned)blk < (unsigned)C.num_blocks ? ((long)blk * C.heads + kvh) * C.block_size + (p0 - lb * C.block_size) : -1;
+                }
+                const uint32_t mask = ring + st + X::STAGE - 16;
+                if (one && p0 + A4_TILE <= len && first >= 0) {
+                    copy_whole(st, (const unsigned char *)C.k_codes + first * X::ROW + lane * 16, (const unsigned char *)C.v_codes + first * X::ROW + lane * 16,
+                               params + first * X::PROW);
+                    if (lane == 0) asm volatile("st.shared.u32 [%0], %1;" ::"r"(mask), "r"(0xffffu) : "memory");
+                } else {
+                    auto row_of = [&](int row) {           // -1: behind the context, or in a block that the pool does not have
+                        if (p0 + row >= len) return -1l;
+                        if (one) return first < 0 ? -1l : first + row;
+                        return kv4_row(C, b, kvh, p0 + row);
+                    };
+#pragma unroll 1
+                    for (int c = lane; c < A4_TILE * NB; c += 32) {
+                        const long row = row_of(c / NB);
+                        const long off = max(row, 0l) * X::ROW + (c % NB) * 16;
+                        const uint32_t dst = dst_codes + st + (c - lane) * 16;
+                        a4_copy<16>(dst, (const unsigned char *)C.k_codes + off, row < 0 ? 0 : 16);
+                        a4_copy<16>(dst + A4_TILE * X::ROW, (const unsigned char *)C.v_codes + off, row < 0 ? 0 : 16);
+                    }
+                    const long row = row_of(lane & 15);
+#pragma unroll
+                    for (int c = 0; c < X::PROW; c += X::PCOPY)
+                        a4_copy<X::PCOPY>(dst_params + st + c, params + (row < 0 ? 0 : row - (lane & 15)) * X::PROW + c, row < 0 ? 0 : X::PCOPY);
+                    const unsigned valid = __ballot_sync(0xffffffffu, row >= 0) & 0xffffu;
+                    if (lane == 0) {
+                        asm volatile("st.shared.u32 [%0], %1;" ::"r"(mask), "r"(valid) : "memory");
+                        const int rows = min(A4_TILE, len - p0);
+                        if (rows > 0 && __popc(valid) != rows) atomicOr(A.status, KV4_BAD_BLOCK);
+                    }
                 }
             }
             asm volatile("cp.async.commit_group;" ::: "memory");
         };
-        const int tiles = u1 - u0;
 #pragma unroll
-        for (int i = 0; i < A4_STAGES - 1; ++i) {
-            if (i < tiles) issue(i);
-            else asm volatile("cp.async.commit_group;" ::: "memory");
-        }
+        for (int i = 0; i < A4_STAGES - 1; ++i) issue(i, i, i);
 
         // ---- q as the B operand: head r, lane t's dims; scaled by a power of two to [2^14, 2^15) ----------------------------------
         // (any 16-bit type then fits fp16 with all its bits, down to 2^-25 of the head's largest element; nibbles 1 and 3 carry
@@ -351,44 +382,51 @@ attn4_kernel(const Attn4Args A) {
         if (!(fac[0] > 0.f)) { top[0] = 0.f; bar[0] = INFINITY; ref[0] = 0.f; }
         if (!(fac[1] > 0.f)) { top[1] = 0.f; bar[1] = INFINITY; ref[1] = 0.f; }
 
-        for (int i = 0; i < tiles; ++i) {
+        auto tile = [&](int i, int stage) {
             asm volatile("cp.async.wait_group %0;" ::"n"(A4_STAGES - 2) : "memory");
             __syncwarp();
-            if (i + A4_STAGES - 1 < tiles) issue(i + A4_STAGES - 1);
-            else asm volatile("cp.async.commit_group;" ::: "memory");
-            const unsigned char *st = ring + (i % A4_STAGES) * X::STAGE;
-            const unsigned char *sk = st, *sv = st + A4_TILE * X::ROW, *pk = sv + A4_TILE * X::ROW, *pv = pk + A4_TILE * X::PROW;
-            uint32_t valid = 0xffffu;
-            if (C.block_table || (u0 + i) * A4_UNIT + (warp + 1) * A4_TILE > len) valid = *reinterpret_cast<const uint32_t *>(st + X::STAGE - 16);
+            issue(i + A4_STAGES - 1, (stage + A4_STAGES - 1) % A4_STAGES, stage + A4_STAGES - 1);
+            const int st = stage * X::STAGE;
+            const bool edge = i >= whole;         // some rows may have to be left out
+            bool ok0 = true, ok1 = true;
+            if (edge) {
+                uint32_t valid;
+                a4_lds<1>(&valid, ring + st + X::STAGE - 16);
+                ok0 = (valid >> kpos) & 1;
+                ok1 = (valid >> (kpos + 8)) & 1;
+            }
 
             // scores: rows r and r + 8 are positions kpos0 and kpos0 + 8, columns heads 2t and 2t + 1
             float s[4] = {0.f, 0.f, 0.f, 0.f};
             {
                 uint32_t w0[NB], w1[NB];
                 if constexpr (NB == 8) {
-                    const int sw = X::swizzle(kpos0);         // the same for + 8
-                    a4_lds<4>(*reinterpret_cast<uint32_t (*)[4]>(&w0[0]), sk + kpos0 * X::ROW + ((2 * t) ^ sw) * 16);
-                    a4_lds<4>(*reinterpret_cast<uint32_t (*)[4]>(&w0[4]), sk + kpos0 * X::ROW + ((2 * t + 1) ^ sw) * 16);
-                    a4_lds<4>(*reinterpret_cast<uint32_t (*)[4]>(&w1[0]), sk + (kpos0 + 8) * X::ROW + ((2 * t) ^ sw) * 16);
-                    a4_lds<4>(*reinterpret_cast<uint32_t (*)[4]>(&w1[4]), sk + (kpos0 + 8) * X::ROW + ((2 * t + 1) ^ sw) * 16);
+                    a4_lds<4>(w0, at_k + st);
+                    a4_lds<4>(w0 + 4, (at_k ^ 16) + st);
+                    a4_lds<4>(w1, at_k + st + 8 * X::ROW);
+                    a4_lds<4>(w1 + 4, (at_k ^ 16) + st + 8 * X::ROW);
                 } else {
-                    const int off = NB == 4 ? (t ^ X::swizzle(kpos0)) * 16 : t * 4 * NB;
-                    a4_lds<NB>(w0, sk + kpos0 * X::ROW + off);
-                    a4_lds<NB>(w1, sk + (kpos0 + 8) * X::ROW + off);
+                    a4_lds<NB>(w0, at_k + st);
+                    a4_lds<NB>(w1, at_k + st + 8 * X::ROW);
                 }
                 float s0[NG], z0[NG], s1[NG], z1[NG];
-                a4_params<NG>(s0, z0, pk + kpos0 * X::PROW);
-                a4_params<NG>(s1, z1, pk + (kpos0 + 8) * X::PROW);
+                a4_params<NG>(s0, z0, at_p + st);
+                a4_params<NG>(s1, z1, at_p + st + 8 * X::PROW);
 #pragma unroll
                 for (int g = 0; g < NG; ++g) {
-                    float acc[4] = {0.f, 0.f, 0.f, 0.f};
+                    float acc[4];
+                    bool begun = false;
 #pragma unroll
                     for (int j = 0; j < NB; ++j) {
                         if (a4_kgroup<NB, NG, X::PURE>(j) != g) continue;
                         const uint32_t x = a4_kword<NB, X::PURE>(w0, j), y = a4_kword<NB, X::PURE>(w1, j);
-                        const uint32_t x8 = x >> 8, y8 = y >> 8;
-                        a4_mma(acc, x & 0x000f000fu, y & 0x000f000fu, x & 0x00f000f0u, y & 0x00f000f0u, qf[4 * j], qf[4 * j + 1]);
-                        a4_mma(acc, x8 & 0x000f000fu, y8 & 0x000f000fu, x8 & 0x00f000f0u, y8 & 0x00f000f0u, qf[4 * j + 2], qf[4 * j + 3]);
+                        uint32_t x0, x1, x2, x3, y0, y1, y2, y3;
+                        a4_codes(x, x0, x1, x2, x3);
+                        a4_codes(y, y0, y1, y2, y3);
+                        if (begun) a4_mma(acc, x0, y0, x1, y1, qf[4 * j], qf[4 * j + 1]);
+                        else a4_mma0(acc, x0, y0, x1, y1, qf[4 * j], qf[4 * j + 1]);
+                        begun = true;
+                        a4_mma(acc, x2, y2, x3, y3, qf[4 * j + 2], qf[4 * j + 3]);
                     }
                     s[0] = fmaf(s0[g], acc[0], fmaf(z0[g], qsum[g][0], s[0]));
                     s[1] = fmaf(s0[g], acc[1], fmaf(z0[g], qsum[g][1], s[1]));
@@ -397,10 +435,9 @@ attn4_kernel(const Attn4Args A) {
                 }
             }
             float vs0[NG], vz0[NG], vs1[NG], vz1[NG];
-            a4_params<NG>(vs0, vz0, pv + kpos0 * X::PROW);
-            a4_params<NG>(vs1, vz1, pv + (kpos0 + 8) * X::PROW);
-            const bool ok0 = (valid >> kpos0) & 1, ok1 = (valid >> (kpos0 + 8)) & 1;
-            if (valid != 0xffffu) {
+            a4_params<NG>(vs0, vz0, at_p + st + A4_TILE * X::PROW);
+            a4_params<NG>(vs1, vz1, at_p + st + (A4_TILE + 8) * X::PROW);
+            if (edge) {
                 if (!ok0) s[0] = s[1] = -1e30f;
                 if (!ok1) s[2] = s[3] = -1e30f;
             }
@@ -441,7 +478,7 @@ attn4_kernel(const Attn4Args A) {
             p[1] = a4_exp2(fmaf(s[1], fac[1], -ref[1]));
             p[2] = a4_exp2(fmaf(s[2], fac[0], -ref[0]));
             p[3] = a4_exp2(fmaf(s[3], fac[1], -ref[1]));
-            if (valid != 0xffffu) {
+            if (edge) {
                 if (!ok0) p[0] = p[1] = 0.f;
                 if (!ok1) p[2] = p[3] = 0.f;
             }
@@ -458,33 +495,38 @@ attn4_kernel(const Attn4Args A) {
             // output: rows r and r + 8 of m-tile 2 j + h are dims 32 j + 4 r + 2 h and + 1
             auto out_tiles = [&](int j, uint32_t x, uint32_t y) {
                 const int g = j * NG / NB;
-                a4_mma(oacc[2 * j], x & 0x000f000fu, x & 0x00f000f0u, y & 0x000f000fu, y & 0x00f000f0u, pb[g][0], pb[g][1]);
-                x >>= 8;
-                y >>= 8;
-                a4_mma(oacc[2 * j + 1], x & 0x000f000fu, x & 0x00f000f0u, y & 0x000f000fu, y & 0x00f000f0u, pb[g][0], pb[g][1]);
+                uint32_t x0, x1, x2, x3, y0, y1, y2, y3;
+                a4_codes(x, x0, x1, x2, x3);
+                a4_codes(y, y0, y1, y2, y3);
+                a4_mma(oacc[2 * j], x0, x1, y0, y1, pb[g][0], pb[g][1]);
+                a4_mma(oacc[2 * j + 1], x2, x3, y2, y3, pb[g][0], pb[g][1]);
             };
             if constexpr (NB % 2 == 0) {
                 uint32_t va[NB / 2], vb[NB / 2], vc[NB / 2], vd[NB / 2];
-                // lane r's piece of a row: 2 NB bytes at 2 NB r
-                auto piece = [&](int pos) {
-                    const int byte = 2 * NB * r;
-                    return sv + pos * X::ROW + (((byte >> 4) ^ X::swizzle(pos)) << 4) + (byte & 15);
-                };
-                a4_lds<NB / 2>(va, piece(vpos0));
-                a4_lds<NB / 2>(vb, piece(vpos1));
-                a4_lds<NB / 2>(vc, piece(vpos0 + 8));
-                a4_lds<NB / 2>(vd, piece(vpos1 + 8));
+                a4_lds<NB / 2>(va, at_v0 + st);
+                a4_lds<NB / 2>(vb, at_v1 + st);
+                a4_lds<NB / 2>(vc, at_v0 + st + 8 * X::ROW);
+                a4_lds<NB / 2>(vd, at_v1 + st + 8 * X::ROW);
 #pragma unroll
                 for (int j = 0; j < NB; ++j) {
                     const int sel = j & 1 ? 0x7632 : 0x5410;
                     out_tiles(j, __byte_perm(va[j >> 1], vb[j >> 1], sel), __byte_perm(vc[j >> 1], vd[j >> 1], sel));
                 }
             } else {
-                auto unit = [&](int pos, int j) { return (uint32_t) * reinterpret_cast<const uint16_t *>(sv + pos * X::ROW + 2 * (NB * r + j)); };
 #pragma unroll
                 for (int j = 0; j < NB; ++j)
-                    out_tiles(j, unit(vpos0, j) | unit(vpos1, j) << 16, unit(vpos0 + 8, j) | unit(vpos1 + 8, j) << 16);
+                    out_tiles(j, a4_lds16(at_v0 + st + 2 * j) | a4_lds16(at_v1 + st + 2 * j) << 16,
+                              a4_lds16(at_v0 + st + 8 * X::ROW + 2 * j) | a4_lds16(at_v1 + st + 8 * X::ROW + 2 * j) << 16);
             }
+        };
+#pragma unroll 1
+        for (int i = 0; i < tiles; i += A4_STAGES) {
+#pragma unroll
+            for (int stage = 0; stage < A4_STAGES; ++stage)
+                if (i + stage < tiles) tile(i + stage, stage);
+            src_k += A4_STAGES * A4_UNIT * X::ROW;
+            src_v += A4_STAGES * A4_UNIT * X::ROW;
+            src_p += A4_STAGES * A4_UNIT * X::PROW;
         }
         asm volatile("cp.async.wait_group 0;" ::: "memory");
 
@@ -499,77 +541,93 @@ attn4_kernel(const Attn4Args A) {
                 zacc[g][1] += __shfl_xor_sync(0xffffffffu, zacc[g][1], o);
             }
         }
-        __syncthreads();                   // every warp is done with its ring
-        float *so = reinterpret_cast<float *>(smem);       // [warp][m-tile row][head]
-#pragma unroll
-        for (int m = 0; m < X::MTILES; ++m) {
-            const int g = (m / 2) * NG / NB;
-            float *o0 = so + ((warp * X::D) + m * 16 + r) * A4_HEADS + 2 * t;
-            *reinterpret_cast<float2 *>(o0) = make_float2(fmaf(oacc[m][0], 16777216.f, zacc[g][0]), fmaf(oacc[m][1], 16777216.f, zacc[g][1]));
-            *reinterpret_cast<float2 *>(o0 + 8 * A4_HEADS) = make_float2(fmaf(oacc[m][2], 1048576.f, zacc[g][0]), fmaf(oacc[m][3], 1048576.f, zacc[g][1]));
-        }
         if (lane < 4) {
-            const bool some0 = l[0] != 0.f, some1 = l[1] != 0.f;    // a warp without positions has no say in the maximum
-            sm_ref[warp][2 * t] = some0 ? ref[0] : -INFINITY;
-            sm_ref[warp][2 * t + 1] = some1 ? ref[1] : -INFINITY;
-            sm_l[warp][2 * t] = l[0];
-            sm_l[warp][2 * t + 1] = l[1];
+            // a warp without positions has no say in the maximum
+            *reinterpret_cast<float2 *>(&sm_ref[warp][2 * t]) = make_float2(l[0] != 0.f ? ref[0] : -INFINITY, l[1] != 0.f ? ref[1] : -INFINITY);
+            *reinterpret_cast<float2 *>(&sm_l[warp][2 * t]) = make_float2(l[0], l[1]);
         }
-        __syncthreads();
-        if (tid < A4_HEADS) {
-            float M = -INFINITY, L = 0.f;
-            for (int w = 0; w < A4_WARPS; ++w) M = fmaxf(M, sm_ref[w][tid]);
-            for (int w = 0; w < A4_WARPS; ++w) {
-                const float x = sm_l[w][tid] == 0.f ? 0.f : exp2f(sm_ref[w][tid] - M);
-                sm_w[w][tid] = x;
-                L += sm_l[w][tid] * x;
-            }
-            sm_top[tid] = M;
-            sm_sum[tid] = L;
-        }
-        __syncthreads();
-        auto joined = [&](int idx, int h) {
-            float o = 0.f;
+        __syncthreads();                   // and every warp is done with its ring
+        float *so = reinterpret_cast<float *>(smem);       // [warp][m-tile row][head], over the rings
+        {
+            float wgt[2], M[2] = {-INFINITY, -INFINITY}, L[2] = {0.f, 0.f};
 #pragma unroll
             for (int w = 0; w < A4_WARPS; ++w) {
-                const float x = sm_w[w][h];
-                o += x == 0.f ? 0.f : so[(w * X::D + idx) * A4_HEADS + h] * x;
+                M[0] = fmaxf(M[0], sm_ref[w][2 * t]);
+                M[1] = fmaxf(M[1], sm_ref[w][2 * t + 1]);
+            }
+#pragma unroll
+            for (int w = 0; w < A4_WARPS; ++w)
+#pragma unroll
+                for (int e2 = 0; e2 < 2; ++e2) {
+                    const float lw = sm_l[w][2 * t + e2], x = lw == 0.f ? 0.f : a4_exp2(sm_ref[w][2 * t + e2] - M[e2]);
+                    L[e2] += lw * x;
+                    if (w == warp) wgt[e2] = x;
+                }
+            if (tid < 4) {
+                *reinterpret_cast<float2 *>(&sm_top[2 * t]) = make_float2(M[0], M[1]);
+                *reinterpret_cast<float2 *>(&sm_sum[2 * t]) = make_float2(L[0], L[1]);
+            }
+            float *o0 = so + (warp * X::D + r) * A4_HEADS + 2 * t;
+#pragma unroll
+            for (int m = 0; m < X::MTILES; ++m) {
+                const int g = (m / 2) * NG / NB;
+                const float za = zacc[g][0] * wgt[0], zb = zacc[g][1] * wgt[1];
+                *reinterpret_cast<float2 *>(o0 + m * 16 * A4_HEADS) =
+                    make_float2(fmaf(oacc[m][0], 16777216.f * wgt[0], za), fmaf(oacc[m][1], 16777216.f * wgt[1], zb));
+                *reinterpret_cast<float2 *>(o0 + (m * 16 + 8) * A4_HEADS) =
+                    make_float2(fmaf(oacc[m][2], 1048576.f * wgt[0], za), fmaf(oacc[m][3], 1048576.f * wgt[1], zb));
+            }
+        }
+        __syncthreads();
+        const int two = heads > 4, quads = 1 + two;       // groups of four heads that exist
+        // the sum over the warps of float4 i & two of m-tile row i >> two
+        auto sum4 = [&](int i) {
+            const float4 *s4 = reinterpret_cast<const float4 *>(so) + (i >> two) * 2 + (i & two);
+            float4 o = s4[0];
+#pragma unroll
+            for (int w = 1; w < A4_WARPS; ++w) {
+                const float4 x = s4[w * X::D * A4_HEADS / 4];
+                o.x += x.x; o.y += x.y; o.z += x.z; o.w += x.w;
             }
             return o;
         };
-        auto index_of = [](int d) { return (2 * (d >> 5) + ((d >> 1) & 1)) * 16 + ((d & 31) >> 2) + 8 * (d & 1); };   // dim -> m-tile row
-        auto store = [&](int h, int d, float v) {
-            const long at_out = ((long)b * A.hq + h0 + h) * X::D;
-            const int e7 = d & 7, dd = A.out_kperm ? (d & ~7) | (e7 < 4 ? 2 * e7 : 2 * e7 - 7) : d;
-            if (A.bf16) reinterpret_cast<__nv_bfloat16 *>(A.out)[at_out + dd] = __float2bfloat16_rn(v);
-            else reinterpret_cast<__half *>(A.out)[at_out + dd] = __float2half_rn(v);
+        auto finish = [&] {                                // the output rows of these heads
+            for (int i = tid; i < X::D * quads; i += A4_THREADS) {
+                const float4 o4 = sum4(i);
+                const float o[4] = {o4.x, o4.y, o4.z, o4.w};
+                const int idx = i >> two, m = idx >> 4, row = idx & 15, d = 32 * (m >> 1) + 4 * (row & 7) + 2 * (m & 1) + (row >> 3);
+                const int e7 = d & 7, dd = A.out_kperm ? (d & ~7) | (e7 < 4 ? 2 * e7 : 2 * e7 - 7) : d;
+#pragma unroll
+                for (int e4 = 0; e4 < 4; ++e4) {
+                    const int h = 4 * (i & two) + e4;
+                    if (h >= heads) break;
+                    const float v = sm_sum[h] == 0.f ? 0.f : o[e4] / sm_sum[h];      // nothing but blocks outside the pool: 0
+                    const long at_out = ((long)b * A.hq + h0 + h) * X::D + dd;
+                    if (A.bf16) reinterpret_cast<__nv_bfloat16 *>(A.out)[at_out] = __float2bfloat16_rn(v);
+                    else reinterpret_cast<__half *>(A.out)[at_out] = __float2half_rn(v);
+                }
+            }
         };
         if (u0 == 0 && u1 == n) {          // the whole context was here
-            for (int i = tid; i < heads * X::D; i += A4_THREADS) {
-                const int h = i / X::D, d = i % X::D;
-                store(h, d, sm_sum[h] == 0.f ? 0.f : joined(index_of(d), h) / sm_sum[h]);
-            }
+            finish();
             __syncthreads();
             continue;
         }
         // ---- join the CTAs: partial results through the workspace, the last to arrive adds them up in CTA order ------------------
         const int c0 = (int)(item_start / share), c1 = (int)((item_start + n - 1) / share);
         float *part = A.parts + ((long)cta * 2 + (u0 == 0)) * X::PART;
-        for (int i = tid; i < X::D * A4_HEADS; i += A4_THREADS) part[i] = joined(i / A4_HEADS, i % A4_HEADS);
-        if (tid < A4_HEADS) {
-            part[X::D * A4_HEADS + 2 * tid] = sm_top[tid];
-            part[X::D * A4_HEADS + 2 * tid + 1] = sm_sum[tid];
-        }
+        for (int i = tid; i < X::D * quads; i += A4_THREADS) reinterpret_cast<float4 *>(part)[(i >> two) * 2 + (i & two)] = sum4(i);
+        if (tid < A4_HEADS) reinterpret_cast<float2 *>(part + X::D * A4_HEADS)[tid] = make_float2(sm_top[tid], sm_sum[tid]);
         __threadfence();
         __syncthreads();
         if (tid == 0) sm_last = atomicAdd(&A.counters[c0], 1) == c1 - c0;
         __syncthreads();
         if (sm_last) {
             __threadfence();
-            // weights 2^(m_c - M) of the parts to shared memory (over the ring), then the parts dealt out to the warps, each lane
-            // with several loads in flight, then the warps' sums in order
+            // weights 2^(m_c - M) of the parts to shared memory (behind the results), then the parts dealt out to the warps,
+            // each lane with several loads in flight, then the warps' sums in order
             const int parts = c1 - c0 + 1;
-            float *wt = reinterpret_cast<float *>(smem) + A4_WARPS * X::D * A4_HEADS;      // [part][head]
+            float *wt = so + A4_WARPS * X::D * A4_HEADS;       // [part][head]
             auto part_of = [&](int c) { return A.parts + ((long)(c0 + c) * 2 + (c == 0)) * X::PART; };
             const int h = tid & 7;
             float M = -INFINITY, L = 0.f;
@@ -585,7 +643,7 @@ attn4_kernel(const Attn4Args A) {
             for (int w = 0; w < A4_WARPS; ++w) M = fmaxf(M, sm_ref[w][h]);
             for (int c = tid >> 3; c < parts; c += A4_THREADS / 8) {
                 const float2 ml = __ldcg(reinterpret_cast<const float2 *>(part_of(c) + X::D * A4_HEADS) + h);
-                const float x = ml.y == 0.f ? 0.f : exp2f(ml.x - M);
+                const float x = ml.y == 0.f ? 0.f : a4_exp2(ml.x - M);
                 wt[c * A4_HEADS + h] = x;
                 L += ml.y * x;
             }
@@ -594,29 +652,19 @@ attn4_kernel(const Attn4Args A) {
             if (lane < 8) sm_l[warp][lane] = L;
             __syncthreads();
             if (tid < A4_HEADS) sm_sum[tid] = sm_l[0][tid] + sm_l[1][tid] + sm_l[2][tid] + sm_l[3][tid];
-            const int quads = heads <= 4 ? 1 : 2;            // groups of four heads that exist
             for (int i = lane; i < X::D * quads; i += 32) {
-                const int at4 = (i / quads) * 2 + i % quads;  // float4 of a part: (m-tile row, four heads)
+                const int at4 = (i >> two) * 2 + (i & two);
                 float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 8
                 for (int c = warp; c < parts; c += A4_WARPS) {
                     const float4 x = __ldcg(reinterpret_cast<const float4 *>(part_of(c)) + at4);
                     const float4 w = *reinterpret_cast<const float4 *>(wt + c * A4_HEADS + 4 * (at4 & 1));
-                    o.x += w.x == 0.f ? 0.f : w.x * x.x;
-                    o.y += w.y == 0.f ? 0.f : w.y * x.y;
-                    o.z += w.z == 0.f ? 0.f : w.z * x.z;
-                    o.w += w.w == 0.f ? 0.f : w.w * x.w;
+                    o.x = fmaf(w.x, x.x, o.x); o.y = fmaf(w.y, x.y, o.y); o.z = fmaf(w.z, x.z, o.z); o.w = fmaf(w.w, x.w, o.w);
                 }
                 reinterpret_cast<float4 *>(so + warp * X::D * A4_HEADS)[at4] = o;
             }
             __syncthreads();
-            for (int i = tid; i < heads * X::D; i += A4_THREADS) {
-                const int hh = i / X::D, d = i % X::D, idx = index_of(d) * A4_HEADS + hh;
-                float o = 0.f;
-#pragma unroll
-                for (int w = 0; w < A4_WARPS; ++w) o += so[w * X::D * A4_HEADS + idx];
-                store(hh, d, sm_sum[hh] == 0.f ? 0.f : o / sm_sum[hh]);
-            }
+            finish();
             if (tid == 0) A.counters[c0] = 0;      // ready for the next launch
         }
         __syncthreads();
