@@ -23,9 +23,25 @@
 
 namespace b200k {
 
-constexpr int A4_WARPS = 4, A4_THREADS = 32 * A4_WARPS, A4_STAGES = 4;
+#ifndef A4_NSTAGES
+#define A4_NSTAGES 3
+#endif
+#ifndef A4_EDGE
+#define A4_EDGE __forceinline__
+#endif
+#ifndef A4_WAVES
+#define A4_WAVES 1
+#endif
+#ifndef A4_MAXC
+#define A4_MAXC 640
+#endif
+#ifndef A4_C4
+#define A4_C4 4
+#endif
+constexpr int A4_WARPS = 4, A4_THREADS = 32 * A4_WARPS, A4_STAGES = A4_NSTAGES;
 constexpr int A4_TILE = 16, A4_UNIT = A4_WARPS * A4_TILE;      // positions of a warp's tile, of a unit of work
-constexpr int A4_MAX_CTAS = 640;                               // more than four CTAs on every SM
+constexpr int A4_MAX_CTAS = A4_MAXC;                              // CTAs of a launch
+constexpr int A4_FAN = 16;                                     // partial results that are joined at a time
 constexpr int A4_HEADS = 8;                                    // columns of one MMA
 constexpr float A4_LAZY = 6.f;        // the running maximum moves when a score passes it by 2^6: probabilities stay below 2^6
 constexpr float A4_TOP = 512.f;       // 2^e times the largest value scale is set to [2^2, 2^3) and set again when it passes 2^9
@@ -40,7 +56,7 @@ struct Attn4Args {
     int bf16, out_kperm;
     float scale_log2e;
     int *status;
-    int *counters;                // one per CTA, zero between launches
+    int *counters;                // [level of the join][CTA][2], zero between launches
     float *parts;                 // [CTA][2][D * 8 + 16]
 };
 
@@ -51,15 +67,14 @@ struct A4 {
     static constexpr int D = 32 * NB, G = D / NG;
     static constexpr int ROW = 16 * NB, PROW = 4 * NG;        // bytes of a row's codes, of its params
     static constexpr int PCOPY = NG % 4 == 0 ? 16 : NG % 2 == 0 ? 8 : 4;      // as wide as a row of params is aligned
-    static constexpr int STAGE = 2 * A4_TILE * (ROW + PROW) + 16;
-    static constexpr int KSTEPS = 2 * NB, MTILES = 2 * NB;
+    static constexpr int STAGE = 2 * A4_TILE * (ROW + PROW) + 32;              // a multiple of 32: see at_k
+    static constexpr int MTILES = 2 * NB;
     static constexpr bool PURE = G == 32;                     // a group is one block: see kword()
     static constexpr int PART = D * A4_HEADS + 16;            // floats of a partial result
-    static constexpr int CTAS = NB <= 4 ? 4 : NB <= 6 ? 3 : 2;
+    static constexpr int CTAS = NB <= 4 ? A4_C4 : NB <= 5 ? 3 : 2;
     static constexpr int RING = A4_WARPS * A4_STAGES * STAGE;
-    static constexpr int JOIN = A4_WARPS * D * A4_HEADS * 4;  // the warps' results, over the ring
-    static constexpr int JOIN2 = JOIN + A4_MAX_CTAS * A4_HEADS * 4;      // and the weights of the CTAs' results behind them
-    static constexpr int SMEM = RING > JOIN2 ? RING : JOIN2;
+    static constexpr int JOIN = A4_WARPS * D * A4_HEADS * 4;  // the warps' results
+    static constexpr int SMEM = RING > JOIN ? RING : JOIN;    // in turn
     // 16-byte chunk of a row in shared memory is chunk ^ swizzle(position): the K loads of a quarter warp (two rows of
     // opposite parity) and the V loads of a half warp (positions 0-3 or 4-7) then meet no bank twice
     __device__ static int swizzle(int pos) { return NB == 4 ? pos & 2 : NB == 8 ? ((pos & 3) << 1) | (pos & 1) : 0; }
@@ -163,210 +178,254 @@ __device__ __forceinline__ void a4_kdims(int i, int n, int t, int &lo, int &hi) 
 template <int NB, int NG, bool PURE>
 __device__ __forceinline__ constexpr int a4_kgroup(int i) { return PURE ? i : (i % (NB / 2)) * 2 * NG / NB; }
 
+// The copies of a tile of which not all rows are there, or that spans blocks: row by row, zeros for the rows behind the context and
+// for those in a block that the pool does not have; a mask of the rows that are there goes to the stage's last word.  Not
+// inlined: its code would be met between that of the whole tiles.  `first` < 0 with one block: the block is not there.
+template <int NB, int NG>
+__device__ A4_EDGE void a4_copy_edge(const Attn4Args &A, int b, int kvh, int p0, int len, long first, bool one, uint32_t dst_codes,
+                                          uint32_t dst_params, const unsigned char *params, uint32_t mask) {
+    using X = A4<NB, NG>;
+    const Kv4Cache &C = A.C;
+    const int lane = threadIdx.x & 31;
+    auto row_of = [&](int row) {
+        if (p0 + row >= len) return -1l;
+        if (one) return first < 0 ? -1l : first + row;
+        return kv4_row(C, b, kvh, p0 + row);
+    };
+#pragma unroll 1
+    for (int c = lane; c < A4_TILE * NB; c += 32) {
+        const long row = row_of(c / NB);
+        const long off = max(row, 0l) * X::ROW + (c % NB) * 16;
+        const uint32_t dst = dst_codes + (c - lane) * 16;
+        a4_copy<16>(dst, (const unsigned char *)C.k_codes + off, row < 0 ? 0 : 16);
+        a4_copy<16>(dst + A4_TILE * X::ROW, (const unsigned char *)C.v_codes + off, row < 0 ? 0 : 16);
+    }
+    const long row = row_of(lane & 15);
+#pragma unroll
+    for (int c = 0; c < X::PROW; c += X::PCOPY)
+        a4_copy<X::PCOPY>(dst_params + c, params + (row < 0 ? 0 : row - (lane & 15)) * X::PROW + c, row < 0 ? 0 : X::PCOPY);
+    const unsigned valid = __ballot_sync(0xffffffffu, row >= 0) & 0xffffu;
+    if (lane == 0) {
+        asm volatile("st.shared.u32 [%0], %1;" ::"r"(mask), "r"(valid) : "memory");
+        const int rows = min(A4_TILE, len - p0);
+        if (rows > 0 && __popc(valid) != rows) atomicOr(A.status, KV4_BAD_BLOCK);
+    }
+}
+
+// A segment: units [u0, u1) of the n that a context (sequence b, kv head, q heads [h0, h0 + heads)) has.
+struct Attn4Segment {
+    int b, kvh, h0, heads, len, u0, u1, n;
+    unsigned item_start;            // units before this sequence
+};
+
 template <int NB, int NG>
 __global__ void __launch_bounds__(A4_THREADS, A4<NB, NG>::CTAS)
 attn4_kernel(const __grid_constant__ Attn4Args A) {
     using X = A4<NB, NG>;
     extern __shared__ __align__(128) unsigned char smem[];
-    __shared__ float sm_ref[A4_WARPS][A4_HEADS], sm_l[A4_WARPS][A4_HEADS], sm_top[A4_HEADS], sm_sum[A4_HEADS];
+    __shared__ __align__(16) float sm_ref[A4_WARPS][A4_HEADS], sm_l[A4_WARPS][A4_HEADS], sm_top[A4_HEADS], sm_sum[A4_HEADS];
+    __shared__ __align__(16) uint4 sm_q[NB][32];       // q as the B operand: word i of all lanes
+    __shared__ float sm_qsum[NB][A4_HEADS], sm_fac[A4_HEADS], sm_wt[A4_FAN][A4_HEADS];
+    __shared__ Attn4Segment sm_seg;
     __shared__ int sm_last;
     const Kv4Cache &C = A.C;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, r = lane >> 2, t = lane & 3;
-    const int cta = blockIdx.x, gqa = A.hq / C.heads, per_seq = C.heads * A.head_blocks;
     pdl_wait();
     pdl_launch_dependents();
 
-    // ---- the share of this CTA: units [begin, end) of all ------------------------------------------------------------------
-    auto length = [&](int b) { return min(A.lens[b], C.capacity); };
-    auto units_of = [&](int b) { return (max(length(b), 0) + A4_UNIT - 1) / A4_UNIT; };
-    long total = 0;
+    // ---- the share of this CTA: units [at, end) of all (the host made sure that 32 bits hold them) --------------------------------
+    const unsigned per_seq = C.heads * A.head_blocks;      // contexts of a sequence
+    auto units_of = [&](int b) { return (unsigned)(max(min(A.lens[b], C.capacity), 0) + A4_UNIT - 1) / A4_UNIT; };
+    unsigned total = 0;
+#pragma unroll 4
     for (int b = lane; b < A.batch; b += 32) total += units_of(b);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-    total *= per_seq;
-    const long share = max((total + gridDim.x - 1) / (long)gridDim.x, 1l);
-    const long begin = share * cta, end = min(begin + share, total);
-    for (int b = cta; b < A.batch; b += gridDim.x) {
+    total = __reduce_add_sync(0xffffffffu, total) * per_seq;
+    const unsigned share = max((total + gridDim.x - 1) / gridDim.x, 1u);
+#pragma unroll 1
+    for (int b = blockIdx.x; b < A.batch; b += gridDim.x) {
         const int len = A.lens[b];
         if (len > C.capacity && tid == 0) atomicOr(A.status, KV4_BAD_POSITION);
         if (len <= 0)       // no keys: a zero output row
+#pragma unroll 1
             for (int i = tid; i < A.hq * X::D / 2; i += A4_THREADS) reinterpret_cast<uint32_t *>(A.out)[(long)b * A.hq * X::D / 2 + i] = 0u;
     }
-    if (begin >= end) return;
-    int b = 0;
-    long start = 0;         // units before sequence b
-    for (int b0 = 0; b0 < A.batch; b0 += 32) {
-        const long mine = b0 + lane < A.batch ? (long)units_of(b0 + lane) * per_seq : 0;
-        long upto = mine;
+    unsigned at = share * blockIdx.x;
+    const unsigned end = min(at + share, total);
+    if (at >= end) return;
+    if (warp == 0) {        // the sequence that unit `at` belongs to
+        unsigned start = 0;
+        int b = 0;
+#pragma unroll 1
+        for (int b0 = 0;; b0 += 32) {
+            const unsigned mine = b0 + lane < A.batch ? units_of(b0 + lane) * per_seq : 0u;
+            unsigned upto = mine;
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const long x = __shfl_up_sync(0xffffffffu, upto, o);
-            if (lane >= o) upto += x;
+            for (int o = 1; o < 32; o <<= 1) {
+                const unsigned x = __shfl_up_sync(0xffffffffu, upto, o);
+                if (lane >= o) upto += x;
+            }
+            const unsigned past = __ballot_sync(0xffffffffu, start + upto > at);
+            if (past) {
+                const int found = __ffs(past) - 1;
+                b = b0 + found;
+                start += __shfl_sync(0xffffffffu, upto - mine, found);
+                break;
+            }
+            start += __shfl_sync(0xffffffffu, upto, 31);
         }
-        const unsigned past = __ballot_sync(0xffffffffu, start + upto > begin);
-        if (past) {
-            const int at = __ffs(past) - 1;
-            b = b0 + at;
-            start += __shfl_sync(0xffffffffu, upto - mine, at);
-            break;
+        if (lane == 0) {
+            sm_seg.b = b;
+            sm_seg.item_start = start;
         }
-        start += __shfl_sync(0xffffffffu, upto, 31);
     }
 
     const uint32_t ring = smem_u32(smem) + warp * A4_STAGES * X::STAGE;
     // where this lane's first 16-byte piece goes in a stage, and its row of params; lanes 0-15 copy K params, 16-31 V params
     const uint32_t dst_codes = a4_keep(ring + (lane / NB) * X::ROW + ((lane % NB) ^ X::swizzle(lane / NB)) * 16);
     const uint32_t dst_params = a4_keep(ring + 2 * A4_TILE * X::ROW + lane * X::PROW);
-    const unsigned char *params = (const unsigned char *)(lane < 16 ? C.k_params : C.v_params) + (lane & 15) * X::PROW;
     // where it reads: K rows kpos and kpos + 8 (chunk t of a row; two chunks at head_dim 256), their params, and its eighth of V
     // rows t, 4 + (t ^ 1) and these + 8
     const int kpos = a4_pos(r);
     const uint32_t at_k = a4_keep(ring + kpos * X::ROW + (NB == 4 ? (t ^ X::swizzle(kpos)) * 16 : NB == 8 ? ((2 * t) ^ X::swizzle(kpos)) * 16 : t * 4 * NB));
     const uint32_t at_p = a4_keep(ring + 2 * A4_TILE * X::ROW + kpos * X::PROW);
-    auto piece = [&](int pos) { return ring + (A4_TILE + pos) * X::ROW + (((2 * NB * r >> 4) ^ X::swizzle(pos)) << 4) + (2 * NB * r & 15); };
-    const uint32_t at_v0 = a4_keep(piece(t)), at_v1 = a4_keep(piece(4 + (t ^ 1)));
+    auto piece_at = [&](int pos) { return ring + (A4_TILE + pos) * X::ROW + (((2 * NB * r >> 4) ^ X::swizzle(pos)) << 4) + (2 * NB * r & 15); };
+    const uint32_t at_v0 = a4_keep(piece_at(t)), at_v1 = a4_keep(piece_at(4 + (t ^ 1)));
 
-    for (long at = begin; at < end;) {
-        // ---- one segment: units [u0, u1) of (sequence b, kv head, block of q heads) -------------------------------------------
-        int n = units_of(b);
-        while (at >= start + (long)n * per_seq) {
-            start += (long)n * per_seq;
-            n = units_of(++b);
-        }
-        const int len = length(b);
-        const int item = (int)((at - start) / n);
-        const long item_start = start + (long)item * n;
-        const int u0 = (int)(at - item_start), u1 = (int)min((long)n, end - item_start);
-        const int kvh = item / A.head_blocks, h0 = kvh * gqa + (item % A.head_blocks) * A4_HEADS;
-        const int heads = min(A4_HEADS, (kvh + 1) * gqa - h0);
-        at = item_start + u1;
-
-        // Tile i of this warp goes to stage i % STAGES.  16 neighbouring rows are one linear piece of the cache, so a tile that is
-        // whole and lies in one block takes nothing but copies at fixed distances; the loops below are unrolled over the stages,
-        // which makes the distances of a head-major cache constants (`ahead` tiles from the pointers).
-        const int tiles = u1 - u0;
-        const bool paged = C.block_table != nullptr, one = !paged || C.block_size % A4_TILE == 0;
-        // head-major: this many tiles are whole
-        const int whole = paged ? 0 : min(max((len - (warp + 1) * A4_TILE + A4_UNIT) / A4_UNIT - u0, 0), tiles);
-        const long row0 = ((long)b * C.heads + kvh) * C.capacity + u0 * A4_UNIT + warp * A4_TILE;
-        const unsigned char *src_k = (const unsigned char *)C.k_codes + row0 * X::ROW + lane * 16;
-        const unsigned char *src_v = (const unsigned char *)C.v_codes + row0 * X::ROW + lane * 16;
-        const unsigned char *src_p = params + row0 * X::PROW;
-        auto copy_whole = [&](uint32_t stage, const unsigned char *k, const unsigned char *v, const unsigned char *p) {
+    // ---- streaming a piece: tile i of this warp goes to stage i % STAGES ------------------------------------------------------------
+    // 16 neighbouring rows are one linear part of the cache, so a tile that is whole and lies in one block takes nothing but
+    // copies at fixed distances
+    int tiles, whole;                      // tiles of this segment; so many from the first on are whole (head-major caches)
+    const unsigned char *src_k = nullptr, *src_v = nullptr, *src_p = nullptr;
+    const bool paged = C.block_table != nullptr;
+    auto params = [&] { return (const unsigned char *)(lane < 16 ? C.k_params : C.v_params) + (lane & 15) * X::PROW; };
+    auto row_at = [&](const Attn4Segment &d, int i) { return ((long)d.b * C.heads + d.kvh) * C.capacity + (d.u0 + i) * A4_UNIT + warp * A4_TILE; };
+    auto copy_whole = [&](uint32_t stage, const unsigned char *k, const unsigned char *v, const unsigned char *p) {
 #pragma unroll
-            for (int c = 0; c < NB; c += 2)
-                if (c + 1 < NB || lane < 16) {
-                    a4_copy<16>(dst_codes + stage + c * 256, k + c * 256, 16);
-                    a4_copy<16>(dst_codes + stage + A4_TILE * X::ROW + c * 256, v + c * 256, 16);
-                }
-#pragma unroll
-            for (int c = 0; c < X::PROW; c += X::PCOPY) a4_copy<X::PCOPY>(dst_params + stage + c, p + c, X::PCOPY);
-        };
-        auto issue = [&](int i, int stage, int ahead) {
-            const uint32_t st = stage * X::STAGE;
-            if (i < whole) {
-                copy_whole(st, src_k + ahead * A4_UNIT * X::ROW, src_v + ahead * A4_UNIT * X::ROW, src_p + ahead * A4_UNIT * X::PROW);
-            } else if (i < tiles) {
-                const int p0 = (u0 + i) * A4_UNIT + warp * A4_TILE;
-                long first = row0 + (long)i * A4_UNIT;
-                if (paged && one && p0 < len) {
-                    const int lb = (int)__umul64hi((unsigned long long)p0, A.block_magic);
-                    const int blk = C.block_table[(long)b * C.max_blocks + lb];
-                    first = (unsigned)blk < (unsigned)C.num_blocks ? ((long)blk * C.heads + kvh) * C.block_size + (p0 - lb * C.block_size) : -1;
-                }
-                const uint32_t mask = ring + st + X::STAGE - 16;
-                if (one && p0 + A4_TILE <= len && first >= 0) {
-                    copy_whole(st, (const unsigned char *)C.k_codes + first * X::ROW + lane * 16, (const unsigned char *)C.v_codes + first * X::ROW + lane * 16,
-                               params + first * X::PROW);
-                    if (lane == 0) asm volatile("st.shared.u32 [%0], %1;" ::"r"(mask), "r"(0xffffu) : "memory");
-                } else {
-                    auto row_of = [&](int row) {           // -1: behind the context, or in a block that the pool does not have
-                        if (p0 + row >= len) return -1l;
-                        if (one) return first < 0 ? -1l : first + row;
-                        return kv4_row(C, b, kvh, p0 + row);
-                    };
-#pragma unroll 1
-                    for (int c = lane; c < A4_TILE * NB; c += 32) {
-                        const long row = row_of(c / NB);
-                        const long off = max(row, 0l) * X::ROW + (c % NB) * 16;
-                        const uint32_t dst = dst_codes + st + (c - lane) * 16;
-                        a4_copy<16>(dst, (const unsigned char *)C.k_codes + off, row < 0 ? 0 : 16);
-                        a4_copy<16>(dst + A4_TILE * X::ROW, (const unsigned char *)C.v_codes + off, row < 0 ? 0 : 16);
-                    }
-                    const long row = row_of(lane & 15);
-#pragma unroll
-                    for (int c = 0; c < X::PROW; c += X::PCOPY)
-                        a4_copy<X::PCOPY>(dst_params + st + c, params + (row < 0 ? 0 : row - (lane & 15)) * X::PROW + c, row < 0 ? 0 : X::PCOPY);
-                    const unsigned valid = __ballot_sync(0xffffffffu, row >= 0) & 0xffffu;
-                    if (lane == 0) {
-                        asm volatile("st.shared.u32 [%0], %1;" ::"r"(mask), "r"(valid) : "memory");
-                        const int rows = min(A4_TILE, len - p0);
-                        if (rows > 0 && __popc(valid) != rows) atomicOr(A.status, KV4_BAD_BLOCK);
-                    }
-                }
+        for (int c = 0; c < NB; c += 2)
+            if (c + 1 < NB || lane < 16) {
+                a4_copy<16>(dst_codes + stage + c * 256, k + c * 256, 16);
+                a4_copy<16>(dst_codes + stage + A4_TILE * X::ROW + c * 256, v + c * 256, 16);
             }
-            asm volatile("cp.async.commit_group;" ::: "memory");
-        };
 #pragma unroll
-        for (int i = 0; i < A4_STAGES - 1; ++i) issue(i, i, i);
+        for (int c = 0; c < X::PROW; c += X::PCOPY) a4_copy<X::PCOPY>(dst_params + stage + c, p + c, X::PCOPY);
+    };
+    auto issue = [&](const Attn4Segment &d, int i, int stage) {
+        const uint32_t st = stage * X::STAGE;
+        if (i < whole) {
+            copy_whole(st, src_k, src_v, src_p);
+            src_k += A4_UNIT * X::ROW;
+            src_v += A4_UNIT * X::ROW;
+            src_p += A4_UNIT * X::PROW;
+        } else if (i < tiles) {
+            const int p0 = (d.u0 + i) * A4_UNIT + warp * A4_TILE;
+            const bool one = !paged || C.block_size % A4_TILE == 0;
+            long first = row_at(d, i);
+            if (paged && one && p0 < d.len) {
+                const int lb = (int)__umul64hi((unsigned long long)p0, A.block_magic);
+                const int blk = C.block_table[(long)d.b * C.max_blocks + lb];
+                first = (unsigned)blk < (unsigned)C.num_blocks ? ((long)blk * C.heads + d.kvh) * C.block_size + (p0 - lb * C.block_size) : -1;
+            }
+            const uint32_t mask = ring + st + X::STAGE - 16;
+            if (one && p0 + A4_TILE <= d.len && first >= 0) {
+                copy_whole(st, (const unsigned char *)C.k_codes + first * X::ROW + lane * 16, (const unsigned char *)C.v_codes + first * X::ROW + lane * 16,
+                           params() + first * X::PROW);
+                if (lane == 0) asm volatile("st.shared.u32 [%0], %1;" ::"r"(mask), "r"(0xffffu) : "memory");
+            } else {
+                a4_copy_edge<NB, NG>(A, d.b, d.kvh, p0, d.len, first, one, dst_codes + st, dst_params + st, params(), mask);
+            }
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+#pragma unroll 1
+    for (;;) {
+        if (tid == 0) {                    // the segment that begins with unit `at`
+            Attn4Segment d = sm_seg;       // its sequence and the units before that, or those of the segment before
+            unsigned seq_start = d.item_start, n = units_of(d.b);
+            while (at >= seq_start + n * per_seq) {
+                seq_start += n * per_seq;
+                n = units_of(++d.b);
+            }
+            const unsigned ctx = (at - seq_start) / n, hb = ctx % A.head_blocks, gqa = A.hq / C.heads;
+            d.item_start = seq_start;
+            d.kvh = ctx / A.head_blocks;
+            d.h0 = d.kvh * gqa + hb * A4_HEADS;
+            d.heads = min((unsigned)A4_HEADS, gqa - hb * A4_HEADS);
+            d.len = min(A.lens[d.b], C.capacity);
+            d.n = n;
+            d.u0 = at - seq_start - ctx * n;
+            d.u1 = min(n, d.u0 + (end - at));
+            sm_seg = d;
+        }
+        __syncthreads();
+        const Attn4Segment &d = sm_seg;
+        tiles = d.u1 - d.u0;
+        whole = paged ? 0 : min(max((d.len - (warp + 1) * A4_TILE + A4_UNIT) / A4_UNIT - d.u0, 0), tiles);
+        const long row0 = row_at(d, 0);
+        src_k = (const unsigned char *)C.k_codes + row0 * X::ROW + lane * 16;
+        src_v = (const unsigned char *)C.v_codes + row0 * X::ROW + lane * 16;
+        src_p = params() + row0 * X::PROW;
+#pragma unroll 1
+        for (int i = 0; i < A4_STAGES - 1; ++i) issue(d, i, i);
 
-        // ---- q as the B operand: head r, lane t's dims; scaled by a power of two to [2^14, 2^15) ----------------------------------
+        // ---- q as the B operand, a word by each warp; scaled by a power of two to [2^14, 2^15) -------------------------------------------
         // (any 16-bit type then fits fp16 with all its bits, down to 2^-25 of the head's largest element; nibbles 1 and 3 carry
         // 2^4 more than 0 and 2, so their q is divided by 16)
-        uint32_t qf[4 * NB];
-        float qsum[NG][2], fac[2];             // of heads 2t and 2t + 1: sum of q over a group, and what a score is multiplied by
         {
-            // word i's dims: 4 + 4 (two blocks), or 8 in a row (one block)
-            uint32_t raw[NB][4];
-            const uint16_t *qrow = (const uint16_t *)A.q + ((long)b * A.hq + h0 + (r < heads ? r : 0)) * X::D;
-#pragma unroll
-            for (int i = 0; i < NB; ++i) {
+            // head r, lane t's dims: of operand word i 4 + 4 (two blocks), or 8 in a row (one block)
+            const uint16_t *qrow = (const uint16_t *)A.q + ((long)d.b * A.hq + d.h0 + (r < d.heads ? r : 0)) * X::D;
+            auto word = [&](int i) {
                 int lo, hi;
                 a4_kdims<NB, X::PURE>(i, 0, t, lo, hi);
-                if constexpr (X::PURE) {
-                    const uint4 u = *reinterpret_cast<const uint4 *>(qrow + lo);
-                    raw[i][0] = u.x; raw[i][1] = u.y; raw[i][2] = u.z; raw[i][3] = u.w;
-                } else {
-                    const uint2 u = *reinterpret_cast<const uint2 *>(qrow + lo), w = *reinterpret_cast<const uint2 *>(qrow + hi);
-                    raw[i][0] = u.x; raw[i][1] = u.y; raw[i][2] = w.x; raw[i][3] = w.y;
-                }
-            }
-            auto pick = [&](int i, int n) {      // n 0-3: the low half's dims, 4-7: the high half's
-                const uint32_t x = r < heads ? raw[i][n >> 1] : 0u;
-                if (A.bf16) return __uint_as_float(n & 1 ? x & 0xffff0000u : x << 16);
-                const float2 f = h2_to_f2(x);
-                return n & 1 ? f.y : f.x;
+                if constexpr (X::PURE) return *reinterpret_cast<const uint4 *>(qrow + lo);
+                const uint2 u = *reinterpret_cast<const uint2 *>(qrow + lo), w = *reinterpret_cast<const uint2 *>(qrow + hi);
+                return make_uint4(u.x, u.y, w.x, w.y);
             };
-            float big = 0.f;
+            uint32_t top2 = 0;                 // the largest magnitude: its bits order like the value, in either type
 #pragma unroll
-            for (int i = 0; i < NB; ++i)
-#pragma unroll
-                for (int nn = 0; nn < 8; ++nn) big = fmaxf(big, fabsf(pick(i, nn)));
-            big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
-            big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
-            const int k = min(14 - ((int)(__float_as_uint(big) >> 23) - 127), 126);
-            const float up = copysignf(__uint_as_float((uint32_t)(k + 127) << 23), A.scale_log2e);
-            float sum[NG] = {};
-#pragma unroll
-            for (int i = 0; i < NB; ++i)
-#pragma unroll
-                for (int nn = 0; nn < 4; ++nn) {
-                    const float a = pick(i, nn) * up, c = pick(i, nn + 4) * up;
-                    sum[a4_kgroup<NB, NG, X::PURE>(i)] += a + c;
-                    qf[4 * i + nn] = (nn & 1) ? f2_to_h2(a * 0.0625f, c * 0.0625f) : f2_to_h2(a, c);
-                }
-            // an infinite q has no finite score: NaN, as inf - inf gives
-            const float f = big < INFINITY ? fabsf(A.scale_log2e) / fabsf(up) * 16777216.f : NAN;
-#pragma unroll
-            for (int g = 0; g < NG; ++g) {
-                sum[g] += __shfl_xor_sync(0xffffffffu, sum[g], 1);
-                sum[g] += __shfl_xor_sync(0xffffffffu, sum[g], 2);
-                sum[g] *= 1.f / 16777216.f;
-                qsum[g][0] = __shfl_sync(0xffffffffu, sum[g], 8 * t);
-                qsum[g][1] = __shfl_sync(0xffffffffu, sum[g], 8 * t + 4);
+            for (int i = 0; i < NB; ++i) {
+                const uint4 u = word(i);
+                top2 = __vmaxu2(__vmaxu2(top2, u.x & 0x7fff7fffu), __vmaxu2(u.y & 0x7fff7fffu, __vmaxu2(u.z & 0x7fff7fffu, u.w & 0x7fff7fffu)));
             }
-            fac[0] = __shfl_sync(0xffffffffu, r < heads ? f : 0.f, 8 * t);
-            fac[1] = __shfl_sync(0xffffffffu, r < heads ? f : 0.f, 8 * t + 4);
+            top2 = max(top2 & 0xffffu, top2 >> 16);
+            top2 = max(top2, __shfl_xor_sync(0xffffffffu, top2, 1));
+            top2 = max(top2, __shfl_xor_sync(0xffffffffu, top2, 2));
+            const float big = A.bf16 ? __uint_as_float(top2 << 16) : __half2float(__ushort_as_half((unsigned short)top2));
+            const int k = min(14 - ((int)(__float_as_uint(big) >> 23) - 127), 126);
+            const float up = r < d.heads ? copysignf(__uint_as_float((uint32_t)(k + 127) << 23), A.scale_log2e) : 0.f, up16 = up * 0.0625f;
+#pragma unroll 1
+            for (int i = warp; i < NB; i += A4_WARPS) {
+                const uint4 u = word(i);       // u.x, u.y: dims 0-3 of the low half, u.z, u.w of the high one
+                float f[8];
+                if (A.bf16) {
+                    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+                    for (int e2 = 0; e2 < 4; ++e2) { f[2 * e2] = __uint_as_float(w[e2] << 16); f[2 * e2 + 1] = __uint_as_float(w[e2] & 0xffff0000u); }
+                } else {
+                    const float2 w[4] = {h2_to_f2(u.x), h2_to_f2(u.y), h2_to_f2(u.z), h2_to_f2(u.w)};
+#pragma unroll
+                    for (int e2 = 0; e2 < 4; ++e2) { f[2 * e2] = w[e2].x; f[2 * e2 + 1] = w[e2].y; }
+                }
+#pragma unroll
+                for (int e2 = 0; e2 < 8; ++e2) f[e2] *= e2 & 1 ? up16 : up;
+                if (r >= d.heads) f[0] = f[1] = f[2] = f[3] = f[4] = f[5] = f[6] = f[7] = 0.f;     // another head's row stood in
+                sm_q[i][lane] = make_uint4(f2_to_h2(f[0], f[4]), f2_to_h2(f[1], f[5]), f2_to_h2(f[2], f[6]), f2_to_h2(f[3], f[7]));
+                float sum = fmaf((f[1] + f[5]) + (f[3] + f[7]), 16.f, (f[0] + f[4]) + (f[2] + f[6]));
+                sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+                sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+                if (t == 0) sm_qsum[i][r] = sum * (1.f / 16777216.f);
+            }
+            // what a score is multiplied by; a q with an infinity or a NaN has no finite score: NaN
+            if (warp == 0 && t == 0) sm_fac[r] = r >= d.heads ? 0.f : big < INFINITY ? fabsf(A.scale_log2e) / fabsf(up) * 16777216.f : NAN;
+        }
+        __syncthreads();
+        float qsum[NG][2], fac[2];             // of heads 2t and 2t + 1
+#pragma unroll
+        for (int e2 = 0; e2 < 2; ++e2) {
+            fac[e2] = sm_fac[2 * t + e2];
+#pragma unroll
+            for (int g = 0; g < NG; ++g) qsum[g][e2] = 0.f;
+#pragma unroll
+            for (int i = 0; i < NB; ++i) qsum[a4_kgroup<NB, NG, X::PURE>(i)][e2] += sm_qsum[i][2 * t + e2];
         }
 
         float oacc[X::MTILES][4], zacc[NG][2], l[2] = {0.f, 0.f};
@@ -379,14 +438,15 @@ attn4_kernel(const __grid_constant__ Attn4Args A) {
         // top: the running maximum of the raw scores; a probability is 2^(score fac - ref), ref = top fac - e: the factor 2^e,
         // the same for all heads, keeps probability times value scale inside fp16 and cancels in the end
         float top[2] = {-1e30f, -1e30f}, ref[2] = {0.f, 0.f}, bar[2] = {-1e30f, -1e30f}, e = 0.f, most = -1.f;
-        if (!(fac[0] > 0.f)) { top[0] = 0.f; bar[0] = INFINITY; ref[0] = 0.f; }
-        if (!(fac[1] > 0.f)) { top[1] = 0.f; bar[1] = INFINITY; ref[1] = 0.f; }
+        if (!(fac[0] > 0.f)) { top[0] = 0.f; bar[0] = INFINITY; }
+        if (!(fac[1] > 0.f)) { top[1] = 0.f; bar[1] = INFINITY; }
 
-        auto tile = [&](int i, int stage) {
+#pragma unroll 1
+        for (int i = 0, stage = 0; i < tiles; ++i, stage = stage == A4_STAGES - 1 ? 0 : stage + 1) {
             asm volatile("cp.async.wait_group %0;" ::"n"(A4_STAGES - 2) : "memory");
             __syncwarp();
-            issue(i + A4_STAGES - 1, (stage + A4_STAGES - 1) % A4_STAGES, stage + A4_STAGES - 1);
-            const int st = stage * X::STAGE;
+            issue(d, i + A4_STAGES - 1, stage == 0 ? A4_STAGES - 1 : stage - 1);
+            const uint32_t st = stage * X::STAGE;
             const bool edge = i >= whole;         // some rows may have to be left out
             bool ok0 = true, ok1 = true;
             if (edge) {
@@ -423,10 +483,11 @@ attn4_kernel(const __grid_constant__ Attn4Args A) {
                         uint32_t x0, x1, x2, x3, y0, y1, y2, y3;
                         a4_codes(x, x0, x1, x2, x3);
                         a4_codes(y, y0, y1, y2, y3);
-                        if (begun) a4_mma(acc, x0, y0, x1, y1, qf[4 * j], qf[4 * j + 1]);
-                        else a4_mma0(acc, x0, y0, x1, y1, qf[4 * j], qf[4 * j + 1]);
+                        const uint4 q4 = sm_q[j][lane];
+                        if (begun) a4_mma(acc, x0, y0, x1, y1, q4.x, q4.y);
+                        else a4_mma0(acc, x0, y0, x1, y1, q4.x, q4.y);
                         begun = true;
-                        a4_mma(acc, x2, y2, x3, y3, qf[4 * j + 2], qf[4 * j + 3]);
+                        a4_mma(acc, x2, y2, x3, y3, q4.z, q4.w);
                     }
                     s[0] = fmaf(s0[g], acc[0], fmaf(z0[g], qsum[g][0], s[0]));
                     s[1] = fmaf(s0[g], acc[1], fmaf(z0[g], qsum[g][1], s[1]));
@@ -518,19 +579,9 @@ attn4_kernel(const __grid_constant__ Attn4Args A) {
                     out_tiles(j, a4_lds16(at_v0 + st + 2 * j) | a4_lds16(at_v1 + st + 2 * j) << 16,
                               a4_lds16(at_v0 + st + 8 * X::ROW + 2 * j) | a4_lds16(at_v1 + st + 8 * X::ROW + 2 * j) << 16);
             }
-        };
-#pragma unroll 1
-        for (int i = 0; i < tiles; i += A4_STAGES) {
-#pragma unroll
-            for (int stage = 0; stage < A4_STAGES; ++stage)
-                if (i + stage < tiles) tile(i + stage, stage);
-            src_k += A4_STAGES * A4_UNIT * X::ROW;
-            src_v += A4_STAGES * A4_UNIT * X::ROW;
-            src_p += A4_STAGES * A4_UNIT * X::PROW;
         }
-        asm volatile("cp.async.wait_group 0;" ::: "memory");
 
-        // ---- join the warps ----------------------------------------------------------------------------------------------
+        // ---- join the warps ------------------------------------------------------------------------------------------------------
 #pragma unroll
         for (int o = 4; o <= 16; o <<= 1) {
             l[0] += __shfl_xor_sync(0xffffffffu, l[0], o);
@@ -579,7 +630,7 @@ attn4_kernel(const __grid_constant__ Attn4Args A) {
             }
         }
         __syncthreads();
-        const int two = heads > 4, quads = 1 + two;       // groups of four heads that exist
+        const int two = d.heads > 4, quads = 1 + two;      // groups of four heads that exist
         // the sum over the warps of float4 i & two of m-tile row i >> two
         auto sum4 = [&](int i) {
             const float4 *s4 = reinterpret_cast<const float4 *>(so) + (i >> two) * 2 + (i & two);
@@ -591,87 +642,116 @@ attn4_kernel(const __grid_constant__ Attn4Args A) {
             }
             return o;
         };
-        auto finish = [&] {                                // the output rows of these heads
+        // ---- join the CTAs: partial results through the workspace, A4_FAN neighbours by the last of them to arrive, and so on with
+        // these sums, always in CTA order -------------------------------------------------------------------------------------------
+        bool last = true;
+        if (d.u1 - d.u0 < d.n) {           // not the whole context was here
+            const unsigned first = at - d.u0, c0 = first / share;       // units before this context; the CTA it begins in
+            int members = (first + d.n - 1) / share - c0 + 1, me = blockIdx.x - c0, step = 1;
+            // a CTA has two places: for a context that it continues, and for one that it begins
+            auto place = [&](int c) { return (int)(c0 + c) * 2 + (c == 0); };
+            int *counters = A.counters;
+#pragma unroll 1
+            while (members > 1) {
+                const int lead = me / A4_FAN * A4_FAN, count = min(A4_FAN, members - lead);
+                float *part = A.parts + (long)place(me * step) * X::PART;
+#pragma unroll 1
+                for (int i = tid; i < X::D * quads; i += A4_THREADS) reinterpret_cast<float4 *>(part)[(i >> two) * 2 + (i & two)] = sum4(i);
+                if (tid < A4_HEADS) reinterpret_cast<float2 *>(part + X::D * A4_HEADS)[tid] = make_float2(sm_top[tid], sm_sum[tid]);
+                __syncthreads();
+                if (tid == 0) {
+                    __threadfence();       // orders the whole block's stores: the barrier came before it
+                    sm_last = atomicAdd(&counters[place(lead * step)], 1) == count - 1;
+                    if (sm_last) counters[place(lead * step)] = 0;      // ready for the next launch
+                    __threadfence();
+                }
+                __syncthreads();
+                last = sm_last;
+                if (!last) break;
+                // every thread one (part, head): the weights 2^(m - M); every warp a quarter of the parts, all loads under way at once
+                static_assert(A4_FAN * A4_HEADS == A4_THREADS && A4_FAN == 4 * A4_WARPS, "a thread for every part and head");
+                auto part_at = [&](int c) { return A.parts + (long)place((lead + c) * step) * X::PART; };
+                const int c = tid >> 3, h = tid & 7;
+                float2 ml = make_float2(0.f, 0.f);
+                if (c < count) ml = __ldcg(reinterpret_cast<const float2 *>(part_at(c) + X::D * A4_HEADS) + h);
+                constexpr int DEEP = X::D / 32 < 4 ? X::D / 32 : 4;
+#pragma unroll 1
+                for (int i0 = lane; i0 < X::D * quads; i0 += 32 * DEEP) {
+                    float4 x[DEEP][4];
+#pragma unroll
+                    for (int j = 0; j < DEEP; ++j)
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            const int i = i0 + 32 * j;
+                            x[j][k] = make_float4(0.f, 0.f, 0.f, 0.f);
+                            if (warp * 4 + k < count && i < X::D * quads)
+                                x[j][k] = __ldcg(reinterpret_cast<const float4 *>(part_at(warp * 4 + k)) + (i >> two) * 2 + (i & two));
+                        }
+                    if (i0 == lane) {
+                        float M = ml.y == 0.f ? -INFINITY : ml.x;
+                        M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, 8));
+                        M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, 16));
+                        if (lane < 8) sm_ref[warp][lane] = M;
+                        __syncthreads();
+#pragma unroll
+                        for (int w = 0; w < A4_WARPS; ++w) M = fmaxf(M, sm_ref[w][h]);
+                        const float wt = ml.y == 0.f ? 0.f : a4_exp2(ml.x - M);
+                        float L = ml.y * wt;
+                        sm_wt[c][h] = wt;
+                        L += __shfl_xor_sync(0xffffffffu, L, 8);
+                        L += __shfl_xor_sync(0xffffffffu, L, 16);
+                        if (lane < 8) sm_l[warp][lane] = L;
+                        __syncthreads();
+                        if (tid < A4_HEADS) {
+                            sm_top[tid] = M;
+                            sm_sum[tid] = sm_l[0][tid] + sm_l[1][tid] + sm_l[2][tid] + sm_l[3][tid];
+                        }
+                    }
+#pragma unroll
+                    for (int j = 0; j < DEEP; ++j) {
+                        const int i = i0 + 32 * j, at4 = (i >> two) * 2 + (i & two);
+                        if (i >= X::D * quads) break;
+                        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            const float4 w = *reinterpret_cast<const float4 *>(&sm_wt[warp * 4 + k][4 * (at4 & 1)]);
+                            o.x = fmaf(w.x, x[j][k].x, o.x); o.y = fmaf(w.y, x[j][k].y, o.y); o.z = fmaf(w.z, x[j][k].z, o.z); o.w = fmaf(w.w, x[j][k].w, o.w);
+                        }
+                        reinterpret_cast<float4 *>(so + warp * X::D * A4_HEADS)[at4] = o;
+                    }
+                }
+                __syncthreads();
+                me /= A4_FAN;
+                members = (members + A4_FAN - 1) / A4_FAN;
+                step *= A4_FAN;
+                counters += 2 * A4_MAX_CTAS;       // a level's own counters
+            }
+        }
+        if (last) {                        // the output rows of these heads
+#pragma unroll 1
             for (int i = tid; i < X::D * quads; i += A4_THREADS) {
                 const float4 o4 = sum4(i);
                 const float o[4] = {o4.x, o4.y, o4.z, o4.w};
-                const int idx = i >> two, m = idx >> 4, row = idx & 15, d = 32 * (m >> 1) + 4 * (row & 7) + 2 * (m & 1) + (row >> 3);
-                const int e7 = d & 7, dd = A.out_kperm ? (d & ~7) | (e7 < 4 ? 2 * e7 : 2 * e7 - 7) : d;
+                const int idx = i >> two, m = idx >> 4, row = idx & 15, dim = 32 * (m >> 1) + 4 * (row & 7) + 2 * (m & 1) + (row >> 3);
+                const int e7 = dim & 7, dd = A.out_kperm ? (dim & ~7) | (e7 < 4 ? 2 * e7 : 2 * e7 - 7) : dim;
 #pragma unroll
                 for (int e4 = 0; e4 < 4; ++e4) {
                     const int h = 4 * (i & two) + e4;
-                    if (h >= heads) break;
-                    const float v = sm_sum[h] == 0.f ? 0.f : o[e4] / sm_sum[h];      // nothing but blocks outside the pool: 0
-                    const long at_out = ((long)b * A.hq + h0 + h) * X::D + dd;
+                    if (h >= d.heads) break;
+                    const float v = sm_sum[h] == 0.f ? 0.f : __fdividef(o[e4], sm_sum[h]);   // nothing but blocks outside the pool: 0
+                    const long at_out = ((long)d.b * A.hq + d.h0 + h) * X::D + dd;
                     if (A.bf16) reinterpret_cast<__nv_bfloat16 *>(A.out)[at_out] = __float2bfloat16_rn(v);
                     else reinterpret_cast<__half *>(A.out)[at_out] = __float2half_rn(v);
                 }
             }
-        };
-        if (u0 == 0 && u1 == n) {          // the whole context was here
-            finish();
-            __syncthreads();
-            continue;
         }
-        // ---- join the CTAs: partial results through the workspace, the last to arrive adds them up in CTA order ------------------
-        const int c0 = (int)(item_start / share), c1 = (int)((item_start + n - 1) / share);
-        float *part = A.parts + ((long)cta * 2 + (u0 == 0)) * X::PART;
-        for (int i = tid; i < X::D * quads; i += A4_THREADS) reinterpret_cast<float4 *>(part)[(i >> two) * 2 + (i & two)] = sum4(i);
-        if (tid < A4_HEADS) reinterpret_cast<float2 *>(part + X::D * A4_HEADS)[tid] = make_float2(sm_top[tid], sm_sum[tid]);
-        __threadfence();
-        __syncthreads();
-        if (tid == 0) sm_last = atomicAdd(&A.counters[c0], 1) == c1 - c0;
-        __syncthreads();
-        if (sm_last) {
-            __threadfence();
-            // weights 2^(m_c - M) of the parts to shared memory (behind the results), then the parts dealt out to the warps,
-            // each lane with several loads in flight, then the warps' sums in order
-            const int parts = c1 - c0 + 1;
-            float *wt = so + A4_WARPS * X::D * A4_HEADS;       // [part][head]
-            auto part_of = [&](int c) { return A.parts + ((long)(c0 + c) * 2 + (c == 0)) * X::PART; };
-            const int h = tid & 7;
-            float M = -INFINITY, L = 0.f;
-            for (int c = tid >> 3; c < parts; c += A4_THREADS / 8) {
-                const float2 ml = __ldcg(reinterpret_cast<const float2 *>(part_of(c) + X::D * A4_HEADS) + h);
-                if (ml.y != 0.f) M = fmaxf(M, ml.x);
-            }
-            M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, 8));
-            M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, 16));
-            if (lane < 8) sm_ref[warp][lane] = M;
-            __syncthreads();
-#pragma unroll
-            for (int w = 0; w < A4_WARPS; ++w) M = fmaxf(M, sm_ref[w][h]);
-            for (int c = tid >> 3; c < parts; c += A4_THREADS / 8) {
-                const float2 ml = __ldcg(reinterpret_cast<const float2 *>(part_of(c) + X::D * A4_HEADS) + h);
-                const float x = ml.y == 0.f ? 0.f : a4_exp2(ml.x - M);
-                wt[c * A4_HEADS + h] = x;
-                L += ml.y * x;
-            }
-            L += __shfl_xor_sync(0xffffffffu, L, 8);
-            L += __shfl_xor_sync(0xffffffffu, L, 16);
-            if (lane < 8) sm_l[warp][lane] = L;
-            __syncthreads();
-            if (tid < A4_HEADS) sm_sum[tid] = sm_l[0][tid] + sm_l[1][tid] + sm_l[2][tid] + sm_l[3][tid];
-            for (int i = lane; i < X::D * quads; i += 32) {
-                const int at4 = (i >> two) * 2 + (i & two);
-                float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
-                for (int c = warp; c < parts; c += A4_WARPS) {
-                    const float4 x = __ldcg(reinterpret_cast<const float4 *>(part_of(c)) + at4);
-                    const float4 w = *reinterpret_cast<const float4 *>(wt + c * A4_HEADS + 4 * (at4 & 1));
-                    o.x = fmaf(w.x, x.x, o.x); o.y = fmaf(w.y, x.y, o.y); o.z = fmaf(w.z, x.z, o.z); o.w = fmaf(w.w, x.w, o.w);
-                }
-                reinterpret_cast<float4 *>(so + warp * X::D * A4_HEADS)[at4] = o;
-            }
-            __syncthreads();
-            finish();
-            if (tid == 0) A.counters[c0] = 0;      // ready for the next launch
-        }
+        at += d.u1 - d.u0;
+        if (at >= end) break;
         __syncthreads();
     }
 }
 
-// Workspace: the status word, the arrival counters (one per CTA) from byte 256, and from 128 KiB the partial results.
+// Workspace: the status word, the arrival counters from byte 256, and from 128 KiB the partial results.
 constexpr size_t A4_COUNTERS_OFF = 256, A4_PARTS_OFF = 128 * 1024;
 static size_t attn4_ws_bytes(int d) { return A4_PARTS_OFF + (size_t)A4_MAX_CTAS * 2 * (d * A4_HEADS + 16) * sizeof(float); }
 
@@ -681,8 +761,8 @@ static int attn4_launch_as(const char *name, const Attn4Args &A, long max_units,
     static OncePerDevice once;
     cudaError_t e = once.run([&] { return cudaFuncSetAttribute(attn4_kernel<NB, NG>, cudaFuncAttributeMaxDynamicSharedMemorySize, X::SMEM); });
     if (e != cudaSuccess) return fail((int)e, "%s: shared memory %d: %s", name, X::SMEM, cudaGetErrorString(e));
-    const long wave = min((long)sm_count() * X::CTAS, (long)A4_MAX_CTAS);
-    launch_kernel(attn4_kernel<NB, NG>, dim3((unsigned)(max_units < wave ? max_units : wave)), dim3(A4_THREADS), X::SMEM, st, A);
+    const int wave = min(sm_count() * X::CTAS * A4_WAVES, A4_MAX_CTAS);
+    launch_kernel(attn4_kernel<NB, NG>, dim3((unsigned)min(max_units, (long)wave)), dim3(A4_THREADS), X::SMEM, st, A);
     return launch_status(name);
 }
 
@@ -710,6 +790,7 @@ static int attn4_launch(const char *name, const void *q, const Kv4Cache &C, bool
     A.counters = (int *)((unsigned char *)ws + A4_COUNTERS_OFF);
     A.parts = (float *)((unsigned char *)ws + A4_PARTS_OFF);
     const long max_units = (long)batch * C.heads * A.head_blocks * (((long)C.capacity + A4_UNIT - 1) / A4_UNIT);
+    B200K_REQUIRE(max_units < (1l << 31), B200K_E_SHAPE, "%s: batch * num_kv_heads * ceil(gqa / 8) * ceil(positions / 64) = %ld exceeds 31 bits", name, max_units);
     cudaStream_t st = to_stream(stream);
     switch (C.d / 32 * 1000 + C.d / C.g) {
         case 1001: return attn4_launch_as<1, 1>(name, A, max_units, st);
