@@ -24,7 +24,10 @@
 namespace b200k {
 
 #ifndef A4_NSTAGES
-#define A4_NSTAGES 3
+#define A4_NSTAGES 2
+#endif
+#ifndef A4_NSUBS
+#define A4_NSUBS 2
 #endif
 #ifndef A4_EDGE
 #define A4_EDGE __forceinline__
@@ -39,7 +42,8 @@ namespace b200k {
 #define A4_C4 4
 #endif
 constexpr int A4_WARPS = 4, A4_THREADS = 32 * A4_WARPS, A4_STAGES = A4_NSTAGES;
-constexpr int A4_TILE = 16, A4_UNIT = A4_WARPS * A4_TILE;      // positions of a warp's tile, of a unit of work
+constexpr int A4_TILE = 16, A4_SUBS = A4_NSUBS;                // positions of a tile (the rows of an MMA), tiles of a stage
+constexpr int A4_STEP = A4_SUBS * A4_TILE, A4_UNIT = A4_WARPS * A4_STEP;       // positions of a warp's stage, of a unit of work
 constexpr int A4_MAX_CTAS = A4_MAXC;                              // CTAs of a launch
 constexpr int A4_FAN = 16;                                     // partial results that are joined at a time
 constexpr int A4_HEADS = 8;                                    // columns of one MMA
@@ -67,7 +71,8 @@ struct A4 {
     static constexpr int D = 32 * NB, G = D / NG;
     static constexpr int ROW = 16 * NB, PROW = 4 * NG;        // bytes of a row's codes, of its params
     static constexpr int PCOPY = NG % 4 == 0 ? 16 : NG % 2 == 0 ? 8 : 4;      // as wide as a row of params is aligned
-    static constexpr int STAGE = 2 * A4_TILE * (ROW + PROW) + 32;              // a multiple of 32: see at_k
+    static constexpr int SUB = 2 * A4_TILE * (ROW + PROW) + 32;                // bytes of a tile in a stage; a multiple of 32: see at_k
+    static constexpr int STAGE = A4_SUBS * SUB;
     static constexpr int MTILES = 2 * NB;
     static constexpr bool PURE = G == 32;                     // a group is one block: see kword()
     static constexpr int PART = D * A4_HEADS + 16;            // floats of a partial result
@@ -129,9 +134,7 @@ __device__ __forceinline__ uint32_t a4_lds16(uint32_t at) {
     return h;
 }
 template <int NG>
-__device__ __forceinline__ void a4_params(float (&s)[NG], float (&z)[NG], uint32_t at) {
-    uint32_t w[NG];
-    a4_lds<NG>(w, at);
+__device__ __forceinline__ void a4_params(float (&s)[NG], float (&z)[NG], const uint32_t *w) {
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
         const float2 f = h2_to_f2(w[g]);
@@ -280,14 +283,15 @@ attn4_kernel(const __grid_constant__ Attn4Args A) {
     }
 
     const uint32_t ring = smem_u32(smem) + warp * A4_STAGES * X::STAGE;
-    // where this lane's first 16-byte piece goes in a stage, and its row of params; lanes 0-15 copy K params, 16-31 V params
+    // where this lane's first 16-byte piece goes in a tile of a stage, and its row of params: lanes 0-15 copy those of K, 16-31 those
+    // of V, which stand beside them
     const uint32_t dst_codes = a4_keep(ring + (lane / NB) * X::ROW + ((lane % NB) ^ X::swizzle(lane / NB)) * 16);
-    const uint32_t dst_params = a4_keep(ring + 2 * A4_TILE * X::ROW + lane * X::PROW);
+    const uint32_t dst_params = a4_keep(ring + 2 * A4_TILE * X::ROW + ((lane & 15) * 2 + (lane >> 4)) * X::PROW);
     // where it reads: K rows kpos and kpos + 8 (chunk t of a row; two chunks at head_dim 256), their params, and its eighth of V
     // rows t, 4 + (t ^ 1) and these + 8
     const int kpos = a4_pos(r);
     const uint32_t at_k = a4_keep(ring + kpos * X::ROW + (NB == 4 ? (t ^ X::swizzle(kpos)) * 16 : NB == 8 ? ((2 * t) ^ X::swizzle(kpos)) * 16 : t * 4 * NB));
-    const uint32_t at_p = a4_keep(ring + 2 * A4_TILE * X::ROW + kpos * X::PROW);
+    const uint32_t at_p = a4_keep(ring + 2 * A4_TILE * X::ROW + kpos * 2 * X::PROW);
     auto piece_at = [&](int pos) { return ring + (A4_TILE + pos) * X::ROW + (((2 * NB * r >> 4) ^ X::swizzle(pos)) << 4) + (2 * NB * r & 15); };
     const uint32_t at_v0 = a4_keep(piece_at(t)), at_v1 = a4_keep(piece_at(4 + (t ^ 1)));
 
@@ -298,7 +302,7 @@ attn4_kernel(const __grid_constant__ Attn4Args A) {
     const unsigned char *src_k = nullptr, *src_v = nullptr, *src_p = nullptr;
     const bool paged = C.block_table != nullptr;
     auto params = [&] { return (const unsigned char *)(lane < 16 ? C.k_params : C.v_params) + (lane & 15) * X::PROW; };
-    auto row_at = [&](const Attn4Segment &d, int i) { return ((long)d.b * C.heads + d.kvh) * C.capacity + (d.u0 + i) * A4_UNIT + warp * A4_TILE; };
+    auto row_at = [&](const Attn4Segment &d, int i) { return ((long)d.b * C.heads + d.kvh) * C.capacity + (d.u0 + i) * A4_UNIT + warp * A4_STEP; };
     auto copy_whole = [&](uint32_t stage, const unsigned char *k, const unsigned char *v, const unsigned char *p) {
 #pragma unroll
         for (int c = 0; c < NB; c += 2)
@@ -309,29 +313,33 @@ attn4_kernel(const __grid_constant__ Attn4Args A) {
 #pragma unroll
         for (int c = 0; c < X::PROW; c += X::PCOPY) a4_copy<X::PCOPY>(dst_params + stage + c, p + c, X::PCOPY);
     };
-    auto issue = [&](const Attn4Segment &d, int i, int stage) {
-        const uint32_t st = stage * X::STAGE;
+    auto issue = [&](const Attn4Segment &d, int i, uint32_t stage) {
         if (i < whole) {
-            copy_whole(st, src_k, src_v, src_p);
+#pragma unroll
+            for (int s = 0; s < A4_SUBS; ++s)
+                copy_whole(stage + s * X::SUB, src_k + s * A4_TILE * X::ROW, src_v + s * A4_TILE * X::ROW, src_p + s * A4_TILE * X::PROW);
             src_k += A4_UNIT * X::ROW;
             src_v += A4_UNIT * X::ROW;
             src_p += A4_UNIT * X::PROW;
         } else if (i < tiles) {
-            const int p0 = (d.u0 + i) * A4_UNIT + warp * A4_TILE;
             const bool one = !paged || C.block_size % A4_TILE == 0;
-            long first = row_at(d, i);
-            if (paged && one && p0 < d.len) {
-                const int lb = (int)__umul64hi((unsigned long long)p0, A.block_magic);
-                const int blk = C.block_table[(long)d.b * C.max_blocks + lb];
-                first = (unsigned)blk < (unsigned)C.num_blocks ? ((long)blk * C.heads + d.kvh) * C.block_size + (p0 - lb * C.block_size) : -1;
-            }
-            const uint32_t mask = ring + st + X::STAGE - 16;
-            if (one && p0 + A4_TILE <= d.len && first >= 0) {
-                copy_whole(st, (const unsigned char *)C.k_codes + first * X::ROW + lane * 16, (const unsigned char *)C.v_codes + first * X::ROW + lane * 16,
-                           params() + first * X::PROW);
-                if (lane == 0) asm volatile("st.shared.u32 [%0], %1;" ::"r"(mask), "r"(0xffffu) : "memory");
-            } else {
-                a4_copy_edge<NB, NG>(A, d.b, d.kvh, p0, d.len, first, one, dst_codes + st, dst_params + st, params(), mask);
+#pragma unroll 1
+            for (int s = 0; s < A4_SUBS; ++s, stage += X::SUB) {
+                const int p0 = (d.u0 + i) * A4_UNIT + warp * A4_STEP + s * A4_TILE;
+                long first = row_at(d, i) + s * A4_TILE;
+                if (paged && one && p0 < d.len) {
+                    const int lb = (int)__umul64hi((unsigned long long)p0, A.block_magic);
+                    const int blk = C.block_table[(long)d.b * C.max_blocks + lb];
+                    first = (unsigned)blk < (unsigned)C.num_blocks ? ((long)blk * C.heads + d.kvh) * C.block_size + (p0 - lb * C.block_size) : -1;
+                }
+                const uint32_t mask = ring + stage + X::SUB - 32;
+                if (one && p0 + A4_TILE <= d.len && first >= 0) {
+                    copy_whole(stage, (const unsigned char *)C.k_codes + first * X::ROW + lane * 16,
+                               (const unsigned char *)C.v_codes + first * X::ROW + lane * 16, params() + first * X::PROW);
+                    if (lane == 0) asm volatile("st.shared.u32 [%0], %1;" ::"r"(mask), "r"(0xffffu) : "memory");
+                } else {
+                    a4_copy_edge<NB, NG>(A, d.b, d.kvh, p0, d.len, first, one, dst_codes + stage, dst_params + stage, params(), mask);
+                }
             }
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
@@ -359,13 +367,13 @@ attn4_kernel(const __grid_constant__ Attn4Args A) {
         __syncthreads();
         const Attn4Segment &d = sm_seg;
         tiles = d.u1 - d.u0;
-        whole = paged ? 0 : min(max((d.len - (warp + 1) * A4_TILE + A4_UNIT) / A4_UNIT - d.u0, 0), tiles);
+        whole = paged ? 0 : min(max((d.len - (warp + 1) * A4_STEP + A4_UNIT) / A4_UNIT - d.u0, 0), tiles);
         const long row0 = row_at(d, 0);
         src_k = (const unsigned char *)C.k_codes + row0 * X::ROW + lane * 16;
         src_v = (const unsigned char *)C.v_codes + row0 * X::ROW + lane * 16;
         src_p = params() + row0 * X::PROW;
 #pragma unroll 1
-        for (int i = 0; i < A4_STAGES - 1; ++i) issue(d, i, i);
+        for (int i = 0; i < A4_STAGES - 1; ++i) issue(d, i, i * X::STAGE);
 
         // ---- q as the B operand, a word by each warp; scaled by a power of two to [2^14, 2^15) -------------------------------------------
         // (any 16-bit type then fits fp16 with all its bits, down to 2^-25 of the head's largest element; nibbles 1 and 3 carry
@@ -441,23 +449,29 @@ attn4_kernel(const __grid_constant__ Attn4Args A) {
         if (!(fac[0] > 0.f)) { top[0] = 0.f; bar[0] = INFINITY; }
         if (!(fac[1] > 0.f)) { top[1] = 0.f; bar[1] = INFINITY; }
 
+        uint32_t stage = 0;
 #pragma unroll 1
-        for (int i = 0, stage = 0; i < tiles; ++i, stage = stage == A4_STAGES - 1 ? 0 : stage + 1) {
+        for (int i = 0; i < tiles; ++i) {
             asm volatile("cp.async.wait_group %0;" ::"n"(A4_STAGES - 2) : "memory");
             __syncwarp();
-            issue(d, i + A4_STAGES - 1, stage == 0 ? A4_STAGES - 1 : stage - 1);
-            const uint32_t st = stage * X::STAGE;
+            issue(d, i + A4_STAGES - 1, stage == 0 ? (A4_STAGES - 1) * X::STAGE : stage - X::STAGE);
             const bool edge = i >= whole;         // some rows may have to be left out
+#pragma unroll
+            for (int sub = 0; sub < A4_SUBS; ++sub) {
+            const uint32_t st = stage + sub * X::SUB;
             bool ok0 = true, ok1 = true;
             if (edge) {
                 uint32_t valid;
-                a4_lds<1>(&valid, ring + st + X::STAGE - 16);
+                a4_lds<1>(&valid, ring + st + X::SUB - 32);
                 ok0 = (valid >> kpos) & 1;
                 ok1 = (valid >> (kpos + 8)) & 1;
             }
 
             // scores: rows r and r + 8 are positions kpos0 and kpos0 + 8, columns heads 2t and 2t + 1
             float s[4] = {0.f, 0.f, 0.f, 0.f};
+            uint32_t pw0[2 * NG], pw1[2 * NG];     // params of these rows: K's, V's
+            a4_lds<2 * NG>(pw0, at_p + st);
+            a4_lds<2 * NG>(pw1, at_p + st + 16 * X::PROW);
             {
                 uint32_t w0[NB], w1[NB];
                 if constexpr (NB == 8) {
@@ -470,8 +484,8 @@ attn4_kernel(const __grid_constant__ Attn4Args A) {
                     a4_lds<NB>(w1, at_k + st + 8 * X::ROW);
                 }
                 float s0[NG], z0[NG], s1[NG], z1[NG];
-                a4_params<NG>(s0, z0, at_p + st);
-                a4_params<NG>(s1, z1, at_p + st + 8 * X::PROW);
+                a4_params<NG>(s0, z0, pw0);
+                a4_params<NG>(s1, z1, pw1);
 #pragma unroll
                 for (int g = 0; g < NG; ++g) {
                     float acc[4];
@@ -495,9 +509,17 @@ attn4_kernel(const __grid_constant__ Attn4Args A) {
                     s[3] = fmaf(s1[g], acc[3], fmaf(z1[g], qsum[g][1], s[3]));
                 }
             }
+            constexpr int VW = NB % 2 == 0 ? NB / 2 : 1;
+            uint32_t va[VW], vb[VW], vc[VW], vd[VW];
+            if constexpr (NB % 2 == 0) {
+                a4_lds<VW>(va, at_v0 + st);
+                a4_lds<VW>(vb, at_v1 + st);
+                a4_lds<VW>(vc, at_v0 + st + 8 * X::ROW);
+                a4_lds<VW>(vd, at_v1 + st + 8 * X::ROW);
+            }
             float vs0[NG], vz0[NG], vs1[NG], vz1[NG];
-            a4_params<NG>(vs0, vz0, at_p + st + A4_TILE * X::PROW);
-            a4_params<NG>(vs1, vz1, at_p + st + (A4_TILE + 8) * X::PROW);
+            a4_params<NG>(vs0, vz0, pw0 + NG);
+            a4_params<NG>(vs1, vz1, pw1 + NG);
             if (edge) {
                 if (!ok0) s[0] = s[1] = -1e30f;
                 if (!ok1) s[2] = s[3] = -1e30f;
@@ -563,11 +585,6 @@ attn4_kernel(const __grid_constant__ Attn4Args A) {
                 a4_mma(oacc[2 * j + 1], x2, x3, y2, y3, pb[g][0], pb[g][1]);
             };
             if constexpr (NB % 2 == 0) {
-                uint32_t va[NB / 2], vb[NB / 2], vc[NB / 2], vd[NB / 2];
-                a4_lds<NB / 2>(va, at_v0 + st);
-                a4_lds<NB / 2>(vb, at_v1 + st);
-                a4_lds<NB / 2>(vc, at_v0 + st + 8 * X::ROW);
-                a4_lds<NB / 2>(vd, at_v1 + st + 8 * X::ROW);
 #pragma unroll
                 for (int j = 0; j < NB; ++j) {
                     const int sel = j & 1 ? 0x7632 : 0x5410;
@@ -579,6 +596,8 @@ attn4_kernel(const __grid_constant__ Attn4Args A) {
                     out_tiles(j, a4_lds16(at_v0 + st + 2 * j) | a4_lds16(at_v1 + st + 2 * j) << 16,
                               a4_lds16(at_v0 + st + 8 * X::ROW + 2 * j) | a4_lds16(at_v1 + st + 8 * X::ROW + 2 * j) << 16);
             }
+            }
+            stage = stage == (A4_STAGES - 1) * X::STAGE ? 0 : stage + X::STAGE;
         }
 
         // ---- join the warps ------------------------------------------------------------------------------------------------------
