@@ -74,6 +74,7 @@ class Library:
         self._dll = ctypes.CDLL(str(path), mode=ctypes.RTLD_GLOBAL)
         self.protos = parse_header()
         self._fns = {}
+        self._callers = {}
         missing = []
         for name, (ret, args) in self.protos.items():
             try:
@@ -93,6 +94,47 @@ class Library:
     def raw(self, name: str):
         return self._fns[name]
 
+    def caller(self, name: str, tensor_type):
+        """A function of `name`'s arguments that does what `call` does, with the conversions written out for its prototype: a
+        decode step makes a dozen calls of a few microseconds each, and the loop in `call` takes as long as a kernel.
+        `tensor_type` is torch.Tensor (this module does not import torch); anything else goes the way of `call`."""
+        fn = self._callers.get(name)
+        if fn is None:
+            ret, proto = self.protos[name]
+            conv = []
+            for ty, an in proto:
+                if ty == "ptr":
+                    conv.append(f"{an}.data_ptr() if {an}.__class__ is T and {an}.is_cuda else P({an}, {an!r})")
+                elif ty == "b200k_stream":
+                    conv.append(f"{an} if {an}.__class__ is int and {an} else S({an})")
+                elif ty == "float":
+                    conv.append(f"{an} if {an}.__class__ is float else float({an})")
+                else:
+                    conv.append(f"{an} if {an}.__class__ is int else int({an})")
+            check = "    if rc: E(rc)\n" if ret == "int" and name not in _NOT_STATUS else ""
+            src = f"def caller({', '.join(an for _, an in proto)}):\n    rc = F({', '.join(conv)})\n{check}    return rc\n"
+
+            def fail(rc):
+                raise B200KError(name, rc, self.last_error())
+            space = {"T": tensor_type, "F": self._fns[name], "P": lambda a, an: self._pointer(name, an, a), "S": self._stream, "E": fail}
+            exec(compile(src, f"<{name}>", "exec"), space)
+            fn = self._callers[name] = space["caller"]
+        return fn
+
+    @staticmethod
+    def _pointer(name, an, a):
+        if a is None:
+            return None
+        if hasattr(a, "data_ptr"):
+            if not a.is_cuda and not an.startswith("host"):
+                raise ValueError(f"{name}: argument {an} must be a CUDA tensor (no CPU fallback exists)")
+            return a.data_ptr()
+        return int(a)
+
+    @staticmethod
+    def _stream(a):
+        return None if a in (None, 0) else int(getattr(a, "cuda_stream", a))
+
     def call(self, name: str, *args):
         """Call `name`; torch tensors become device pointers; a non-zero status raises."""
         ret, proto = self.protos[name]
@@ -101,16 +143,9 @@ class Library:
         conv = []
         for (ty, an), a in zip(proto, args):
             if ty == "ptr":
-                if a is None:
-                    conv.append(None)
-                elif hasattr(a, "data_ptr"):
-                    if not a.is_cuda and not an.startswith("host"):
-                        raise ValueError(f"{name}: argument {an} must be a CUDA tensor (no CPU fallback exists)")
-                    conv.append(a.data_ptr())
-                else:
-                    conv.append(int(a))
+                conv.append(self._pointer(name, an, a))
             elif ty == "b200k_stream":
-                conv.append(None if a in (None, 0) else int(getattr(a, "cuda_stream", a)))
+                conv.append(self._stream(a))
             elif ty == "float":
                 conv.append(float(a))
             else:

@@ -17,12 +17,21 @@ import torch
 from ._lib import lib
 
 
+def _current_stream():
+    return torch.cuda.current_stream().cuda_stream
+
+
+if hasattr(torch._C, "_cuda_getCurrentRawStream"):   # the same stream without building a Stream object around it
+    def _current_stream():  # noqa: F811
+        return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
+
+
 def _make(name, nargs):
     def fn(*args, stream=None):
+        call = lib().caller(name, torch.Tensor)
         if len(args) == nargs - 1:  # stream omitted
-            st = stream if stream is not None else torch.cuda.current_stream().cuda_stream
-            return lib().call(name, *args, st)
-        return lib().call(name, *args)
+            return call(*args, _current_stream() if stream is None else stream)
+        return call(*args)
     fn.__name__ = name
     fn.__doc__ = f"C ABI `{name}`; see include/b200_kernels.h for the argument list."
     return fn
