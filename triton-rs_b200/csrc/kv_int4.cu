@@ -2,110 +2,197 @@
 //
 // All three kernels are one pass over their rows and bound by memory: an append reads 2 D bytes a row and writes
 // D/2 + 4 D/G, the read-back the other way round.
+#include <type_traits>
+
 #include "kv_int4.cuh"
 
 namespace b200k {
 
-// min / max that keep a NaN (fminf and fmaxf drop it)
-__device__ __forceinline__ float min_nan(float a, float b) {
-    float r;
-    asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-    return r;
+// ---- 16-bit pairs ---------------------------------------------------------------------------------------------------
+template <typename T> struct Kv4Pair;
+template <> struct Kv4Pair<__half> {
+    using type = __half2;
+    __device__ static float2 wide(uint32_t w) { return h2_to_f2(w); }
+};
+template <> struct Kv4Pair<__nv_bfloat16> {
+    using type = __nv_bfloat162;
+    __device__ static float2 wide(uint32_t w) { return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)); }
+};
+// minimum and maximum of both halves; a NaN stays
+template <typename T> __device__ __forceinline__ uint32_t pair_min(uint32_t a, uint32_t b) {
+    using P = typename Kv4Pair<T>::type;
+    const P m = __hmin2_nan(*reinterpret_cast<P *>(&a), *reinterpret_cast<P *>(&b));
+    return *reinterpret_cast<const uint32_t *>(&m);
 }
-__device__ __forceinline__ float max_nan(float a, float b) {
-    float r;
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-    return r;
+template <typename T> __device__ __forceinline__ uint32_t pair_max(uint32_t a, uint32_t b) {
+    using P = typename Kv4Pair<T>::type;
+    const P m = __hmax2_nan(*reinterpret_cast<P *>(&a), *reinterpret_cast<P *>(&b));
+    return *reinterpret_cast<const uint32_t *>(&m);
 }
 
-// One unit (four dims) of a row per thread; the G/4 threads of a group are neighbours in a warp and agree on its range by
-// shuffles.  Every thread of the warp calls this; `row` < 0 stores nothing.
-__device__ __forceinline__ void kv4_store_unit(float (&x)[4], long row, int u, int d, int g, int32_t *codes, __half *params) {
-    float lo, hi;
+// ---- one row by eight neighbouring threads ----------------------------------------------------------------------------
+// Thread r has the units (j, r) of all NB 32-dim blocks j: dims 32 j + 4 r .. + 3, x[2 j] and x[2 j + 1] in pairs.  Its codes
+// are 2 NB neighbouring bytes of the stored row.  The range of a group is the minimum of (x, -x) over its blocks and, by
+// three shuffles, over the eight threads, all of which call this; `row` < 0 stores nothing.
+// A quotient on the border of two codes is common in 16-bit data and has to go to the even code, which a product with the
+// reciprocal can miss.  So the product is rounded twice, with the reciprocal 2^-20 larger and smaller (its own error is
+// 2^-23): where both agree that is the code, where they do not, and for the groups that need a clamp somewhere, the thread
+// divides.  That is 5 instructions an element instead of 20, which made the append compute-bound: 8192 tokens of 8 heads
+// took 65 us.
+template <typename T, int NB>
+__device__ __forceinline__ void kv4_store_row(const uint32_t (&x)[2 * NB], long row, int r, int bpg, int32_t *codes, __half *params) {
+    constexpr float MAGIC = 12582912.f;      // 1.5 * 2^23: a sum with it is rounded to a whole number, which its low bits hold
+    uint32_t range[NB];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        x[i] = max_nan(min_nan(x[i], KV4_LIMIT), -KV4_LIMIT);
-        lo = i ? min_nan(lo, x[i]) : x[0];
-        hi = i ? max_nan(hi, x[i]) : x[0];
-    }
-    for (int o = 1; o < g / 4; o <<= 1) {
-        lo = min_nan(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-        hi = max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-    }
-    if (row < 0) return;
-    const __half base_h = __float2half_rn(lo);
-    const float base = __half2float(base_h);
-    const __half scale_h = __float2half_rn((hi - base) / 15.f);
-    const float scale = __half2float(scale_h);
-    uint32_t bits = 0;
-    if (scale > 0.f) {   // false for a NaN too: its codes are 0
+    for (int j = 0; j < NB; ++j) range[j] = pair_min<T>(x[2 * j], x[2 * j + 1]);      // for now both halves: minimum
+    uint32_t upper[NB];
+#pragma unroll
+    for (int j = 0; j < NB; ++j) upper[j] = pair_max<T>(x[2 * j], x[2 * j + 1]);
+    // blocks of a group
+#pragma unroll
+    for (int step = 1; step < 4; step <<= 1)
+        if (bpg > step)
+#pragma unroll
+            for (int j = 0; j + step < NB; j += 2 * step) {
+                range[j] = pair_min<T>(range[j], range[j + step]);
+                upper[j] = pair_max<T>(upper[j], upper[j + step]);
+            }
+    uint32_t bits[NB];
+    float base = 0.f, scale = 0.f, up = 0.f, down = 0.f;
+    __half2 stored = __halves2half2(__half(0.f), __half(0.f));
+    bool plain = true;
+#pragma unroll
+    for (int j = 0; j < NB; ++j) {
+        if ((j & (bpg - 1)) == 0) {          // a new group
+            // (minimum, -maximum) in one register
+            uint32_t lo = pair_min<T>(range[j], range[j] >> 16 | range[j] << 16);
+            uint32_t hi = pair_max<T>(upper[j], upper[j] >> 16 | upper[j] << 16) ^ 0x80008000u;
+            uint32_t both = __byte_perm(lo, hi, 0x5410);
+#pragma unroll
+            for (int o = 1; o < 8; o <<= 1) both = pair_min<T>(both, __shfl_xor_sync(0xffffffffu, both, o));
+            const float2 f = Kv4Pair<T>::wide(both);
+            // min.NaN / max.NaN: a NaN passes the clamp
+            float least, most;
+            asm("{ .reg .f32 a; max.NaN.f32 a, %1, %2; min.NaN.f32 %0, a, %3; }" : "=f"(least) : "f"(f.x), "f"(-KV4_LIMIT), "f"(KV4_LIMIT));
+            asm("{ .reg .f32 a; max.NaN.f32 a, %1, %2; min.NaN.f32 %0, a, %3; }" : "=f"(most) : "f"(-f.y), "f"(-KV4_LIMIT), "f"(KV4_LIMIT));
+            const __half base_h = __float2half_rn(least);
+            base = __half2float(base_h);
+            const __half scale_h = __float2half_rn((most - base) / 15.f);
+            scale = __half2float(scale_h);
+            stored = __halves2half2(scale_h, base_h);
+            // nothing to clamp: values inside the limits, and a scale that is rounded by 2^-11 at most
+            plain = least == f.x && most == -f.y && scale >= 1.f / 8192.f;
+            const float inv = __fdividef(1.f, scale);
+            up = inv * (1.f + 1.f / 1048576.f);
+            down = inv * (1.f - 1.f / 1048576.f);
+            const int g = j >> (bpg >> 1);   // bpg is 1, 2 or 4
+            if (row >= 0 && r == g) reinterpret_cast<__half2 *>(params)[row * (NB >> (bpg >> 1)) + g] = stored;
+        }
+        float f[4];
+        {
+            const float2 a = Kv4Pair<T>::wide(x[2 * j]), c = Kv4Pair<T>::wide(x[2 * j + 1]);
+            f[0] = a.x; f[1] = a.y; f[2] = c.x; f[3] = c.y;
+        }
+        uint32_t differ = 0, code = 0;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            // a division, not a product with the reciprocal: a quotient on the border of two codes is common in 16-bit
-            // data and has to be met exactly to go to the even one
-            const int c = __float2int_rn((x[i] - base) / scale);
-            bits |= (uint32_t)min(max(c, 0), 15) << (4 * i);
+            const float d = f[i] - base;
+            const uint32_t a = __float_as_uint(fmaf(d, up, MAGIC)), c = __float_as_uint(fmaf(d, down, MAGIC));
+            differ |= a ^ c;
+            code += a << (4 * i);            // the low bits of MAGIC are 0: what is above the nibble falls out of the low 16 bits
         }
+        if (differ || !plain) {
+            code = 0;
+            if (scale > 0.f)                 // false for a NaN too: its codes are 0
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float v = fminf(fmaxf(f[i], -KV4_LIMIT), KV4_LIMIT);
+                    code |= (uint32_t)min(max(__float2int_rn((v - base) / scale), 0), 15) << (4 * i);
+                }
+        }
+        bits[j] = code;
     }
-    const int place = (u & 7) * (d / 32) + (u >> 3);
-    reinterpret_cast<uint16_t *>(codes)[row * (d / 4) + place] = (uint16_t)bits;
-    if (u % (g / 4) == 0) reinterpret_cast<__half2 *>(params)[row * (d / g) + u / (g / 4)] = __halves2half2(scale_h, base_h);
+    if (row < 0) return;
+    unsigned char *to = reinterpret_cast<unsigned char *>(codes) + row * (16 * NB) + r * (2 * NB);
+    if constexpr (NB % 2) {
+#pragma unroll
+        for (int j = 0; j < NB; ++j) reinterpret_cast<uint16_t *>(to)[j] = (uint16_t)bits[j];
+    } else {
+        uint32_t w[NB / 2];
+#pragma unroll
+        for (int j = 0; j < NB / 2; ++j) w[j] = __byte_perm(bits[2 * j], bits[2 * j + 1], 0x5410);
+        if constexpr (NB == 8) *reinterpret_cast<uint4 *>(to) = make_uint4(w[0], w[1], w[2], w[3]);
+        else if constexpr (NB == 4) *reinterpret_cast<uint2 *>(to) = make_uint2(w[0], w[1]);
+        else
+#pragma unroll
+            for (int j = 0; j < NB / 2; ++j) reinterpret_cast<uint32_t *>(to)[j] = w[j];
+    }
 }
 
-// New rows [batch, tokens, heads, D] (token pitch stride_t elements) -> cache rows first[b] + t.  Threads are numbered
-// (b, t, h, unit), units fastest, and walk the grid in strides of whole warps, so a group never straddles a warp.
-template <typename T>
-__global__ void __launch_bounds__(256)
+template <typename T, int NB>
+__device__ __forceinline__ void kv4_load_row(uint32_t (&x)[2 * NB], const T *row, int r) {
+#pragma unroll
+    for (int j = 0; j < NB; ++j) {
+        const uint2 u = *reinterpret_cast<const uint2 *>(row + 32 * j + 4 * r);
+        x[2 * j] = u.x;
+        x[2 * j + 1] = u.y;
+    }
+}
+
+// New rows [batch, tokens, heads, D] (token pitch stride_t elements) -> cache rows first[b] + t.  Eight threads a row of K or V,
+// rows of a sequence (blockIdx.y) numbered (t, h, K | V).
+template <typename T, int NB>
+__global__ void __launch_bounds__(128)
 kv4_append_kernel(const T *__restrict__ nk, const T *__restrict__ nv, Kv4Cache C, const int32_t *__restrict__ first,
-                  const int32_t *__restrict__ new_lens, int tokens, long stride_kt, long stride_vt, long total, int *status) {
+                  const int32_t *__restrict__ new_lens, int tokens, long stride_kt, long stride_vt, int *status) {
     pdl_wait();
     pdl_launch_dependents();
-    const int units = C.d / 4;
-    for (long i0 = ((long)blockIdx.x * blockDim.x + threadIdx.x) & ~31l; i0 < total; i0 += (long)gridDim.x * blockDim.x) {
-        const long i = i0 + (threadIdx.x & 31);
-        const bool live = i < total;
-        const long rh = (live ? i : total - 1) / units;
-        const int u = (int)((live ? i : total - 1) - rh * units);
-        const long bt = rh / C.heads;
-        const int h = (int)(rh - bt * C.heads), b = (int)(bt / tokens), t = (int)(bt - (long)b * tokens);
-        int n = tokens;
-        if (new_lens) {
-            n = new_lens[b];
-            if (n > tokens) {
-                n = tokens;
-                if (t == 0 && h == 0 && u == 0) atomicOr(status, KV4_BAD_POSITION);
-            }
+    const int b = blockIdx.y, r = threadIdx.x & 7, bpg = C.g / 32;
+    const long start = first[b];
+    int n = tokens;
+    if (new_lens) {
+        n = new_lens[b];
+        if (n > tokens) {
+            n = tokens;
+            if (blockIdx.x == 0 && threadIdx.x == 0) atomicOr(status, KV4_BAD_POSITION);
         }
+    }
+    const unsigned rows = 2u * C.heads * (unsigned)max(n, 0);
+    for (unsigned i0 = (blockIdx.x * blockDim.x + threadIdx.x & ~31u) >> 3; i0 < rows; i0 += gridDim.x * blockDim.x >> 3) {
+        const unsigned i = i0 + ((threadIdx.x & 31) >> 3);
+        const bool live = i < rows;
+        const unsigned th = (live ? i : 0u) >> 1, t = th / (unsigned)C.heads, h = th - t * C.heads;
+        const bool is_v = i & 1;
         long row = -1;
-        if (live && t < n) {
-            const long pos = (long)first[b] + t;
+        if (live) {
+            const long pos = start + t;
             if ((unsigned long)pos < (unsigned long)C.capacity) {
                 row = kv4_row(C, b, h, (int)pos);
-                if (row < 0 && u == 0) atomicOr(status, KV4_BAD_BLOCK);
-            } else if (u == 0) {
+                if (row < 0 && r == 0) atomicOr(status, KV4_BAD_BLOCK);
+            } else if (r == 0) {
                 atomicOr(status, KV4_BAD_POSITION);
             }
         }
-        float x[4], y[4];
-        Kv4Elem<T>::load(nk + bt * stride_kt + (long)h * C.d + 4 * u, x);
-        Kv4Elem<T>::load(nv + bt * stride_vt + (long)h * C.d + 4 * u, y);
-        kv4_store_unit(x, row, u, C.d, C.g, C.k_codes, C.k_params);
-        kv4_store_unit(y, row, u, C.d, C.g, C.v_codes, C.v_params);
+        uint32_t x[2 * NB];
+        kv4_load_row<T, NB>(x, (is_v ? nv : nk) + ((long)b * tokens + t) * (is_v ? stride_vt : stride_kt) + (long)h * (32 * NB), r);
+        kv4_store_row<T, NB>(x, row, r, bpg, is_v ? C.v_codes : C.k_codes, is_v ? C.v_params : C.k_params);
     }
 }
 
 // A fused QKV row a sequence [q heads | k heads | v heads] -> q_out rotated, k rotated and quantised, v quantised.
 // Rotation of the pairs (i, i + D/2) as in rope_full; the products and their sum are each rounded on their own, so that
 // the key that is quantised does not depend on which of them a compiler contracts, and the key is rounded to its type
-// first, as in the unfused sequence.
-template <typename T>
-__global__ void __launch_bounds__(256)
+// first, as in the unfused sequence.  Eight threads a head; the other half of a pair is the same thread's where the
+// number of blocks is even, and loaded again (from L1) where it is odd.
+template <typename T, int NB>
+__global__ void __launch_bounds__(128)
 kv4_rope_append_kernel(const T *__restrict__ qkv, const float *__restrict__ cos_t, const float *__restrict__ sin_t,
                        const int32_t *__restrict__ positions, T *__restrict__ q_out, Kv4Cache C, int32_t *__restrict__ lens_out, int hq,
-                       int *status) {
+                       int vec, int *status) {
+    constexpr int D = 32 * NB, HALF = D / 2;
     pdl_wait();
     pdl_launch_dependents();
-    const int b = blockIdx.y, units = C.d / 4, heads = hq + 2 * C.heads, total = heads * units;
+    const int b = blockIdx.y, heads = hq + 2 * C.heads, r = threadIdx.x & 7;
     int pos = positions[b];
     // A position outside the cache: as in rope_kv_append_hm, nothing is stored, q is rotated with the nearest valid table
     // row, the length handed on stays within the cache and the status word says so.
@@ -115,83 +202,149 @@ kv4_rope_append_kernel(const T *__restrict__ qkv, const float *__restrict__ cos_
         if (threadIdx.x == 0 && blockIdx.x == 0) atomicOr(status, KV4_BAD_POSITION);
     }
     if (lens_out && threadIdx.x == 0 && blockIdx.x == 0) lens_out[b] = pos + 1;
-    const int half = C.d / 2;
-    const T *row = qkv + (size_t)b * heads * C.d;
-    for (int i0 = (blockIdx.x * blockDim.x + threadIdx.x) & ~31; i0 < total; i0 += gridDim.x * blockDim.x) {
-        const bool live = i0 + (int)(threadIdx.x & 31) < total;
-        const int i = live ? i0 + (threadIdx.x & 31) : total - 1;
-        const int h = i / units, u = i - h * units;
-        float x[4];
-        Kv4Elem<T>::load(row + (size_t)h * C.d + 4 * u, x);
-        if (h < hq + C.heads) {
-            const bool upper = 4 * u >= half;
-            const int p = 4 * u - (upper ? half : 0);
-            float y[4];
-            Kv4Elem<T>::load(row + (size_t)h * C.d + (upper ? p : p + half), y);
+    const int h0 = (blockIdx.x * blockDim.x + threadIdx.x) >> 3;
+    const bool live = h0 < heads;
+    const int h = live ? h0 : 0;
+    const T *row = qkv + ((size_t)b * heads + h) * D;
+    uint32_t x[2 * NB];
+    kv4_load_row<T, NB>(x, row, r);
+    if (h < hq + C.heads) {
+        const float *cr = cos_t + (size_t)pos * HALF, *sr = sin_t + (size_t)pos * HALF;
+        uint32_t other[2 * NB];
+        if constexpr (NB % 2) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const float c = cos_t[(size_t)pos * half + p + e], s = sin_t[(size_t)pos * half + p + e];
-                const float a = __fmul_rn(x[e], c), z = __fmul_rn(y[e], s);
-                x[e] = Kv4Elem<T>::round(upper ? __fadd_rn(a, z) : __fsub_rn(a, z));
+            for (int j = 0; j < NB; ++j) {
+                const int d = 32 * j + 4 * r;
+                const uint2 u = *reinterpret_cast<const uint2 *>(row + (d < HALF ? d + HALF : d - HALF));
+                other[2 * j] = u.x;
+                other[2 * j + 1] = u.y;
             }
-            if (h < hq && live)
-                *reinterpret_cast<uint2 *>(q_out + ((size_t)b * hq + h) * C.d + 4 * u) =
-                    make_uint2(Kv4Elem<T>::pack(x[0], x[1]), Kv4Elem<T>::pack(x[2], x[3]));
+        } else {
+#pragma unroll
+            for (int j = 0; j < 2 * NB; ++j) other[j] = x[(j + NB) % (2 * NB)];
         }
-        const int kvh = h < hq + C.heads ? h - hq : h - hq - C.heads;
-        const long r = live && in_range && h >= hq ? kv4_row(C, b, kvh, pos) : -1;
-        const bool is_v = h >= hq + C.heads;
-        kv4_store_unit(x, r, u, C.d, C.g, is_v ? C.v_codes : C.k_codes, is_v ? C.v_params : C.k_params);
+        uint32_t out[2 * NB];
+#pragma unroll
+        for (int j = 0; j < NB; ++j) {
+            const int d = 32 * j + 4 * r;
+            const bool upper = d >= HALF;
+            const int p = d - (upper ? HALF : 0);
+            float c[4], s[4];
+            if (vec) {
+                const float4 c4 = *reinterpret_cast<const float4 *>(cr + p), s4 = *reinterpret_cast<const float4 *>(sr + p);
+                c[0] = c4.x; c[1] = c4.y; c[2] = c4.z; c[3] = c4.w;
+                s[0] = s4.x; s[1] = s4.y; s[2] = s4.z; s[3] = s4.w;
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) { c[e] = cr[p + e]; s[e] = sr[p + e]; }
+            }
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const float2 f = Kv4Pair<T>::wide(x[2 * j + e]), o = Kv4Pair<T>::wide(other[2 * j + e]);
+                const float a0 = __fmul_rn(f.x, c[2 * e]), z0 = __fmul_rn(o.x, s[2 * e]);
+                const float a1 = __fmul_rn(f.y, c[2 * e + 1]), z1 = __fmul_rn(o.y, s[2 * e + 1]);
+                out[2 * j + e] = Kv4Elem<T>::pack(upper ? __fadd_rn(a0, z0) : __fsub_rn(a0, z0), upper ? __fadd_rn(a1, z1) : __fsub_rn(a1, z1));
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < 2 * NB; ++j) x[j] = out[j];
+        if (h < hq && live)
+#pragma unroll
+            for (int j = 0; j < NB; ++j)
+                *reinterpret_cast<uint2 *>(q_out + ((size_t)b * hq + h) * D + 32 * j + 4 * r) = make_uint2(x[2 * j], x[2 * j + 1]);
     }
+    if (__all_sync(0xffffffffu, h < hq)) return;
+    const bool is_v = h >= hq + C.heads;
+    const long to = live && in_range && h >= hq ? kv4_row(C, b, is_v ? h - hq - C.heads : h - hq, pos) : -1;
+    kv4_store_row<T, NB>(x, to, r, C.g / 32, is_v ? C.v_codes : C.k_codes, is_v ? C.v_params : C.k_params);
 }
 
 // Rows first[b] + i of the cache, i < out_len and below context_lens[b] -> out [batch, heads, out_len, D]; rows behind
-// them are left as they were.
-template <typename T>
+// them are left as they were.  Four threads a row of K or V: a thread's quarter of the codes (NB words) holds eight
+// neighbouring dims of every block, 16 bytes of the output.
+template <typename T, int NB>
 __global__ void __launch_bounds__(256)
 kv4_read_kernel(Kv4Cache C, const int32_t *__restrict__ first, const int32_t *__restrict__ lens, T *__restrict__ k_out, T *__restrict__ v_out,
-                int out_len, long total, int *status) {
+                int out_len, int *status) {
+    constexpr int D = 32 * NB;
     pdl_wait();
     pdl_launch_dependents();
-    const int units = C.d / 4;
-    for (long i = (long)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (long)gridDim.x * blockDim.x) {
-        const long r = i / units;                 // row of the output
-        const int place = (int)(i - r * units);
-        const long bh = r / out_len;
-        const int b = (int)(bh / C.heads), h = (int)(bh - (long)b * C.heads);
-        const long pos = (first ? (long)first[b] : 0) + (r - bh * out_len);
-        int len = lens[b];
-        if (len > C.capacity) {
-            len = C.capacity;
-            if (place == 0) atomicOr(status, KV4_BAD_POSITION);
-        }
-        if (pos >= len) continue;
+    const int b = blockIdx.z, h = blockIdx.y, t = threadIdx.x & 3, bpg = C.g / 32;
+    int len = lens[b];
+    if (len > C.capacity) {
+        len = C.capacity;
+        if (blockIdx.x == 0 && h == 0 && threadIdx.x == 0) atomicOr(status, KV4_BAD_POSITION);
+    }
+    const long start = first ? (long)first[b] : 0l;
+    const unsigned rows = (unsigned)max(min((long)out_len, len - start), 0l);
+    for (unsigned i2 = blockIdx.x * blockDim.x + threadIdx.x >> 2; i2 < 2 * rows; i2 += gridDim.x * blockDim.x >> 2) {
+        const unsigned i = i2 >> 1;
+        const bool is_v = i2 & 1;
+        const long pos = start + i;
         if (pos < 0) {
-            if (place == 0) atomicOr(status, KV4_BAD_POSITION);
+            if (t == 0) atomicOr(status, KV4_BAD_POSITION);
             continue;
         }
         const long row = kv4_row(C, b, h, (int)pos);
         if (row < 0) {
-            if (place == 0) atomicOr(status, KV4_BAD_BLOCK);
+            if (t == 0) atomicOr(status, KV4_BAD_BLOCK);
             continue;
         }
-        const int nb = C.d / 32, u = (place % nb) * 8 + place / nb;
+        uint32_t w[NB];
+        const uint32_t *from = reinterpret_cast<const uint32_t *>(is_v ? C.v_codes : C.k_codes) + row * (4 * NB) + t * NB;
+        if constexpr (NB % 4 == 0) {
 #pragma unroll
-        for (int kv = 0; kv < 2; ++kv) {
-            const uint32_t bits = reinterpret_cast<const uint16_t *>(kv ? C.v_codes : C.k_codes)[row * units + place];
-            const float2 p = __half22float2(reinterpret_cast<const __half2 *>(kv ? C.v_params : C.k_params)[row * (C.d / C.g) + 4 * u / C.g]);
-            float f[4];
+            for (int j = 0; j < NB; j += 4) {
+                const uint4 u = ldg_nc_v4(from + j);
+                w[j] = u.x; w[j + 1] = u.y; w[j + 2] = u.z; w[j + 3] = u.w;
+            }
+        } else {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) f[e] = fmaf((float)((bits >> (4 * e)) & 15u), p.x, p.y);
-            *reinterpret_cast<uint2 *>((kv ? v_out : k_out) + r * C.d + 4 * u) =
-                make_uint2(Kv4Elem<T>::pack(f[0], f[1]), Kv4Elem<T>::pack(f[2], f[3]));
+            for (int j = 0; j < NB; ++j) w[j] = from[j];
+        }
+        const __half2 *params = reinterpret_cast<const __half2 *>(is_v ? C.v_params : C.k_params) + row * (NB >> (bpg >> 1));
+        T *to = (is_v ? v_out : k_out) + (((long)b * C.heads + h) * out_len + i) * D + 8 * t;
+        float2 p = make_float2(0.f, 0.f);
+#pragma unroll
+        for (int j = 0; j < NB; ++j) {
+            if ((j & (bpg - 1)) == 0) {
+                p = __half22float2(params[j >> (bpg >> 1)]);
+                p.x *= 16777216.f;           // the codes come as fp16 subnormals, c 2^-24: exact either way
+            }
+            // units (2 t, j) and (2 t + 1, j): dims 8 t .. + 3 in the low half, + 4 .. + 7 in the high one
+            const uint32_t u = __byte_perm(w[j >> 1], w[(NB + j) >> 1], (j & 1 ? 0x32 : 0x10) | ((NB + j & 1 ? 0x76 : 0x54) << 8));
+            float f[8];
+#pragma unroll
+            for (int n = 0; n < 4; ++n) {
+                const float2 c = h2_to_f2((u >> (4 * n)) & 0x000f000fu);
+                f[n] = fmaf(c.x, p.x, p.y);
+                f[n + 4] = fmaf(c.y, p.x, p.y);
+            }
+            *reinterpret_cast<uint4 *>(to + 32 * j) = make_uint4(Kv4Elem<T>::pack(f[0], f[1]), Kv4Elem<T>::pack(f[2], f[3]), Kv4Elem<T>::pack(f[4], f[5]),
+                                                                 Kv4Elem<T>::pack(f[6], f[7]));
         }
     }
 }
 
-static int kv4_grid(long threads) {
-    const long blocks = (threads + 255) / 256, cap = (long)sm_count() * 32;
-    return (int)(blocks < cap ? blocks : cap);
+// calls f with the number of 32-dim blocks as a constant
+template <typename F>
+static int kv4_by_blocks(int d, F f) {
+    switch (d / 32) {
+        case 1: return f(std::integral_constant<int, 1>());
+        case 2: return f(std::integral_constant<int, 2>());
+        case 3: return f(std::integral_constant<int, 3>());
+        case 4: return f(std::integral_constant<int, 4>());
+        case 5: return f(std::integral_constant<int, 5>());
+        case 6: return f(std::integral_constant<int, 6>());
+        case 7: return f(std::integral_constant<int, 7>());
+        default: return f(std::integral_constant<int, 8>());
+    }
+}
+
+// blocks along x for `rows` rows a sequence: one pass over them while the grid fits the machine a few times over
+static unsigned kv4_grid(long rows, int rows_per_block, long others) {
+    const long blocks = (rows + rows_per_block - 1) / rows_per_block, cap = ((long)sm_count() * 64 + others - 1) / others;
+    return (unsigned)(blocks < cap ? blocks : cap);
 }
 
 template <typename T>
@@ -200,16 +353,20 @@ static int kv4_append_launch(const char *name, const T *nk, const T *nv, const K
     B200K_REQUIRE(nk && nv && first, B200K_E_NULL, "%s: NULL pointer", name);
     int rc = kv4_check(name, C, batch, paged);
     if (rc) return rc;
-    B200K_REQUIRE(tokens >= 0 && stride_kt >= C.heads * C.d && stride_vt >= C.heads * C.d, B200K_E_SHAPE,
-                  "%s: tokens %d, strides %d and %d (at least heads * head_dim = %d)", name, tokens, stride_kt, stride_vt, C.heads * C.d);
+    B200K_REQUIRE(tokens >= 0 && (long)tokens * C.heads < (1l << 30) && stride_kt >= C.heads * C.d && stride_vt >= C.heads * C.d, B200K_E_SHAPE,
+                  "%s: tokens %d (tokens * heads below 2^30), strides %d and %d (at least heads * head_dim = %d)", name, tokens, stride_kt, stride_vt,
+                  C.heads * C.d);
     B200K_REQUIRE(aligned16(nk) && aligned16(nv) && stride_kt % 8 == 0 && stride_vt % 8 == 0, B200K_E_ALIGN,
                   "%s: new_keys and new_values must be 16-byte aligned, their token strides multiples of 8", name);
-    const long total = (long)batch * tokens * C.heads * (C.d / 4);
-    if (total == 0) return 0;
+    if (batch == 0 || tokens == 0) return 0;
     int *status = status_word();
     if (!status) return B200K_E_WORKSPACE;
-    launch_kernel(kv4_append_kernel<T>, dim3(kv4_grid(total)), dim3(256), 0, to_stream(stream), nk, nv, C, first, new_lens, tokens, (long)stride_kt,
-                  (long)stride_vt, total, status);
+    const dim3 grid(kv4_grid(2l * tokens * C.heads, 16, batch), batch);
+    kv4_by_blocks(C.d, [&](auto nb) {
+        launch_kernel(kv4_append_kernel<T, nb()>, grid, dim3(128), 0, to_stream(stream), nk, nv, C, first, new_lens, tokens, (long)stride_kt,
+                      (long)stride_vt, status);
+        return 0;
+    });
     return launch_status(name);
 }
 
@@ -224,9 +381,13 @@ static int kv4_rope_append_launch(const char *name, const T *qkv, const float *c
     if (batch == 0) return 0;
     int *status = status_word();
     if (!status) return B200K_E_WORKSPACE;
-    const int total = (hq + 2 * C.heads) * (C.d / 4);
-    launch_kernel(kv4_rope_append_kernel<T>, dim3(ceil_div(total, 256), batch), dim3(256), 0, to_stream(stream), qkv, cos_t, sin_t, positions, q_out, C,
-                  lens_out, hq, status);
+    const int vec = aligned16(cos_t) && aligned16(sin_t);
+    const dim3 grid(ceil_div(hq + 2 * C.heads, 16), batch);
+    kv4_by_blocks(C.d, [&](auto nb) {
+        launch_kernel(kv4_rope_append_kernel<T, nb()>, grid, dim3(128), 0, to_stream(stream), qkv, cos_t, sin_t, positions, q_out, C, lens_out, hq, vec,
+                      status);
+        return 0;
+    });
     return launch_status(name);
 }
 
@@ -236,13 +397,17 @@ static int kv4_read_launch(const char *name, const Kv4Cache &C, bool paged, cons
     B200K_REQUIRE(lens && k_out && v_out, B200K_E_NULL, "%s: NULL pointer", name);
     int rc = kv4_check(name, C, batch, paged);
     if (rc) return rc;
-    B200K_REQUIRE(out_len >= 0, B200K_E_SHAPE, "%s: out_len %d", name, out_len);
+    B200K_REQUIRE(C.heads <= 65535, B200K_E_SHAPE, "%s: heads %d", name, C.heads);
+    B200K_REQUIRE(out_len >= 0 && out_len <= KV4_MAX_LEN, B200K_E_SHAPE, "%s: out_len %d", name, out_len);
     B200K_REQUIRE(aligned16(k_out) && aligned16(v_out), B200K_E_ALIGN, "%s: k_out and v_out must be 16-byte aligned", name);
-    const long total = (long)batch * C.heads * out_len * (C.d / 4);
-    if (total == 0) return 0;
+    if (batch == 0 || out_len == 0) return 0;
     int *status = status_word();
     if (!status) return B200K_E_WORKSPACE;
-    launch_kernel(kv4_read_kernel<T>, dim3(kv4_grid(total)), dim3(256), 0, to_stream(stream), C, first, lens, k_out, v_out, out_len, total, status);
+    const dim3 grid(kv4_grid(2l * out_len, 64, (long)batch * C.heads), C.heads, batch);
+    kv4_by_blocks(C.d, [&](auto nb) {
+        launch_kernel(kv4_read_kernel<T, nb()>, grid, dim3(256), 0, to_stream(stream), C, first, lens, k_out, v_out, out_len, status);
+        return 0;
+    });
     return launch_status(name);
 }
 
