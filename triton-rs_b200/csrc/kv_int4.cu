@@ -30,17 +30,38 @@ template <typename T> __device__ __forceinline__ uint32_t pair_max(uint32_t a, u
     return *reinterpret_cast<const uint32_t *>(&m);
 }
 
+// a / b for normal a, b and y = 1 / b to 2^-23 (Markstein's division with a fused multiply-add): the remainder of the first
+// quotient is exact, so a quotient that fp32 can hold comes out exact, and any other rounded to nearest but for a
+// hair's breadth around the middle of two numbers.
+__device__ __forceinline__ float kv4_quotient(float a, float b, float y) {
+    const float q = a * y;
+    return fmaf(fmaf(-q, b, a), y, q);
+}
+
 // ---- one row by eight neighbouring threads ----------------------------------------------------------------------------
 // Thread r has the units (j, r) of all NB 32-dim blocks j: dims 32 j + 4 r .. + 3, x[2 j] and x[2 j + 1] in pairs.  Its codes
 // are 2 NB neighbouring bytes of the stored row.  The range of a group is the minimum of (x, -x) over its blocks and, by
 // three shuffles, over the eight threads, all of which call this; `row` < 0 stores nothing.
 // A quotient on the border of two codes is common in 16-bit data and has to go to the even code, which a product with the
-// reciprocal can miss.  So the product is rounded twice, with the reciprocal 2^-20 larger and smaller (its own error is
-// 2^-23): where both agree that is the code, where they do not, and for the groups that need a clamp somewhere, the thread
-// divides.  That is 5 instructions an element instead of 20, which made the append compute-bound: 8192 tokens of 8 heads
-// took 65 us.
-template <typename T, int NB>
-__device__ __forceinline__ void kv4_store_row(const uint32_t (&x)[2 * NB], long row, int r, int bpg, int32_t *codes, __half *params) {
+// reciprocal can miss; see kv4_quotient.  A sum with 1.5 * 2^23 then rounds it.  6 instructions an element where the compiler's
+// division, good for all operands, takes some 20: with it the append was bound by the issue of instructions (8192 tokens of
+// 8 heads: 65 us, 6.5 us being the floor).  Groups that need a clamp somewhere take the division.
+template <typename T>
+__device__ __noinline__ uint32_t kv4_codes_clamped(uint32_t x0, uint32_t x1, float base, float scale) {
+    const float2 a = Kv4Pair<T>::wide(x0), c = Kv4Pair<T>::wide(x1);
+    const float f[4] = {a.x, a.y, c.x, c.y};
+    uint32_t code = 0;
+    if (scale > 0.f)                         // false for a NaN too: its codes are 0
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float v = fminf(fmaxf(f[i], -KV4_LIMIT), KV4_LIMIT);
+            code |= (uint32_t)min(max(__float2int_rn((v - base) / scale), 0), 15) << (4 * i);
+        }
+    return code;
+}
+
+template <typename T, int NB, int BPG>
+__device__ __forceinline__ void kv4_store_row(const uint32_t (&x)[2 * NB], long row, int r, int32_t *codes, __half *params) {
     constexpr float MAGIC = 12582912.f;      // 1.5 * 2^23: a sum with it is rounded to a whole number, which its low bits hold
     uint32_t range[NB];
 #pragma unroll
@@ -51,19 +72,18 @@ __device__ __forceinline__ void kv4_store_row(const uint32_t (&x)[2 * NB], long 
     // blocks of a group
 #pragma unroll
     for (int step = 1; step < 4; step <<= 1)
-        if (bpg > step)
+        if (BPG > step)
 #pragma unroll
             for (int j = 0; j + step < NB; j += 2 * step) {
                 range[j] = pair_min<T>(range[j], range[j + step]);
                 upper[j] = pair_max<T>(upper[j], upper[j + step]);
             }
     uint32_t bits[NB];
-    float base = 0.f, scale = 0.f, up = 0.f, down = 0.f;
-    __half2 stored = __halves2half2(__half(0.f), __half(0.f));
-    bool plain = true;
+    float base = 0.f, scale = 0.f, inv = 0.f;
+    bool plain = true;                       // BPG blocks are a group
 #pragma unroll
     for (int j = 0; j < NB; ++j) {
-        if ((j & (bpg - 1)) == 0) {          // a new group
+        if (j % BPG == 0) {                  // a new group
             // (minimum, -maximum) in one register
             uint32_t lo = pair_min<T>(range[j], range[j] >> 16 | range[j] << 16);
             uint32_t hi = pair_max<T>(upper[j], upper[j] >> 16 | upper[j] << 16) ^ 0x80008000u;
@@ -77,39 +97,25 @@ __device__ __forceinline__ void kv4_store_row(const uint32_t (&x)[2 * NB], long 
             asm("{ .reg .f32 a; max.NaN.f32 a, %1, %2; min.NaN.f32 %0, a, %3; }" : "=f"(most) : "f"(-f.y), "f"(-KV4_LIMIT), "f"(KV4_LIMIT));
             const __half base_h = __float2half_rn(least);
             base = __half2float(base_h);
-            const __half scale_h = __float2half_rn((most - base) / 15.f);
+            const __half scale_h = __float2half_rn(kv4_quotient(most - base, 15.f, 1.f / 15.f));
             scale = __half2float(scale_h);
-            stored = __halves2half2(scale_h, base_h);
             // nothing to clamp: values inside the limits, and a scale that is rounded by 2^-11 at most
             plain = least == f.x && most == -f.y && scale >= 1.f / 8192.f;
-            const float inv = __fdividef(1.f, scale);
-            up = inv * (1.f + 1.f / 1048576.f);
-            down = inv * (1.f - 1.f / 1048576.f);
-            const int g = j >> (bpg >> 1);   // bpg is 1, 2 or 4
-            if (row >= 0 && r == g) reinterpret_cast<__half2 *>(params)[row * (NB >> (bpg >> 1)) + g] = stored;
+            asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(scale));
+            if (row >= 0 && r == j / BPG) reinterpret_cast<__half2 *>(params)[row * (NB / BPG) + j / BPG] = __halves2half2(scale_h, base_h);
         }
         float f[4];
         {
             const float2 a = Kv4Pair<T>::wide(x[2 * j]), c = Kv4Pair<T>::wide(x[2 * j + 1]);
             f[0] = a.x; f[1] = a.y; f[2] = c.x; f[3] = c.y;
         }
-        uint32_t differ = 0, code = 0;
+        uint32_t code = 0;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const float d = f[i] - base;
-            const uint32_t a = __float_as_uint(fmaf(d, up, MAGIC)), c = __float_as_uint(fmaf(d, down, MAGIC));
-            differ |= a ^ c;
-            code += a << (4 * i);            // the low bits of MAGIC are 0: what is above the nibble falls out of the low 16 bits
+            const float c = kv4_quotient(f[i] - base, scale, inv) + MAGIC;
+            code += __float_as_uint(c) * (1u << (4 * i));      // the low bits of MAGIC are 0: only the nibble reaches the low 16 bits
         }
-        if (differ || !plain) {
-            code = 0;
-            if (scale > 0.f)                 // false for a NaN too: its codes are 0
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float v = fminf(fmaxf(f[i], -KV4_LIMIT), KV4_LIMIT);
-                    code |= (uint32_t)min(max(__float2int_rn((v - base) / scale), 0), 15) << (4 * i);
-                }
-        }
+        if (!plain) code = kv4_codes_clamped<T>(x[2 * j], x[2 * j + 1], base, scale);
         bits[j] = code;
     }
     if (row < 0) return;
@@ -139,15 +145,15 @@ __device__ __forceinline__ void kv4_load_row(uint32_t (&x)[2 * NB], const T *row
     }
 }
 
-// New rows [batch, tokens, heads, D] (token pitch stride_t elements) -> cache rows first[b] + t.  Eight threads a row of K or V,
-// rows of a sequence (blockIdx.y) numbered (t, h, K | V).
-template <typename T, int NB>
+// New rows [batch, tokens, heads, D] (token pitch stride_t elements) -> cache rows first[b] + t.  Eight threads a row of K and the
+// same row of V, rows of a sequence (blockIdx.y) numbered (t, h).
+template <typename T, int NB, int BPG>
 __global__ void __launch_bounds__(128)
 kv4_append_kernel(const T *__restrict__ nk, const T *__restrict__ nv, Kv4Cache C, const int32_t *__restrict__ first,
                   const int32_t *__restrict__ new_lens, int tokens, long stride_kt, long stride_vt, int *status) {
     pdl_wait();
     pdl_launch_dependents();
-    const int b = blockIdx.y, r = threadIdx.x & 7, bpg = C.g / 32;
+    const int b = blockIdx.y, r = threadIdx.x & 7;
     const long start = first[b];
     int n = tokens;
     if (new_lens) {
@@ -157,12 +163,15 @@ kv4_append_kernel(const T *__restrict__ nk, const T *__restrict__ nv, Kv4Cache C
             if (blockIdx.x == 0 && threadIdx.x == 0) atomicOr(status, KV4_BAD_POSITION);
         }
     }
-    const unsigned rows = 2u * C.heads * (unsigned)max(n, 0);
+    const unsigned rows = C.heads * (unsigned)max(n, 0);
     for (unsigned i0 = (blockIdx.x * blockDim.x + threadIdx.x & ~31u) >> 3; i0 < rows; i0 += gridDim.x * blockDim.x >> 3) {
         const unsigned i = i0 + ((threadIdx.x & 31) >> 3);
         const bool live = i < rows;
-        const unsigned th = (live ? i : 0u) >> 1, t = th / (unsigned)C.heads, h = th - t * C.heads;
-        const bool is_v = i & 1;
+        const unsigned th = live ? i : 0u, t = th / (unsigned)C.heads, h = th - t * C.heads;
+        uint32_t x[2 * NB], y[2 * NB];
+        const long at = (long)b * tokens + t, in_row = (long)h * (32 * NB);
+        kv4_load_row<T, NB>(x, nk + at * stride_kt + in_row, r);
+        kv4_load_row<T, NB>(y, nv + at * stride_vt + in_row, r);
         long row = -1;
         if (live) {
             const long pos = start + t;
@@ -173,9 +182,8 @@ kv4_append_kernel(const T *__restrict__ nk, const T *__restrict__ nv, Kv4Cache C
                 atomicOr(status, KV4_BAD_POSITION);
             }
         }
-        uint32_t x[2 * NB];
-        kv4_load_row<T, NB>(x, (is_v ? nv : nk) + ((long)b * tokens + t) * (is_v ? stride_vt : stride_kt) + (long)h * (32 * NB), r);
-        kv4_store_row<T, NB>(x, row, r, bpg, is_v ? C.v_codes : C.k_codes, is_v ? C.v_params : C.k_params);
+        kv4_store_row<T, NB, BPG>(x, row, r, C.k_codes, C.k_params);
+        kv4_store_row<T, NB, BPG>(y, row, r, C.v_codes, C.v_params);
     }
 }
 
@@ -184,7 +192,7 @@ kv4_append_kernel(const T *__restrict__ nk, const T *__restrict__ nv, Kv4Cache C
 // the key that is quantised does not depend on which of them a compiler contracts, and the key is rounded to its type
 // first, as in the unfused sequence.  Eight threads a head; the other half of a pair is the same thread's where the
 // number of blocks is even, and loaded again (from L1) where it is odd.
-template <typename T, int NB>
+template <typename T, int NB, int BPG>
 __global__ void __launch_bounds__(128)
 kv4_rope_append_kernel(const T *__restrict__ qkv, const float *__restrict__ cos_t, const float *__restrict__ sin_t,
                        const int32_t *__restrict__ positions, T *__restrict__ q_out, Kv4Cache C, int32_t *__restrict__ lens_out, int hq,
@@ -256,30 +264,33 @@ kv4_rope_append_kernel(const T *__restrict__ qkv, const float *__restrict__ cos_
     if (__all_sync(0xffffffffu, h < hq)) return;
     const bool is_v = h >= hq + C.heads;
     const long to = live && in_range && h >= hq ? kv4_row(C, b, is_v ? h - hq - C.heads : h - hq, pos) : -1;
-    kv4_store_row<T, NB>(x, to, r, C.g / 32, is_v ? C.v_codes : C.k_codes, is_v ? C.v_params : C.k_params);
+    kv4_store_row<T, NB, BPG>(x, to, r, is_v ? C.v_codes : C.k_codes, is_v ? C.v_params : C.k_params);
 }
 
 // Rows first[b] + i of the cache, i < out_len and below context_lens[b] -> out [batch, heads, out_len, D]; rows behind
 // them are left as they were.  Four threads a row of K or V: a thread's quarter of the codes (NB words) holds eight
 // neighbouring dims of every block, 16 bytes of the output.
-template <typename T, int NB>
+template <typename T, int NB, int BPG>
 __global__ void __launch_bounds__(256)
 kv4_read_kernel(Kv4Cache C, const int32_t *__restrict__ first, const int32_t *__restrict__ lens, T *__restrict__ k_out, T *__restrict__ v_out,
                 int out_len, int *status) {
     constexpr int D = 32 * NB;
     pdl_wait();
     pdl_launch_dependents();
-    const int b = blockIdx.z, h = blockIdx.y, t = threadIdx.x & 3, bpg = C.g / 32;
+    const int b = blockIdx.y, t = threadIdx.x & 3;
     int len = lens[b];
     if (len > C.capacity) {
         len = C.capacity;
-        if (blockIdx.x == 0 && h == 0 && threadIdx.x == 0) atomicOr(status, KV4_BAD_POSITION);
+        if (blockIdx.x == 0 && threadIdx.x == 0) atomicOr(status, KV4_BAD_POSITION);
     }
     const long start = first ? (long)first[b] : 0l;
-    const unsigned rows = (unsigned)max(min((long)out_len, len - start), 0l);
-    for (unsigned i2 = blockIdx.x * blockDim.x + threadIdx.x >> 2; i2 < 2 * rows; i2 += gridDim.x * blockDim.x >> 2) {
-        const unsigned i = i2 >> 1;
+    const unsigned rows = (unsigned)max(min((long)out_len, len - start), 0l);     // of a head, times K and V, times heads:
+    const long total = 2l * rows * C.heads;
+    for (long i2 = ((long)blockIdx.x * blockDim.x + threadIdx.x) >> 2; i2 < total; i2 += gridDim.x * blockDim.x >> 2) {
         const bool is_v = i2 & 1;
+        // (head, row) of a number below 2^32 by a 32-bit division, beyond that by a 64-bit one
+        const int h = total >> 33 ? (int)((i2 >> 1) / rows) : (int)((unsigned)(i2 >> 1) / rows);
+        const unsigned i = (unsigned)((i2 >> 1) - (long)h * rows);
         const long pos = start + i;
         if (pos < 0) {
             if (t == 0) atomicOr(status, KV4_BAD_POSITION);
@@ -302,13 +313,13 @@ kv4_read_kernel(Kv4Cache C, const int32_t *__restrict__ first, const int32_t *__
 #pragma unroll
             for (int j = 0; j < NB; ++j) w[j] = from[j];
         }
-        const __half2 *params = reinterpret_cast<const __half2 *>(is_v ? C.v_params : C.k_params) + row * (NB >> (bpg >> 1));
+        const __half2 *params = reinterpret_cast<const __half2 *>(is_v ? C.v_params : C.k_params) + row * (NB / BPG);
         T *to = (is_v ? v_out : k_out) + (((long)b * C.heads + h) * out_len + i) * D + 8 * t;
         float2 p = make_float2(0.f, 0.f);
 #pragma unroll
         for (int j = 0; j < NB; ++j) {
-            if ((j & (bpg - 1)) == 0) {
-                p = __half22float2(params[j >> (bpg >> 1)]);
+            if (j % BPG == 0) {
+                p = __half22float2(params[j / BPG]);
                 p.x *= 16777216.f;           // the codes come as fp16 subnormals, c 2^-24: exact either way
             }
             // units (2 t, j) and (2 t + 1, j): dims 8 t .. + 3 in the low half, + 4 .. + 7 in the high one
@@ -326,18 +337,16 @@ kv4_read_kernel(Kv4Cache C, const int32_t *__restrict__ first, const int32_t *__
     }
 }
 
-// calls f with the number of 32-dim blocks as a constant
+// calls f with the number of 32-dim blocks of a row and of a group as constants
 template <typename F>
-static int kv4_by_blocks(int d, F f) {
-    switch (d / 32) {
-        case 1: return f(std::integral_constant<int, 1>());
-        case 2: return f(std::integral_constant<int, 2>());
-        case 3: return f(std::integral_constant<int, 3>());
-        case 4: return f(std::integral_constant<int, 4>());
-        case 5: return f(std::integral_constant<int, 5>());
-        case 6: return f(std::integral_constant<int, 6>());
-        case 7: return f(std::integral_constant<int, 7>());
-        default: return f(std::integral_constant<int, 8>());
+static void kv4_by_shape(int d, int g, F f) {
+    using std::integral_constant;
+    switch (d / 32 * 10 + g / 32) {
+#define KV4_SHAPE(NB, BPG) \
+    case NB * 10 + BPG: return f(integral_constant<int, NB>(), integral_constant<int, BPG>());
+        KV4_SHAPE(1, 1) KV4_SHAPE(2, 1) KV4_SHAPE(2, 2) KV4_SHAPE(3, 1) KV4_SHAPE(4, 1) KV4_SHAPE(4, 2) KV4_SHAPE(4, 4) KV4_SHAPE(5, 1)
+        KV4_SHAPE(6, 1) KV4_SHAPE(6, 2) KV4_SHAPE(7, 1) KV4_SHAPE(8, 1) KV4_SHAPE(8, 2) KV4_SHAPE(8, 4)
+#undef KV4_SHAPE
     }
 }
 
@@ -361,11 +370,10 @@ static int kv4_append_launch(const char *name, const T *nk, const T *nv, const K
     if (batch == 0 || tokens == 0) return 0;
     int *status = status_word();
     if (!status) return B200K_E_WORKSPACE;
-    const dim3 grid(kv4_grid(2l * tokens * C.heads, 16, batch), batch);
-    kv4_by_blocks(C.d, [&](auto nb) {
-        launch_kernel(kv4_append_kernel<T, nb()>, grid, dim3(128), 0, to_stream(stream), nk, nv, C, first, new_lens, tokens, (long)stride_kt,
+    const dim3 grid(kv4_grid((long)tokens * C.heads, 16, batch), batch);
+    kv4_by_shape(C.d, C.g, [&](auto nb, auto bpg) {
+        launch_kernel(kv4_append_kernel<T, nb(), bpg()>, grid, dim3(128), 0, to_stream(stream), nk, nv, C, first, new_lens, tokens, (long)stride_kt,
                       (long)stride_vt, status);
-        return 0;
     });
     return launch_status(name);
 }
@@ -383,10 +391,9 @@ static int kv4_rope_append_launch(const char *name, const T *qkv, const float *c
     if (!status) return B200K_E_WORKSPACE;
     const int vec = aligned16(cos_t) && aligned16(sin_t);
     const dim3 grid(ceil_div(hq + 2 * C.heads, 16), batch);
-    kv4_by_blocks(C.d, [&](auto nb) {
-        launch_kernel(kv4_rope_append_kernel<T, nb()>, grid, dim3(128), 0, to_stream(stream), qkv, cos_t, sin_t, positions, q_out, C, lens_out, hq, vec,
+    kv4_by_shape(C.d, C.g, [&](auto nb, auto bpg) {
+        launch_kernel(kv4_rope_append_kernel<T, nb(), bpg()>, grid, dim3(128), 0, to_stream(stream), qkv, cos_t, sin_t, positions, q_out, C, lens_out, hq, vec,
                       status);
-        return 0;
     });
     return launch_status(name);
 }
@@ -397,16 +404,15 @@ static int kv4_read_launch(const char *name, const Kv4Cache &C, bool paged, cons
     B200K_REQUIRE(lens && k_out && v_out, B200K_E_NULL, "%s: NULL pointer", name);
     int rc = kv4_check(name, C, batch, paged);
     if (rc) return rc;
-    B200K_REQUIRE(C.heads <= 65535, B200K_E_SHAPE, "%s: heads %d", name, C.heads);
     B200K_REQUIRE(out_len >= 0 && out_len <= KV4_MAX_LEN, B200K_E_SHAPE, "%s: out_len %d", name, out_len);
     B200K_REQUIRE(aligned16(k_out) && aligned16(v_out), B200K_E_ALIGN, "%s: k_out and v_out must be 16-byte aligned", name);
     if (batch == 0 || out_len == 0) return 0;
     int *status = status_word();
     if (!status) return B200K_E_WORKSPACE;
-    const dim3 grid(kv4_grid(2l * out_len, 64, (long)batch * C.heads), C.heads, batch);
-    kv4_by_blocks(C.d, [&](auto nb) {
-        launch_kernel(kv4_read_kernel<T, nb()>, grid, dim3(256), 0, to_stream(stream), C, first, lens, k_out, v_out, out_len, status);
-        return 0;
+    const int threads = 8l * out_len * C.heads <= 128 ? 64 : 256;       // a few rows a sequence: small blocks
+    const dim3 grid(kv4_grid(2l * out_len * C.heads, threads / 4, batch), batch);
+    kv4_by_shape(C.d, C.g, [&](auto nb, auto bpg) {
+        launch_kernel(kv4_read_kernel<T, nb(), bpg()>, grid, dim3(threads), 0, to_stream(stream), C, first, lens, k_out, v_out, out_len, status);
     });
     return launch_status(name);
 }
