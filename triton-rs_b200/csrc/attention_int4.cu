@@ -23,14 +23,8 @@
 
 namespace b200k {
 
-#ifndef A4_NSTAGES
-#define A4_NSTAGES 2
-#endif
 #ifndef A4_NSUBS
 #define A4_NSUBS 2
-#endif
-#ifndef A4_EDGE
-#define A4_EDGE __forceinline__
 #endif
 #ifndef A4_WAVES
 #define A4_WAVES 1
@@ -41,7 +35,7 @@ namespace b200k {
 #ifndef A4_C4
 #define A4_C4 4
 #endif
-constexpr int A4_WARPS = 4, A4_THREADS = 32 * A4_WARPS, A4_STAGES = A4_NSTAGES;
+constexpr int A4_WARPS = 4, A4_THREADS = 32 * A4_WARPS, A4_STAGES = 2;
 constexpr int A4_TILE = 16, A4_SUBS = A4_NSUBS;                // positions of a tile (the rows of an MMA), tiles of a stage
 constexpr int A4_STEP = A4_SUBS * A4_TILE, A4_UNIT = A4_WARPS * A4_STEP;       // positions of a warp's stage, of a unit of work
 constexpr int A4_MAX_CTAS = A4_MAXC;                              // CTAs of a launch
@@ -181,20 +175,15 @@ __device__ __forceinline__ void a4_kdims(int i, int n, int t, int &lo, int &hi) 
 template <int NB, int NG, bool PURE>
 __device__ __forceinline__ constexpr int a4_kgroup(int i) { return PURE ? i : (i % (NB / 2)) * 2 * NG / NB; }
 
-// The copies of a tile of which not all rows are there, or that spans blocks: row by row, zeros for the rows behind the context and
-// for those in a block that the pool does not have; a mask of the rows that are there goes to the stage's last word.  Not
-// inlined: its code would be met between that of the whole tiles.  `first` < 0 with one block: the block is not there.
+// The copies of a tile of which not all rows are there, or that spans blocks, or one of whose blocks the pool does not have: row
+// by row, zeros for what is not there; a mask of the rows that are there goes to the tile's last words.
 template <int NB, int NG>
-__device__ A4_EDGE void a4_copy_edge(const Attn4Args &A, int b, int kvh, int p0, int len, long first, bool one, uint32_t dst_codes,
-                                          uint32_t dst_params, const unsigned char *params, uint32_t mask) {
+__device__ __forceinline__ void a4_copy_edge(const Attn4Args &A, int b, int kvh, int p0, int len, uint32_t dst_codes, uint32_t dst_params,
+                                             uint32_t mask) {
     using X = A4<NB, NG>;
     const Kv4Cache &C = A.C;
     const int lane = threadIdx.x & 31;
-    auto row_of = [&](int row) {
-        if (p0 + row >= len) return -1l;
-        if (one) return first < 0 ? -1l : first + row;
-        return kv4_row(C, b, kvh, p0 + row);
-    };
+    auto row_of = [&](int row) { return p0 + row < len ? kv4_row(C, b, kvh, p0 + row) : -1l; };
 #pragma unroll 1
     for (int c = lane; c < A4_TILE * NB; c += 32) {
         const long row = row_of(c / NB);
@@ -204,9 +193,9 @@ __device__ A4_EDGE void a4_copy_edge(const Attn4Args &A, int b, int kvh, int p0,
         a4_copy<16>(dst + A4_TILE * X::ROW, (const unsigned char *)C.v_codes + off, row < 0 ? 0 : 16);
     }
     const long row = row_of(lane & 15);
+    const unsigned char *params = (const unsigned char *)(lane < 16 ? C.k_params : C.v_params) + max(row, 0l) * X::PROW;
 #pragma unroll
-    for (int c = 0; c < X::PROW; c += X::PCOPY)
-        a4_copy<X::PCOPY>(dst_params + c, params + (row < 0 ? 0 : row - (lane & 15)) * X::PROW + c, row < 0 ? 0 : X::PCOPY);
+    for (int c = 0; c < X::PROW; c += X::PCOPY) a4_copy<X::PCOPY>(dst_params + c, params + c, row < 0 ? 0 : X::PCOPY);
     const unsigned valid = __ballot_sync(0xffffffffu, row >= 0) & 0xffffu;
     if (lane == 0) {
         asm volatile("st.shared.u32 [%0], %1;" ::"r"(mask), "r"(valid) : "memory");
@@ -298,11 +287,9 @@ attn4_kernel(const __grid_constant__ Attn4Args A) {
     // ---- streaming a piece: tile i of this warp goes to stage i % STAGES ------------------------------------------------------------
     // 16 neighbouring rows are one linear part of the cache, so a tile that is whole and lies in one block takes nothing but
     // copies at fixed distances
-    int tiles, whole;                      // tiles of this segment; so many from the first on are whole (head-major caches)
+    int tiles, whole;                      // stages of a segment; so many from the first on are whole (where blocks hold whole tiles)
     const unsigned char *src_k = nullptr, *src_v = nullptr, *src_p = nullptr;
     const bool paged = C.block_table != nullptr;
-    auto params = [&] { return (const unsigned char *)(lane < 16 ? C.k_params : C.v_params) + (lane & 15) * X::PROW; };
-    auto row_at = [&](const Attn4Segment &d, int i) { return ((long)d.b * C.heads + d.kvh) * C.capacity + (d.u0 + i) * A4_UNIT + warp * A4_STEP; };
     auto copy_whole = [&](uint32_t stage, const unsigned char *k, const unsigned char *v, const unsigned char *p) {
 #pragma unroll
         for (int c = 0; c < NB; c += 2)
@@ -313,36 +300,48 @@ attn4_kernel(const __grid_constant__ Attn4Args A) {
 #pragma unroll
         for (int c = 0; c < X::PROW; c += X::PCOPY) a4_copy<X::PCOPY>(dst_params + stage + c, p + c, X::PCOPY);
     };
+    // returns whether the tiles need a look at their masks
     auto issue = [&](const Attn4Segment &d, int i, uint32_t stage) {
-        if (i < whole) {
+        bool fine = i < whole;
+        if (fine) {
+            if (paged) {
+                // blocks of whole tiles: a tile lies in one block
+                const int p0 = (d.u0 + i) * A4_UNIT + warp * A4_STEP;
+                int lb = (int)__umul64hi((unsigned long long)p0, A.block_magic), slot = p0 - lb * C.block_size;
+                long row[A4_SUBS];
 #pragma unroll
-            for (int s = 0; s < A4_SUBS; ++s)
-                copy_whole(stage + s * X::SUB, src_k + s * A4_TILE * X::ROW, src_v + s * A4_TILE * X::ROW, src_p + s * A4_TILE * X::PROW);
-            src_k += A4_UNIT * X::ROW;
-            src_v += A4_UNIT * X::ROW;
-            src_p += A4_UNIT * X::PROW;
-        } else if (i < tiles) {
-            const bool one = !paged || C.block_size % A4_TILE == 0;
-#pragma unroll 1
-            for (int s = 0; s < A4_SUBS; ++s, stage += X::SUB) {
-                const int p0 = (d.u0 + i) * A4_UNIT + warp * A4_STEP + s * A4_TILE;
-                long first = row_at(d, i) + s * A4_TILE;
-                if (paged && one && p0 < d.len) {
-                    const int lb = (int)__umul64hi((unsigned long long)p0, A.block_magic);
+                for (int s = 0; s < A4_SUBS; ++s) {
                     const int blk = C.block_table[(long)d.b * C.max_blocks + lb];
-                    first = (unsigned)blk < (unsigned)C.num_blocks ? ((long)blk * C.heads + d.kvh) * C.block_size + (p0 - lb * C.block_size) : -1;
+                    fine = fine && (unsigned)blk < (unsigned)C.num_blocks;
+                    row[s] = ((long)blk * C.heads + d.kvh) * C.block_size + slot;
+                    slot += A4_TILE;
+                    if (slot == C.block_size) {
+                        slot = 0;
+                        ++lb;
+                    }
                 }
-                const uint32_t mask = ring + stage + X::SUB - 32;
-                if (one && p0 + A4_TILE <= d.len && first >= 0) {
-                    copy_whole(stage, (const unsigned char *)C.k_codes + first * X::ROW + lane * 16,
-                               (const unsigned char *)C.v_codes + first * X::ROW + lane * 16, params() + first * X::PROW);
-                    if (lane == 0) asm volatile("st.shared.u32 [%0], %1;" ::"r"(mask), "r"(0xffffu) : "memory");
-                } else {
-                    a4_copy_edge<NB, NG>(A, d.b, d.kvh, p0, d.len, first, one, dst_codes + stage, dst_params + stage, params(), mask);
+                if (fine) {
+#pragma unroll
+                    for (int s = 0; s < A4_SUBS; ++s)
+                        copy_whole(stage + s * X::SUB, src_k + row[s] * X::ROW, src_v + row[s] * X::ROW, src_p + row[s] * X::PROW);
                 }
+            } else {
+#pragma unroll
+                for (int s = 0; s < A4_SUBS; ++s)
+                    copy_whole(stage + s * X::SUB, src_k + s * A4_TILE * X::ROW, src_v + s * A4_TILE * X::ROW, src_p + s * A4_TILE * X::PROW);
+                src_k += A4_UNIT * X::ROW;
+                src_v += A4_UNIT * X::ROW;
+                src_p += A4_UNIT * X::PROW;
             }
         }
+        const bool edge = !fine && i < tiles;
+        if (edge)
+#pragma unroll 1
+            for (int s = 0; s < A4_SUBS; ++s)
+                a4_copy_edge<NB, NG>(A, d.b, d.kvh, (d.u0 + i) * A4_UNIT + warp * A4_STEP + s * A4_TILE, d.len, dst_codes + stage + s * X::SUB,
+                                     dst_params + stage + s * X::SUB, ring + stage + (s + 1) * X::SUB - 32);
         asm volatile("cp.async.commit_group;" ::: "memory");
+        return edge;
     };
 #pragma unroll 1
     for (;;) {
@@ -367,13 +366,12 @@ attn4_kernel(const __grid_constant__ Attn4Args A) {
         __syncthreads();
         const Attn4Segment &d = sm_seg;
         tiles = d.u1 - d.u0;
-        whole = paged ? 0 : min(max((d.len - (warp + 1) * A4_STEP + A4_UNIT) / A4_UNIT - d.u0, 0), tiles);
-        const long row0 = row_at(d, 0);
+        whole = paged && C.block_size % A4_TILE ? 0 : min(max((d.len - (warp + 1) * A4_STEP + A4_UNIT) / A4_UNIT - d.u0, 0), tiles);
+        const long row0 = paged ? 0l : ((long)d.b * C.heads + d.kvh) * C.capacity + d.u0 * A4_UNIT + warp * A4_STEP;
         src_k = (const unsigned char *)C.k_codes + row0 * X::ROW + lane * 16;
         src_v = (const unsigned char *)C.v_codes + row0 * X::ROW + lane * 16;
-        src_p = params() + row0 * X::PROW;
-#pragma unroll 1
-        for (int i = 0; i < A4_STAGES - 1; ++i) issue(d, i, i * X::STAGE);
+        src_p = (const unsigned char *)(lane < 16 ? C.k_params : C.v_params) + (row0 + (lane & 15)) * X::PROW;
+        bool edge = issue(d, 0, 0);
 
         // ---- q as the B operand, a word by each warp; scaled by a power of two to [2^14, 2^15) -------------------------------------------
         // (any 16-bit type then fits fp16 with all its bits, down to 2^-25 of the head's largest element; nibbles 1 and 3 carry
@@ -452,15 +450,15 @@ attn4_kernel(const __grid_constant__ Attn4Args A) {
         uint32_t stage = 0;
 #pragma unroll 1
         for (int i = 0; i < tiles; ++i) {
-            asm volatile("cp.async.wait_group %0;" ::"n"(A4_STAGES - 2) : "memory");
+            asm volatile("cp.async.wait_group 0;" ::: "memory");
             __syncwarp();
-            issue(d, i + A4_STAGES - 1, stage == 0 ? (A4_STAGES - 1) * X::STAGE : stage - X::STAGE);
-            const bool edge = i >= whole;         // some rows may have to be left out
+            const bool look = edge;               // some rows may have to be left out
+            edge = issue(d, i + 1, stage ^ X::STAGE);
 #pragma unroll
             for (int sub = 0; sub < A4_SUBS; ++sub) {
             const uint32_t st = stage + sub * X::SUB;
             bool ok0 = true, ok1 = true;
-            if (edge) {
+            if (look) {
                 uint32_t valid;
                 a4_lds<1>(&valid, ring + st + X::SUB - 32);
                 ok0 = (valid >> kpos) & 1;
@@ -520,7 +518,7 @@ attn4_kernel(const __grid_constant__ Attn4Args A) {
             float vs0[NG], vz0[NG], vs1[NG], vz1[NG];
             a4_params<NG>(vs0, vz0, pw0 + NG);
             a4_params<NG>(vs1, vz1, pw1 + NG);
-            if (edge) {
+            if (look) {
                 if (!ok0) s[0] = s[1] = -1e30f;
                 if (!ok1) s[2] = s[3] = -1e30f;
             }
@@ -561,7 +559,7 @@ attn4_kernel(const __grid_constant__ Attn4Args A) {
             p[1] = a4_exp2(fmaf(s[1], fac[1], -ref[1]));
             p[2] = a4_exp2(fmaf(s[2], fac[0], -ref[0]));
             p[3] = a4_exp2(fmaf(s[3], fac[1], -ref[1]));
-            if (edge) {
+            if (look) {
                 if (!ok0) p[0] = p[1] = 0.f;
                 if (!ok1) p[2] = p[3] = 0.f;
             }
@@ -597,7 +595,7 @@ attn4_kernel(const __grid_constant__ Attn4Args A) {
                               a4_lds16(at_v0 + st + 8 * X::ROW + 2 * j) | a4_lds16(at_v1 + st + 8 * X::ROW + 2 * j) << 16);
             }
             }
-            stage = stage == (A4_STAGES - 1) * X::STAGE ? 0 : stage + X::STAGE;
+            stage ^= X::STAGE;
         }
 
         // ---- join the warps ------------------------------------------------------------------------------------------------------
