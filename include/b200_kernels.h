@@ -777,6 +777,11 @@ int b200k_layer_set_norms_rope(b200k_layer *layer, const b200k_half *ln1, const 
                                const float *cos_table, const float *sin_table);
 /* caches [max_batch, num_kv_heads, max_len, D] fp16 head-major, caller-owned. */
 int b200k_layer_set_kv_cache(b200k_layer *layer, b200k_half *k_cache, b200k_half *v_cache);
+/* The cache in 4 bits instead (head-major, see "4-bit KV cache"): codes [max_batch, num_kv_heads, max_len, head_dim/8], params
+ * [max_batch, num_kv_heads, max_len, head_dim/kv_group_size, 2], caller-owned.  The layer then rotates, quantises and appends in
+ * one kernel and attends over the codes; the same ten launches.  Whichever cache is set last is the one in use. */
+int b200k_layer_set_kv_cache_int4(b200k_layer *layer, int32_t *k_codes, b200k_half *k_params, int32_t *v_codes,
+                                  b200k_half *v_params, int kv_group_size);
 /* ---- tensor-parallel exchange: one-shot all-reduce over NVLink peer memory -----------------------
  * No counterpart in the reference, which is single-GPU (its consumer would call NCCL).  One process
  * per GPU.  Each rank creates an exchange buffer (flags + two slots of slot_bytes), publishes its

@@ -106,6 +106,23 @@ def test_refusals(pkg, call, kw, code):
     assert e.value.code == code, e.value.message
 
 
+def test_layer_cache_refusals(pkg):
+    L = pkg.lib()
+    for args, code in ([(None, PTR, PTR, PTR, PTR, 64), NULL], [(PTR, None, PTR, PTR, PTR, 64), NULL], [(PTR, PTR, PTR, PTR, None, 64), NULL],
+                       [(PTR, PTR, PTR, PTR, PTR, 48), SHAPE], [(PTR, PTR, PTR + 4, PTR, PTR, 64), ALIGN]):
+        with pytest.raises(pkg.B200KError) as e:
+            L.call("b200k_layer_set_kv_cache_int4", *args)
+        assert e.value.code == code
+
+
+def test_cache_tensors(pkg):
+    codes, params = pkg.prelude.int4_kv_cache(3, 2, 5, 96, 32, "cpu")
+    assert codes.shape == (3, 2, 5, 12) and params.shape == (3, 2, 5, 3, 2)
+    for d, g in ((100, 32), (96, 64)):
+        with pytest.raises(ValueError):
+            pkg.prelude.int4_kv_cache(1, 1, 1, d, g, "cpu")
+
+
 def test_empty_calls_launch_nothing(pkg):
     L = pkg.lib()
     _append(L, b=0); _append(L, t=0); _append_paged(L, b=0); _rope(L, b=0); _read(L, b=0); _read(L, ol=0); _attn(L, b=0); _attn_paged(L, b=0)

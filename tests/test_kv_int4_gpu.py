@@ -582,3 +582,56 @@ def test_chunked_prefill_then_decode(P, pkg, oracle):
             done += 1
             c.attend(P, "f16", qr, t(np.array([done], np.int32)), out, scale)
             check_attention(oracle, c, qr, [done], out, scale, "f16")
+
+
+@pytest.mark.parametrize("use_graph", [False, True])
+@pytest.mark.parametrize("awq", [False, True])
+def test_decode_layer_over_a_4_bit_cache(pkg, P, oracle, use_graph, awq):
+    """The layer's steps with the 4-bit cache, against the same entry points called one by one (bit for bit), and a switch back to
+    the fp16 cache."""
+    rng = np.random.default_rng(5)
+    B, H, hq, hkv, d, I, G, ml, kg = 3, 256, 4, 2, 128, 384, 128, 40, 64
+
+    def weight(k, n):
+        sc = rng.uniform(0.002, 0.02, (k // G, n)).astype(np.float16)
+        if awq:
+            return (t(oracle.pack_awq(rng.integers(0, 16, (k, n), dtype=np.int32))), t(sc), t(oracle.pack_awq(rng.integers(0, 16, (k // G, n), dtype=np.int32))))
+        return (t(oracle.pack_gptq_qweight(rng.integers(1, 16, (k, n), dtype=np.int32))), t(sc), t(np.full((k // G, n // 8), 0x77777777, dtype=np.int32)))
+    w = {"qkv": weight(H, (hq + 2 * hkv) * d), "o": weight(hq * d, H), "gate_up": weight(H, 2 * I), "down": weight(I, H)}
+    ln1, ln2 = (t(rng.uniform(0.5, 1.5, H).astype(np.float16)) for _ in range(2))
+    cos, sin = (t(a) for a in oracle.rope_tables(ml, d, 500000.0))
+    fmt = "awq" if awq else "gptq"
+    layer = pkg.DecodeLayer(pkg.LayerShape(H, hq, hkv, d, I, G, 1e-5), w, ln1, ln2, cos, sin, max_batch=4, max_len=ml, fmt=fmt, use_graph=use_graph,
+                            kv_group_size=kg)
+    c = Cache(4, hkv, d, kg, ml)
+    c.words, c.params = [torch.zeros_like(x) for x in c.words], [torch.zeros_like(x) for x in c.params]
+    gemm = P.awq_gemm if awq else P.gptq_gemm
+    hid, pos, out = torch.empty(B, H, dtype=torch.float16, device=DEV), torch.empty(B, dtype=torch.int32, device=DEV), torch.empty(B, H, dtype=torch.float16, device=DEV)
+    for p in ([5, 0, 38], [6, 1, 39], [7, 2, 3]):               # the first step captures, the others replay
+        hid.copy_(torch.from_numpy(rng.standard_normal((B, H)).astype(np.float16)))
+        pos.copy_(torch.tensor(p, dtype=torch.int32))
+        layer.forward(hid, pos, out=out)
+        n1, n2, h1, want = (torch.empty_like(hid) for _ in range(4))
+        P.rms_norm_f16(hid, ln1, n1, H, 1.0 / H, 1e-5, B)
+        qkv = gemm(n1, *w["qkv"], G)
+        q, att = (torch.empty(B, hq, d, dtype=torch.float16, device=DEV) for _ in range(2))
+        P.rope_kv_append_hm_int4_f16(qkv, cos, sin, pos, q, *c.tensors, hq, hkv, d, kg, ml, B)
+        P.batched_decode_attention_hm_int4_f16(q, *c.tensors, pos + 1, att, B, hq, hkv, d, kg, ml, 1.0 / float(np.sqrt(d)))
+        o = gemm(att.view(B, hq * d), *w["o"], G)
+        P.fused_add_rms_norm_f16(o, hid, ln2, n2, h1, H, 1.0 / H, 1e-5, B)
+        gu = gemm(n2, *w["gate_up"], G)
+        act = torch.empty(B, I, dtype=torch.float16, device=DEV)
+        P.fused_silu_mul_interleaved_f16(gu, act, I, B * I)
+        dn = gemm(act, *w["down"], G)
+        P.residual_add_f16(h1, dn, want, B * H)
+        torch.cuda.synchronize()
+        assert torch.isfinite(out).all() and torch.equal(out, want)
+        for a, b in zip((*layer.k_cache, *layer.v_cache), c.tensors):
+            assert torch.equal(a, b)
+    half = [torch.zeros(4, hkv, ml, d, dtype=torch.float16, device=DEV) for _ in "kv"]
+    pkg.lib().call("b200k_layer_set_kv_cache", layer.handle, *half)
+    before = [x.clone() for x in (*layer.k_cache, *layer.v_cache)]
+    layer.forward(hid, pos, out=out)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(before, (*layer.k_cache, *layer.v_cache)))
+    layer.close()

@@ -828,6 +828,14 @@ static int attn4_launch(const char *name, const void *q, const Kv4Cache &C, bool
     return fail(B200K_E_SHAPE, "%s: head_dim %d, group_size %d", name, C.d, C.g);
 }
 
+// The head-major call with the output in the pre-permuted order the int4 GEMM wants, where asked for (used by the decode layer)
+int batched_decode_attention_hm_int4_f16_layer(const __half *q, const int32_t *kc, const __half *kp, const int32_t *vc, const __half *vp,
+                                               const int32_t *context_lens, __half *output, int batch, int hq, int hkv, int d, int g, int max_len,
+                                               float scale, bool kperm, cudaStream_t st) {
+    return attn4_launch("batched_decode_attention_hm_int4_f16", q, kv4_cache(kc, (const b200k_half *)kp, vc, (const b200k_half *)vp, hkv, d, g, max_len),
+                        false, context_lens, output, batch, hq, scale, false, kperm, nullptr, 0, true, (b200k_stream)st);
+}
+
 }  // namespace b200k
 
 using namespace b200k;

@@ -13,6 +13,13 @@ namespace b200k {
 int rope_kv_append_lens_launch(const __half *qkv, const float *cos_t, const float *sin_t, const int32_t *positions,
                                __half *q_out, __half *kc, __half *vc, int32_t *lens_out, int hq, int hkv, int d,
                                int max_len, int batch, cudaStream_t st);
+// the same step and attention over a 4-bit cache (kv_int4.cu, attention_int4.cu)
+int rope_kv_append_int4_lens_launch(const __half *qkv, const float *cos_t, const float *sin_t, const int32_t *positions, __half *q_out, int32_t *kc,
+                                    __half *kp, int32_t *vc, __half *vp, int32_t *lens_out, int hq, int hkv, int d, int g, int max_len, int batch,
+                                    cudaStream_t st);
+int batched_decode_attention_hm_int4_f16_layer(const __half *q, const int32_t *kc, const __half *kp, const int32_t *vc, const __half *vp,
+                                               const int32_t *context_lens, __half *output, int batch, int hq, int hkv, int d, int g, int max_len,
+                                               float scale, bool kperm, cudaStream_t st);
 // peer-to-peer all-reduce (comm.cu): the partial sums sit in slot `slot` of every rank's exchange buffer
 int comm_allreduce_f16(struct ::b200k_comm *comm, int slot, __half *out, size_t count, cudaStream_t st);
 int comm_allreduce_add_f16(struct ::b200k_comm *comm, int slot, const __half *addend, __half *out, size_t count, cudaStream_t st);
@@ -38,7 +45,10 @@ struct b200k_layer {
     const int32_t *qz[4];
     const b200k_half *ln1, *ln2;
     const float *cos_t, *sin_t;
-    b200k_half *kc, *vc;
+    b200k_half *kc, *vc;             // the cache in fp16, or
+    int32_t *k_codes, *v_codes;      // in 4 bits: the one that was set last
+    b200k_half *k_params, *v_params;
+    int kv_group;
     struct b200k_comm *comm;
     // activations (device), sized for max_batch
     b200k_half *x_in, *n1, *qkv, *qrot, *att, *o, *h1, *n2, *gu, *act, *dn, *y_out;
@@ -77,6 +87,17 @@ static int stage0(b200k_layer *L, const b200k_half *hidden, const int32_t *posit
     else rc = rms_norm_f16(hidden, L->ln1, L->n1, H, 1.0f / H, c.rms_eps, b, st);
     if (rc) return rc;
     if ((rc = gemm(L, 0, L->n1, L->qkv, b, (hq + 2 * hkv) * d, H, st))) return rc;
+    if (L->k_codes) {
+        if ((rc = rope_kv_append_int4_lens_launch((const __half *)L->qkv, L->cos_t, L->sin_t, positions, (__half *)L->qrot, L->k_codes,
+                                                  (__half *)L->k_params, L->v_codes, (__half *)L->v_params, L->lens, hq, hkv, d, L->kv_group,
+                                                  c.max_len, b, to_stream(st))))
+            return rc;
+        if ((rc = batched_decode_attention_hm_int4_f16_layer((const __half *)L->qrot, L->k_codes, (const __half *)L->k_params, L->v_codes,
+                                                             (const __half *)L->v_params, L->lens, (__half *)L->att, b, hq, hkv, d, L->kv_group,
+                                                             c.max_len, 1.0f / sqrtf((float)d), L->kperm, to_stream(st))))
+            return rc;
+        return gemm(L, 1, L->att, o_out, b, H, hq * d, st);
+    }
     if ((rc = rope_kv_append_lens_launch((const __half *)L->qkv, L->cos_t, L->sin_t, positions, (__half *)L->qrot,
                                          (__half *)L->kc, (__half *)L->vc, L->lens, hq, hkv, d, c.max_len, b,
                                          to_stream(st))))
@@ -153,7 +174,7 @@ static int check_ready(const b200k_layer *L, int batch, const char *name) {
     for (int i = 0; i < 4; ++i)
         B200K_REQUIRE(L->qw[i] && L->sc[i], B200K_E_STATE, "%s: weight %d not set", name, i);
     B200K_REQUIRE(L->ln1 && L->ln2 && L->cos_t && L->sin_t, B200K_E_STATE, "%s: norms / RoPE tables not set", name);
-    B200K_REQUIRE(L->kc && L->vc, B200K_E_STATE, "%s: KV cache not set", name);
+    B200K_REQUIRE((L->kc && L->vc) || L->k_codes, B200K_E_STATE, "%s: KV cache not set", name);
     B200K_REQUIRE(batch >= 0 && batch <= L->cfg.max_batch, B200K_E_SHAPE, "%s: batch %d outside 0..%d", name, batch,
                   L->cfg.max_batch);
     return 0;
@@ -247,6 +268,20 @@ extern "C" int b200k_layer_set_norms_rope(b200k_layer *L, const b200k_half *ln1,
 extern "C" int b200k_layer_set_kv_cache(b200k_layer *L, b200k_half *k_cache, b200k_half *v_cache) {
     B200K_REQUIRE(L && k_cache && v_cache, B200K_E_NULL, "b200k_layer_set_kv_cache: NULL pointer");
     L->kc = k_cache; L->vc = v_cache;
+    L->k_codes = L->v_codes = nullptr;
+    drop_graphs(L);
+    return 0;
+}
+extern "C" int b200k_layer_set_kv_cache_int4(b200k_layer *L, int32_t *k_codes, b200k_half *k_params, int32_t *v_codes, b200k_half *v_params,
+                                             int kv_group_size) {
+    B200K_REQUIRE(L && k_codes && k_params && v_codes && v_params, B200K_E_NULL, "b200k_layer_set_kv_cache_int4: NULL pointer");
+    B200K_REQUIRE(kv_group_size == 32 || kv_group_size == 64 || kv_group_size == 128, B200K_E_SHAPE,
+                  "b200k_layer_set_kv_cache_int4: group size %d (32, 64 or 128)", kv_group_size);
+    B200K_REQUIRE(aligned16(k_codes) && aligned16(k_params) && aligned16(v_codes) && aligned16(v_params), B200K_E_ALIGN,
+                  "b200k_layer_set_kv_cache_int4: codes and params must be 16-byte aligned");
+    L->k_codes = k_codes; L->k_params = k_params; L->v_codes = v_codes; L->v_params = v_params;
+    L->kv_group = kv_group_size;
+    L->kc = L->vc = nullptr;
     drop_graphs(L);
     return 0;
 }

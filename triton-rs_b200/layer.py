@@ -150,7 +150,9 @@ class DecodeLayer:
     ORDER = ("qkv", "o", "gate_up", "down")
 
     def __init__(self, shape: LayerShape, weights, ln1, ln2, cos, sin, max_batch, max_len, fmt="gptq",
-                 use_graph=True, k_cache=None, v_cache=None):
+                 use_graph=True, k_cache=None, v_cache=None, kv_group_size=None):
+        """kv_group_size 32, 64 or 128: the KV cache is held in 4 bits with that many dims to a (scale, base); k_cache and v_cache
+        are then (codes, params) pairs, see `prelude.int4_kv_cache`.  None: in fp16."""
         self.shape, self.max_batch, self.max_len = shape, max_batch, max_len
         self._L = lib()
         cfg = _Config(shape.hidden, shape.num_q_heads, shape.num_kv_heads, shape.head_dim, shape.intermediate,
@@ -165,6 +167,13 @@ class DecodeLayer:
             self._L.call("b200k_layer_set_weight", self.handle, i, qw, sc, qz)
         self._L.call("b200k_layer_set_norms_rope", self.handle, ln1, ln2, cos, sin)
         dev = ln1.device
+        self.kv_group_size = kv_group_size
+        if kv_group_size is not None:
+            if k_cache is None:
+                from .prelude import int4_kv_cache
+                k_cache, v_cache = (int4_kv_cache(max_batch, shape.num_kv_heads, max_len, shape.head_dim, kv_group_size, dev) for _ in "kv")
+            self.set_kv_cache(k_cache, v_cache)
+            return
         if k_cache is None:
             k_cache = torch.zeros((max_batch, shape.num_kv_heads, max_len, shape.head_dim), dtype=torch.float16, device=dev)
             v_cache = torch.zeros_like(k_cache)
@@ -173,6 +182,9 @@ class DecodeLayer:
 
     def set_kv_cache(self, k_cache, v_cache):
         self.k_cache, self.v_cache = k_cache, v_cache
+        if self.kv_group_size is not None:
+            self._L.call("b200k_layer_set_kv_cache_int4", self.handle, *k_cache, *v_cache, self.kv_group_size)
+            return
         self._L.call("b200k_layer_set_kv_cache", self.handle, k_cache, v_cache)
 
     def set_comm(self, comm: "Comm | None"):

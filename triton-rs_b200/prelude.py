@@ -78,3 +78,13 @@ def awq_gemm(a, qweight, scales, qzeros, group_size, out=None):
                                      qweight.stride(0), qweight.stride(1), scales.stride(0), scales.stride(1),
                                      qzeros.stride(0), qzeros.stride(1), c.stride(0), c.stride(1))
     return c
+
+
+def int4_kv_cache(batch, num_heads, max_len, head_dim, group_size, device="cuda"):
+    """(codes, params) of an empty head-major 4-bit cache tensor (K or V); with batch = num_blocks and max_len = block_size, of a
+    paged pool."""
+    if head_dim % 32 or head_dim % group_size:
+        raise ValueError(f"head_dim {head_dim} must be a multiple of 32 and of group_size {group_size}")
+    lead = (batch, num_heads, max_len)
+    return (torch.zeros(lead + (head_dim // 8,), dtype=torch.int32, device=device),
+            torch.zeros(lead + (head_dim // group_size, 2), dtype=torch.float16, device=device))

@@ -544,6 +544,10 @@ extern "C" {
     pub fn b200k_layer_set_kv_cache(
         layer: *mut b200k_layer, k_cache: *mut b200k_half, v_cache: *mut b200k_half
     ) -> c_int;
+    pub fn b200k_layer_set_kv_cache_int4(
+        layer: *mut b200k_layer, k_codes: *mut i32, k_params: *mut b200k_half, v_codes: *mut i32,
+        v_params: *mut b200k_half, kv_group_size: c_int
+    ) -> c_int;
     pub fn b200k_comm_create(
         rank: c_int, world: c_int, slot_bytes: usize, out_comm: *mut *mut b200k_comm
     ) -> c_int;
