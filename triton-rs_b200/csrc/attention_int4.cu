@@ -41,6 +41,7 @@ constexpr int A4_STEP = A4_SUBS * A4_TILE, A4_UNIT = A4_WARPS * A4_STEP;       /
 constexpr int A4_MAX_CTAS = A4_MAXC;                              // CTAs of a launch
 constexpr int A4_FAN = 16;                                     // partial results that are joined at a time
 constexpr int A4_HEADS = 8;                                    // columns of one MMA
+constexpr float A4_MIDDLE = 7.5f;     // of the codes
 constexpr float A4_LAZY = 6.f;        // the running maximum moves when a score passes it by 2^6: probabilities stay below 2^6
 constexpr float A4_TOP = 512.f;       // 2^e times the largest value scale is set to [2^2, 2^3) and set again when it passes 2^9
 
@@ -143,8 +144,15 @@ __device__ __forceinline__ uint32_t a4_keep(uint32_t x) {
 
 // The eight codes of a word as four operand registers: nibbles 0 and 2 of both halves as c 2^-24, 1 and 3 as c 2^-20.  Four
 // integer instructions and a subtraction (exact) on the other pipe: the integer one runs at half rate and is the busiest here.
-__device__ __forceinline__ void a4_codes(uint32_t x, uint32_t &n0, uint32_t &n1, uint32_t &n2, uint32_t &n3) {
+__device__ __forceinline__ void a4_codes(uint32_t x, uint32_t &n0, uint32_t &n1, uint32_t &n2, uint32_t &n3, bool fifteen_minus = false) {
     const uint32_t y = __byte_perm(x, 0, 0x4341);
+    if (fifteen_minus) {
+        n0 = ~x & 0x000f000fu;
+        n1 = ~x & 0x00f000f0u;
+        n2 = ~y & 0x000f000fu;
+        n3 = ~y & 0x00f000f0u;
+        return;
+    }
     n0 = x & 0x000f000fu;
     n1 = x & 0x00f000f0u;
     n3 = y & 0x00f000f0u;
@@ -308,16 +316,23 @@ attn4_kernel(const __grid_constant__ Attn4Args A) {
                 // blocks of whole tiles: a tile lies in one block
                 const int p0 = (d.u0 + i) * A4_UNIT + warp * A4_STEP;
                 int lb = (int)__umul64hi((unsigned long long)p0, A.block_magic), slot = p0 - lb * C.block_size;
-                long row[A4_SUBS];
-#pragma unroll
-                for (int s = 0; s < A4_SUBS; ++s) {
-                    const int blk = C.block_table[(long)d.b * C.max_blocks + lb];
+                const int32_t *table = C.block_table + (long)d.b * C.max_blocks;
+                auto look_up = [&] {
+                    const int blk = table[lb];
                     fine = fine && (unsigned)blk < (unsigned)C.num_blocks;
-                    row[s] = ((long)blk * C.heads + d.kvh) * C.block_size + slot;
+                    return ((long)blk * C.heads + d.kvh) * C.block_size + slot;
+                };
+                long row[A4_SUBS];
+                row[0] = look_up();
+#pragma unroll
+                for (int s = 1; s < A4_SUBS; ++s) {
                     slot += A4_TILE;
                     if (slot == C.block_size) {
                         slot = 0;
                         ++lb;
+                        row[s] = look_up();
+                    } else {
+                        row[s] = row[s - 1] + A4_TILE;
                     }
                 }
                 if (fine) {
@@ -434,13 +449,15 @@ attn4_kernel(const __grid_constant__ Attn4Args A) {
             for (int i = 0; i < NB; ++i) qsum[a4_kgroup<NB, NG, X::PURE>(i)][e2] += sm_qsum[i][2 * t + e2];
         }
 
-        float oacc[X::MTILES][4], zacc[NG][2], l[2] = {0.f, 0.f};
+        // sacc: the sum of w (below), group 2 i in the first two registers, 2 i + 1 in the others
+        float oacc[X::MTILES][4], sacc[(NG + 1) / 2][4], zacc[NG][2], l[2] = {0.f, 0.f};
 #pragma unroll
         for (int i = 0; i < X::MTILES; ++i)
 #pragma unroll
             for (int j = 0; j < 4; ++j) oacc[i][j] = 0.f;
 #pragma unroll
-        for (int g = 0; g < NG; ++g) zacc[g][0] = zacc[g][1] = 0.f;
+        for (int g = 0; g < NG; ++g) zacc[g][0] = zacc[g][1] = sacc[g / 2][2 * (g & 1)] = sacc[g / 2][2 * (g & 1) + 1] = 0.f;
+        if (NG & 1) sacc[NG / 2][2] = sacc[NG / 2][3] = 0.f;
         // top: the running maximum of the raw scores; a probability is 2^(score fac - ref), ref = top fac - e: the factor 2^e,
         // the same for all heads, keeps probability times value scale inside fp16 and cancels in the end
         float top[2] = {-1e30f, -1e30f}, ref[2] = {0.f, 0.f}, bar[2] = {-1e30f, -1e30f}, e = 0.f, most = -1.f;
@@ -468,8 +485,10 @@ attn4_kernel(const __grid_constant__ Attn4Args A) {
             // scores: rows r and r + 8 are positions kpos0 and kpos0 + 8, columns heads 2t and 2t + 1
             float s[4] = {0.f, 0.f, 0.f, 0.f};
             uint32_t pw0[2 * NG], pw1[2 * NG];     // params of these rows: K's, V's
-            a4_lds<2 * NG>(pw0, at_p + st);
-            a4_lds<2 * NG>(pw1, at_p + st + 16 * X::PROW);
+            // with many groups V's words wait until they are needed: registers are short
+            constexpr bool LATE = NG >= 4 && NB == 4;
+            a4_lds<LATE ? NG : 2 * NG>(pw0, at_p + st);
+            a4_lds<LATE ? NG : 2 * NG>(pw1, at_p + st + 16 * X::PROW);
             {
                 uint32_t w0[NB], w1[NB];
                 if constexpr (NB == 8) {
@@ -509,11 +528,17 @@ attn4_kernel(const __grid_constant__ Attn4Args A) {
             }
             constexpr int VW = NB % 2 == 0 ? NB / 2 : 1;
             uint32_t va[VW], vb[VW], vc[VW], vd[VW];
-            if constexpr (NB % 2 == 0) {
+            auto load_v = [&] {
                 a4_lds<VW>(va, at_v0 + st);
                 a4_lds<VW>(vb, at_v1 + st);
                 a4_lds<VW>(vc, at_v0 + st + 8 * X::ROW);
                 a4_lds<VW>(vd, at_v1 + st + 8 * X::ROW);
+            };
+            if constexpr (LATE) {
+                a4_lds<NG>(pw0 + NG, at_p + st + X::PROW);
+                a4_lds<NG>(pw1 + NG, at_p + st + 17 * X::PROW);
+            } else if constexpr (NB % 2 == 0) {
+                load_v();
             }
             float vs0[NG], vz0[NG], vs1[NG], vz1[NG];
             a4_params<NG>(vs0, vz0, pw0 + NG);
@@ -550,7 +575,12 @@ attn4_kernel(const __grid_constant__ Attn4Args A) {
                 l[0] *= a0;
                 l[1] *= a1;
 #pragma unroll
-                for (int g = 0; g < NG; ++g) { zacc[g][0] *= a0; zacc[g][1] *= a1; }
+                for (int g = 0; g < NG; ++g) {
+                    zacc[g][0] *= a0;
+                    zacc[g][1] *= a1;
+                    sacc[g / 2][2 * (g & 1)] *= a0;
+                    sacc[g / 2][2 * (g & 1) + 1] *= a1;
+                }
 #pragma unroll
                 for (int m = 0; m < X::MTILES; ++m) { oacc[m][0] *= a0; oacc[m][1] *= a1; oacc[m][2] *= a0; oacc[m][3] *= a1; }
             }
@@ -565,24 +595,36 @@ attn4_kernel(const __grid_constant__ Attn4Args A) {
             }
             l[0] += p[0] + p[2];
             l[1] += p[1] + p[3];
-            uint32_t pb[NG][2];            // (probability x value scale)^T as the B operand; the one rounding to fp16 on the way
+            // w = probability x value scale, rounded to fp16, is the B operand.  With it
+            //   sum p v = sum w (c - 7.5) + sum p (z + 7.5 s) = sum w c - 7.5 sum w + sum p (z + 7.5 s)
+            // so that its rounding meets a code's distance from the middle, not the code; a product with ones gives sum w.  Every
+            // other tile adds -w (15 - c) in place of w c: the codes are not centred, their sum would grow with the context, and
+            // the tensor cores truncate.  Output error (batch 64, context 4096, fp16): 6e-4 without either, 3e-4 without the
+            // second, 2.1e-4 being what rounding the output alone leaves.
+            constexpr uint32_t ONES = 0x3c003c00u;
+            const float sign = sub & 1 ? -1.f : 1.f;
+            uint32_t pb[NG][2];
 #pragma unroll
             for (int g = 0; g < NG; ++g) {
-                pb[g][0] = a4_transpose(f2_to_h2(p[0] * vs0[g], p[1] * vs0[g]));
-                pb[g][1] = a4_transpose(f2_to_h2(p[2] * vs1[g], p[3] * vs1[g]));
-                zacc[g][0] = fmaf(p[0], vz0[g], fmaf(p[2], vz1[g], zacc[g][0]));
-                zacc[g][1] = fmaf(p[1], vz0[g], fmaf(p[3], vz1[g], zacc[g][1]));
+                const float y0 = fmaf(vs0[g], A4_MIDDLE, vz0[g]), y1 = fmaf(vs1[g], A4_MIDDLE, vz1[g]);
+                pb[g][0] = a4_transpose(f2_to_h2(p[0] * (sign * vs0[g]), p[1] * (sign * vs0[g])));
+                pb[g][1] = a4_transpose(f2_to_h2(p[2] * (sign * vs1[g]), p[3] * (sign * vs1[g])));
+                zacc[g][0] = fmaf(p[0], y0, fmaf(p[2], y1, zacc[g][0]));
+                zacc[g][1] = fmaf(p[1], y0, fmaf(p[3], y1, zacc[g][1]));
+                if (g & 1) a4_mma(sacc[g / 2], 0u, ONES, 0u, ONES, pb[g][0], pb[g][1]);
+                else a4_mma(sacc[g / 2], ONES, 0u, ONES, 0u, pb[g][0], pb[g][1]);
             }
             // output: rows r and r + 8 of m-tile 2 j + h are dims 32 j + 4 r + 2 h and + 1
             auto out_tiles = [&](int j, uint32_t x, uint32_t y) {
                 const int g = j * NG / NB;
                 uint32_t x0, x1, x2, x3, y0, y1, y2, y3;
-                a4_codes(x, x0, x1, x2, x3);
-                a4_codes(y, y0, y1, y2, y3);
+                a4_codes(x, x0, x1, x2, x3, sub & 1);
+                a4_codes(y, y0, y1, y2, y3, sub & 1);
                 a4_mma(oacc[2 * j], x0, x1, y0, y1, pb[g][0], pb[g][1]);
                 a4_mma(oacc[2 * j + 1], x2, x3, y2, y3, pb[g][0], pb[g][1]);
             };
             if constexpr (NB % 2 == 0) {
+                if constexpr (LATE) load_v();
 #pragma unroll
                 for (int j = 0; j < NB; ++j) {
                     const int sel = j & 1 ? 0x7632 : 0x5410;
@@ -639,7 +681,8 @@ attn4_kernel(const __grid_constant__ Attn4Args A) {
 #pragma unroll
             for (int m = 0; m < X::MTILES; ++m) {
                 const int g = (m / 2) * NG / NB;
-                const float za = zacc[g][0] * wgt[0], zb = zacc[g][1] * wgt[1];
+                const float za = fmaf(sacc[g / 2][2 * (g & 1)], -A4_MIDDLE, zacc[g][0]) * wgt[0];
+                const float zb = fmaf(sacc[g / 2][2 * (g & 1) + 1], -A4_MIDDLE, zacc[g][1]) * wgt[1];
                 *reinterpret_cast<float2 *>(o0 + m * 16 * A4_HEADS) =
                     make_float2(fmaf(oacc[m][0], 16777216.f * wgt[0], za), fmaf(oacc[m][1], 16777216.f * wgt[1], zb));
                 *reinterpret_cast<float2 *>(o0 + (m * 16 + 8) * A4_HEADS) =
