@@ -212,10 +212,11 @@ __device__ __forceinline__ void a4_copy_edge(const Attn4Args &A, int b, int kvh,
     }
 }
 
-// A segment: units [u0, u1) of the n that a context (sequence b, kv head, q heads [h0, h0 + heads)) has.
+// A segment: units [u0, u1) of the n that a context (sequence b, kv head, q heads [h0, h0 + heads)) has.  The context is spread
+// over `members` CTAs from c0 on.  `more`: another segment follows for this CTA.
 struct Attn4Segment {
-    int b, kvh, h0, heads, len, u0, u1, n;
-    unsigned item_start;            // units before this sequence
+    int b, kvh, h0, heads, len, u0, u1, n, c0, members, more;
+    unsigned seq_start;             // units before this sequence
 };
 
 template <int NB, int NG>
@@ -233,51 +234,117 @@ attn4_kernel(const __grid_constant__ Attn4Args A) {
     pdl_wait();
     pdl_launch_dependents();
 
-    // ---- the share of this CTA: units [at, end) of all (the host made sure that 32 bits hold them) --------------------------------
+    // ---- the share of this CTA, by warp 0 (the host made sure that 32 bits hold all units) ----------------------------------------
+    // Either one piece of one context, all contexts being cut into pieces of at most `share` units, no more pieces than CTAs; or,
+    // where the largest piece would be over an eighth more than an equal share, units [at, end) of all, which may begin and end
+    // within contexts: a CTA then joins and starts anew wherever it passes from one to the next.  One context of 131071
+    // positions: 38.7 us in pieces, 43 cut evenly; 32 of 512 to 8192 positions, the pieces up to a third larger: 58.5 and 57.2.
     const unsigned per_seq = C.heads * A.head_blocks;      // contexts of a sequence
     auto units_of = [&](int b) { return (unsigned)(max(min(A.lens[b], C.capacity), 0) + A4_UNIT - 1) / A4_UNIT; };
-    unsigned total = 0;
+    auto place_heads = [&](Attn4Segment &d, unsigned ctx) {
+        const unsigned hb = ctx % A.head_blocks, gqa = A.hq / C.heads;
+        d.kvh = ctx / A.head_blocks;
+        d.h0 = d.kvh * gqa + hb * A4_HEADS;
+        d.heads = min((unsigned)A4_HEADS, gqa - hb * A4_HEADS);
+        d.len = min(A.lens[d.b], C.capacity);
+    };
+    unsigned share = 0, at = 0, end = 0;                   // warp 0's
+    auto segment = [&](Attn4Segment d) {                   // the one that begins with unit `at`, of sequence d.b or a later one
+        unsigned n = units_of(d.b);
+        while (at >= d.seq_start + n * per_seq) {
+            d.seq_start += n * per_seq;
+            n = units_of(++d.b);
+        }
+        const unsigned ctx = (at - d.seq_start) / n, first = d.seq_start + ctx * n;       // units before this context
+        place_heads(d, ctx);
+        d.n = n;
+        d.u0 = at - first;
+        d.u1 = min(n, end - first);
+        d.c0 = first / share;
+        d.members = (first + n - 1) / share - d.c0 + 1;
+        at = first + d.u1;
+        d.more = at < end;
+        sm_seg = d;
+    };
+    if (warp == 0) {
+        unsigned total = 0, contexts = 0;
 #pragma unroll 4
-    for (int b = lane; b < A.batch; b += 32) total += units_of(b);
-    total = __reduce_add_sync(0xffffffffu, total) * per_seq;
-    const unsigned share = max((total + gridDim.x - 1) / gridDim.x, 1u);
+        for (int b = lane; b < A.batch; b += 32) {
+            const unsigned n = units_of(b);
+            total += n;
+            contexts += n > 0;
+        }
+        total = __reduce_add_sync(0xffffffffu, total) * per_seq;
+        contexts = __reduce_add_sync(0xffffffffu, contexts) * per_seq;
+        share = max((total + gridDim.x - 1) / gridDim.x, 1u);
+        bool cut = contexts > gridDim.x;                   // pieces will not do
+        for (unsigned s = share; !cut && share > 1;) {     // with a unit for every CTA, units are the pieces
+            unsigned pieces = 0;
+#pragma unroll 4
+            for (int b = lane; b < A.batch; b += 32) pieces += (units_of(b) + s - 1) / s;
+            pieces = __reduce_add_sync(0xffffffffu, pieces) * per_seq;
+            if (pieces <= gridDim.x) {
+                share = s;
+                break;
+            }
+            s = max(s + 1, (unsigned)(((unsigned long long)s * (pieces + gridDim.x)) / (2 * gridDim.x)));
+            cut = s > share + share / 8 + 1;
+        }
+        // the sequence that this CTA's first unit, or its piece, belongs to
+        if (cut) {
+            at = share * blockIdx.x;
+            end = min(at + share, total);
+        }
+        const unsigned mark = cut ? at : blockIdx.x;
+        unsigned before = 0;
+        if (lane == 0) sm_seg.n = 0;                       // nothing to do
+        __syncwarp();
 #pragma unroll 1
-    for (int b = blockIdx.x; b < A.batch; b += gridDim.x) {
-        const int len = A.lens[b];
-        if (len > C.capacity && tid == 0) atomicOr(A.status, KV4_BAD_POSITION);
-        if (len <= 0)       // no keys: a zero output row
-#pragma unroll 1
-            for (int i = tid; i < A.hq * X::D / 2; i += A4_THREADS) reinterpret_cast<uint32_t *>(A.out)[(long)b * A.hq * X::D / 2 + i] = 0u;
-    }
-    unsigned at = share * blockIdx.x;
-    const unsigned end = min(at + share, total);
-    if (at >= end) return;
-    if (warp == 0) {        // the sequence that unit `at` belongs to
-        unsigned start = 0;
-        int b = 0;
-#pragma unroll 1
-        for (int b0 = 0;; b0 += 32) {
-            const unsigned mine = b0 + lane < A.batch ? units_of(b0 + lane) * per_seq : 0u;
+        for (int b0 = 0; b0 < A.batch && (!cut || at < end); b0 += 32) {
+            const unsigned n = b0 + lane < A.batch ? units_of(b0 + lane) : 0u, parts = cut ? n : (n + share - 1) / share;
+            const unsigned mine = parts * per_seq;
             unsigned upto = mine;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
                 const unsigned x = __shfl_up_sync(0xffffffffu, upto, o);
                 if (lane >= o) upto += x;
             }
-            const unsigned past = __ballot_sync(0xffffffffu, start + upto > at);
+            const unsigned past = __ballot_sync(0xffffffffu, before + upto > mark);
             if (past) {
-                const int found = __ffs(past) - 1;
-                b = b0 + found;
-                start += __shfl_sync(0xffffffffu, upto - mine, found);
+                if (lane == __ffs(past) - 1) {
+                    Attn4Segment d = {};
+                    d.b = b0 + lane;
+                    d.seq_start = before + upto - mine;
+                    if (cut) {
+                        segment(d);
+                    } else {
+                        const unsigned piece = mark - d.seq_start, ctx = piece / parts, part = piece % parts, size = (n + parts - 1) / parts;
+                        place_heads(d, ctx);
+                        d.n = n;
+                        d.u0 = part * size;
+                        d.u1 = min(n, (part + 1) * size);
+                        d.c0 = blockIdx.x - part;
+                        d.members = parts;
+                        sm_seg = d;
+                    }
+                }
+                at = __shfl_sync(0xffffffffu, at, __ffs(past) - 1);
                 break;
             }
-            start += __shfl_sync(0xffffffffu, upto, 31);
+            before += __shfl_sync(0xffffffffu, upto, 31);
         }
-        if (lane == 0) {
-            sm_seg.b = b;
-            sm_seg.item_start = start;
+    } else {
+#pragma unroll 1
+        for (int b = blockIdx.x; b < A.batch; b += gridDim.x) {
+            const int len = A.lens[b];
+            if (len > C.capacity && tid == 32) atomicOr(A.status, KV4_BAD_POSITION);
+            if (len <= 0)       // no keys: a zero output row
+#pragma unroll 1
+                for (int i = tid - 32; i < A.hq * X::D / 2; i += A4_THREADS - 32) reinterpret_cast<uint32_t *>(A.out)[(long)b * A.hq * X::D / 2 + i] = 0u;
         }
     }
+    __syncthreads();
+    if (sm_seg.n == 0) return;
 
     const uint32_t ring = smem_u32(smem) + warp * A4_STAGES * X::STAGE;
     // where this lane's first 16-byte piece goes in a tile of a stage, and its row of params: lanes 0-15 copy those of K, 16-31 those
@@ -360,25 +427,6 @@ attn4_kernel(const __grid_constant__ Attn4Args A) {
     };
 #pragma unroll 1
     for (;;) {
-        if (tid == 0) {                    // the segment that begins with unit `at`
-            Attn4Segment d = sm_seg;       // its sequence and the units before that, or those of the segment before
-            unsigned seq_start = d.item_start, n = units_of(d.b);
-            while (at >= seq_start + n * per_seq) {
-                seq_start += n * per_seq;
-                n = units_of(++d.b);
-            }
-            const unsigned ctx = (at - seq_start) / n, hb = ctx % A.head_blocks, gqa = A.hq / C.heads;
-            d.item_start = seq_start;
-            d.kvh = ctx / A.head_blocks;
-            d.h0 = d.kvh * gqa + hb * A4_HEADS;
-            d.heads = min((unsigned)A4_HEADS, gqa - hb * A4_HEADS);
-            d.len = min(A.lens[d.b], C.capacity);
-            d.n = n;
-            d.u0 = at - seq_start - ctx * n;
-            d.u1 = min(n, d.u0 + (end - at));
-            sm_seg = d;
-        }
-        __syncthreads();
         const Attn4Segment &d = sm_seg;
         tiles = d.u1 - d.u0;
         whole = paged && C.block_size % A4_TILE ? 0 : min(max((d.len - (warp + 1) * A4_STEP + A4_UNIT) / A4_UNIT - d.u0, 0), tiles);
@@ -706,8 +754,8 @@ attn4_kernel(const __grid_constant__ Attn4Args A) {
         // these sums, always in CTA order -------------------------------------------------------------------------------------------
         bool last = true;
         if (d.u1 - d.u0 < d.n) {           // not the whole context was here
-            const unsigned first = at - d.u0, c0 = first / share;       // units before this context; the CTA it begins in
-            int members = (first + d.n - 1) / share - c0 + 1, me = blockIdx.x - c0, step = 1;
+            const int c0 = d.c0;
+            int members = d.members, me = blockIdx.x - c0, step = 1;
             // a CTA has two places: for a context that it continues, and for one that it begins
             auto place = [&](int c) { return (int)(c0 + c) * 2 + (c == 0); };
             int *counters = A.counters;
@@ -805,8 +853,9 @@ attn4_kernel(const __grid_constant__ Attn4Args A) {
                 }
             }
         }
-        at += d.u1 - d.u0;
-        if (at >= end) break;
+        if (!d.more) break;
+        __syncthreads();                   // everybody has done with this segment
+        if (tid == 0) segment(sm_seg);
         __syncthreads();
     }
 }
@@ -850,7 +899,7 @@ static int attn4_launch(const char *name, const void *q, const Kv4Cache &C, bool
     A.counters = (int *)((unsigned char *)ws + A4_COUNTERS_OFF);
     A.parts = (float *)((unsigned char *)ws + A4_PARTS_OFF);
     const long max_units = (long)batch * C.heads * A.head_blocks * (((long)C.capacity + A4_UNIT - 1) / A4_UNIT);
-    B200K_REQUIRE(max_units < (1l << 31), B200K_E_SHAPE, "%s: batch * num_kv_heads * ceil(gqa / 8) * ceil(positions / 64) = %ld exceeds 31 bits", name, max_units);
+    B200K_REQUIRE(max_units < (1l << 31), B200K_E_SHAPE, "%s: batch * num_kv_heads * ceil(gqa / 8) * ceil(positions / 128) = %ld exceeds 31 bits", name, max_units);
     cudaStream_t st = to_stream(stream);
     switch (C.d / 32 * 1000 + C.d / C.g) {
         case 1001: return attn4_launch_as<1, 1>(name, A, max_units, st);
