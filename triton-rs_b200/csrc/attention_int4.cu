@@ -217,6 +217,7 @@ __device__ __forceinline__ void a4_copy_edge(const Attn4Args &A, int b, int kvh,
 struct Attn4Segment {
     int b, kvh, h0, heads, len, u0, u1, n, c0, members, more;
     unsigned seq_start;             // units before this sequence
+    unsigned share, at, end;        // units of a CTA; those that follow this segment in this CTA: [at, end)
 };
 
 template <int NB, int NG>
@@ -236,7 +237,7 @@ attn4_kernel(const __grid_constant__ Attn4Args A) {
 
     // ---- the share of this CTA, by warp 0 (the host made sure that 32 bits hold all units) ----------------------------------------
     // Either one piece of one context, all contexts being cut into pieces of at most `share` units, no more pieces than CTAs; or,
-    // where the largest piece would be over an eighth more than an equal share, units [at, end) of all, which may begin and end
+    // where the largest piece would be over a sixth more than an equal share, units [at, end) of all, which may begin and end
     // within contexts: a CTA then joins and starts anew wherever it passes from one to the next.  One context of 131071
     // positions: 38.7 us in pieces, 43 cut evenly; 32 of 512 to 8192 positions, the pieces up to a third larger: 58.5 and 57.2.
     const unsigned per_seq = C.heads * A.head_blocks;      // contexts of a sequence
@@ -248,34 +249,36 @@ attn4_kernel(const __grid_constant__ Attn4Args A) {
         d.heads = min((unsigned)A4_HEADS, gqa - hb * A4_HEADS);
         d.len = min(A.lens[d.b], C.capacity);
     };
-    unsigned share = 0, at = 0, end = 0;                   // warp 0's
-    auto segment = [&](Attn4Segment d) {                   // the one that begins with unit `at`, of sequence d.b or a later one
+    auto segment = [&](Attn4Segment d) {                   // the one that begins with unit d.at, of sequence d.b or a later one
         unsigned n = units_of(d.b);
-        while (at >= d.seq_start + n * per_seq) {
+#pragma unroll 1
+        while (d.at >= d.seq_start + n * per_seq) {
             d.seq_start += n * per_seq;
             n = units_of(++d.b);
         }
-        const unsigned ctx = (at - d.seq_start) / n, first = d.seq_start + ctx * n;       // units before this context
+        const unsigned ctx = (d.at - d.seq_start) / n, first = d.seq_start + ctx * n;       // units before this context
         place_heads(d, ctx);
         d.n = n;
-        d.u0 = at - first;
-        d.u1 = min(n, end - first);
-        d.c0 = first / share;
-        d.members = (first + n - 1) / share - d.c0 + 1;
-        at = first + d.u1;
-        d.more = at < end;
+        d.u0 = d.at - first;
+        d.u1 = min(n, d.end - first);
+        d.c0 = first / d.share;
+        d.members = (first + n - 1) / d.share - d.c0 + 1;
+        d.at = first + d.u1;
+        d.more = d.at < d.end;
         sm_seg = d;
     };
     if (warp == 0) {
-        unsigned total = 0, contexts = 0;
+        unsigned total = 0, contexts = 0, longest = 0, share, at = 0, end = 0;
 #pragma unroll 4
         for (int b = lane; b < A.batch; b += 32) {
             const unsigned n = units_of(b);
             total += n;
             contexts += n > 0;
+            longest = max(longest, n);
         }
         total = __reduce_add_sync(0xffffffffu, total) * per_seq;
         contexts = __reduce_add_sync(0xffffffffu, contexts) * per_seq;
+        longest = __reduce_max_sync(0xffffffffu, longest);
         share = max((total + gridDim.x - 1) / gridDim.x, 1u);
         bool cut = contexts > gridDim.x;                   // pieces will not do
         for (unsigned s = share; !cut && share > 1;) {     // with a unit for every CTA, units are the pieces
@@ -287,8 +290,11 @@ attn4_kernel(const __grid_constant__ Attn4Args A) {
                 share = s;
                 break;
             }
-            s = max(s + 1, (unsigned)(((unsigned long long)s * (pieces + gridDim.x)) / (2 * gridDim.x)));
-            cut = s > share + share / 8 + 1;
+            // a piece fewer for the longest context
+            const unsigned parts = (longest + s - 1) / s;
+            cut = parts < 2;
+            if (!cut) s = (longest + parts - 2) / (parts - 1);
+            cut = cut || s > share + share / 6 + 2;
         }
         // the sequence that this CTA's first unit, or its piece, belongs to
         if (cut) {
@@ -316,6 +322,9 @@ attn4_kernel(const __grid_constant__ Attn4Args A) {
                     d.b = b0 + lane;
                     d.seq_start = before + upto - mine;
                     if (cut) {
+                        d.share = share;
+                        d.at = at;
+                        d.end = end;
                         segment(d);
                     } else {
                         const unsigned piece = mark - d.seq_start, ctx = piece / parts, part = piece % parts, size = (n + parts - 1) / parts;
@@ -328,7 +337,6 @@ attn4_kernel(const __grid_constant__ Attn4Args A) {
                         sm_seg = d;
                     }
                 }
-                at = __shfl_sync(0xffffffffu, at, __ffs(past) - 1);
                 break;
             }
             before += __shfl_sync(0xffffffffu, upto, 31);
