@@ -441,10 +441,13 @@ def big_cache(oracle, b, hkv, d, g, n, seed, block=0):
     (3, 8, 2, 128, 128, 64, [9000, 0, 4097]),
     (40, 8, 1, 64, 32, 0, None),
     (2, 16, 1, 256, 64, 16, [5000, 12]),
+    (200, 8, 4, 128, 64, 0, None),        # more contexts than CTAs: a CTA goes through several, cut at both ends
+    (90, 16, 8, 64, 64, 16, None),
+    (1, 4, 1, 64, 32, 0, [80001]),        # one context over every CTA: three rounds of joining
 ])
 def test_attention_long_and_ragged(P, oracle, b, hq, hkv, d, g, block, lens):
     rng = np.random.default_rng(b)
-    lens = lens or [int(x) for x in rng.integers(0, 1500, b)]
+    lens = lens or [int(x) for x in rng.integers(0, 1500 if b < 50 else 400, b)]
     c = big_cache(oracle, b, hkv, d, g, max(lens), 70 + b, block)
     q = values((b, hq, d), "f16", 71)
     out = torch.full((b, hq, d), float("nan"), dtype=torch.float16, device=DEV)
@@ -463,6 +466,24 @@ def test_attention_length_beyond_the_cache_is_clamped_and_reported(P, pkg, oracl
     assert status(pkg) == 4 and torch.equal(want, got)
     c.attend(P, "f16", q, t(np.array([700, 37, -(2 ** 31)], np.int32)), got, 0.088)
     assert status(pkg) == 0 and torch.equal(want[:2], got[:2]) and (got[2] == 0).all()
+
+
+def test_tables_that_share_blocks(P, oracle):
+    """Sequences with a common prefix read the same blocks; a table entry behind a context may be anything."""
+    hq, hkv, d, g, block, n = 8, 2, 128, 64, 16, 100
+    c = Cache(3, hkv, d, g, n, block)
+    k, v = (as64(values((1, hkv, n, d), "f16", s)).repeat(3, 0) for s in (91, 92))
+    c.table[1:] = c.table[0]
+    c.dtable = t(c.table)
+    c.fill(k, v, [n, n, n], oracle)
+    q = values((1, hq, d), "f16", 93).repeat(3, 1, 1)
+    out = torch.empty_like(q)
+    lens = [n, 33, 48]
+    bad = c.table.copy()
+    bad[1, 3:], bad[2, 3:] = 2 ** 31 - 1, -5
+    c.dtable = t(bad)
+    c.attend(P, "f16", q, t(np.array(lens, np.int32)), out, 0.088)
+    check_attention(oracle, c, q, lens, out, 0.088, "f16")
 
 
 def test_attention_offsets_beyond_32_bits(P, oracle):
@@ -519,6 +540,31 @@ def test_two_streams_with_a_workspace_each(P, pkg, oracle):
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(want, got))
     assert all(int(w[:128 * 1024].count_nonzero()) == 0 for w in ws)          # counters and status word left at zero
+
+
+def test_two_graphs_share_a_workspace(P, pkg, oracle):
+    """Two captured calls of different shapes on one workspace, replayed in turn: every launch finds the counters at zero."""
+    cs = [big_cache(oracle, 1, 8, 128, 64, 9000, 1), big_cache(oracle, 130, 5, 64, 32, 300, 2)]
+    qs = [values((1, 32, 128), "f16", 3), values((130, 10, 64), "bf16", 4)]
+    lens = [t(np.array([9000], np.int32)), t(np.random.default_rng(3).integers(0, 301, 130).astype(np.int32))]
+    kinds, scale = ["f16", "bf16"], 0.1
+    ws = torch.zeros(pkg.lib().call("b200k_attention_int4_workspace_bytes", 1, 32, 8, 128), dtype=torch.uint8, device=DEV)
+    want, got, graphs = [], [], []
+    for c, q, n, k in zip(cs, qs, lens, kinds):
+        want.append(torch.empty_like(q))
+        got.append(torch.empty_like(q))
+        c.attend(P, k, q, n, want[-1], scale)
+    torch.cuda.synchronize()
+    for c, q, n, k, o in zip(cs, qs, lens, kinds, got):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            c.attend(P, k, q, n, o, scale, ws=ws)
+    for i in (0, 1, 1, 0, 0, 1):
+        got[i].zero_()
+        graphs[i].replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got[i], want[i])
+    assert int(ws[:128 * 1024].count_nonzero()) == 0
 
 
 def test_captured_graph_follows_the_lengths(P, oracle):

@@ -5,40 +5,32 @@
 //   sum_p w_p V[p]  = sum_p (w_p s_pg) c_pd + sum_p w_p z_pg
 // so the matrix instructions multiply by the codes themselves and the scales go to the sums (K) and the probabilities (V).
 // A masked nibble is already an fp16 number: bits 0-3 of a half are the subnormal c 2^-24, bits 4-7 are c 2^-20, both exact,
-// so eight codes cost one shift and four ANDs (and one byte permute where two positions have to share a register).  The
-// factors of two go to q (K side) and to the output (V side).  Dequantising to fp16 first would take two more
-// instructions for every pair of codes and round every value.
+// so eight codes cost five instructions (and a byte permute where two positions have to share a register).  The factors of
+// two go to q (K side) and to the output (V side).  Dequantising to fp16 first would take two more instructions for
+// every pair of codes and round every value.
 //
 // mma.sync m16n8k16 in transposed form, as in the 16-bit kernel: positions (K) or dims (V) fill the 16 rows, up to 8 q heads
-// of a GQA group the 8 columns; one query token a sequence cannot fill a 128-row tcgen05 tile, and the kernel is bound by
-// memory and by the issue of the integer instructions above, not by the tensor pipe.
+// of a GQA group the 8 columns; one query token a sequence cannot fill a 128-row tcgen05 tile.
 //
-// Work is cut evenly, not by sequence: the units of 64 positions of all (sequence, kv head, block of 8 q heads) are numbered
-// through, and every CTA of one wave takes the same number of consecutive units, whatever the lengths are; it works that out
-// from the lengths on the device, so a captured graph follows them.  A (sequence, head) that more than one CTA works on
-// is joined by the last of them to finish, in CTA order.  Each warp streams its 16-position tiles through a ring of
-// cp.async stages of its own, without any barrier between warps; rows behind the context are filled with zeros and never read.
+// What bounds it: the bytes of the cache where contexts are long (74 x 8 contexts of 16384 positions, D 128, groups of 64:
+// 236 us, 0.91 of the copy bandwidth), and just below that the issue of instructions: about 250 a warp for 16 positions of K
+// and V, half of them on the integer pipe, at 0.6 a cycle and scheduler; HBM delivers 16 positions to an SM every 96 cycles.
+// At 64 x 4096 positions (46 us of bytes) 66 us: starting takes 4 us, the joins of the CTAs 4, and the rest is the issue
+// rate.  Groups of 32 take a third more instructions (83 us), groups of 128 a tenth fewer (58 us).
+//
+// Work is dealt out on the device, from the lengths, so a captured graph follows them; see the kernel's first part.  Each warp
+// streams two 16-position tiles a stage through a ring of cp.async stages of its own, without a barrier between warps: four
+// warps a CTA, four CTAs an SM at head_dim 128 keep 74 KB under way.  (Three stages instead of two: 92 instead of 64 us, the
+// shared memory then leaves no room for the fourth CTA.  One tile a stage: 66 us.)  Rows behind the context are not read.
 #include "kv_int4.cuh"
 #include "tma.cuh"
 
 namespace b200k {
 
-#ifndef A4_NSUBS
-#define A4_NSUBS 2
-#endif
-#ifndef A4_WAVES
-#define A4_WAVES 1
-#endif
-#ifndef A4_MAXC
-#define A4_MAXC 640
-#endif
-#ifndef A4_C4
-#define A4_C4 4
-#endif
 constexpr int A4_WARPS = 4, A4_THREADS = 32 * A4_WARPS, A4_STAGES = 2;
-constexpr int A4_TILE = 16, A4_SUBS = A4_NSUBS;                // positions of a tile (the rows of an MMA), tiles of a stage
+constexpr int A4_TILE = 16, A4_SUBS = 2;                // positions of a tile (the rows of an MMA), tiles of a stage
 constexpr int A4_STEP = A4_SUBS * A4_TILE, A4_UNIT = A4_WARPS * A4_STEP;       // positions of a warp's stage, of a unit of work
-constexpr int A4_MAX_CTAS = A4_MAXC;                              // CTAs of a launch
+constexpr int A4_MAX_CTAS = 640;                               // CTAs of a launch: one wave
 constexpr int A4_FAN = 16;                                     // partial results that are joined at a time
 constexpr int A4_HEADS = 8;                                    // columns of one MMA
 constexpr float A4_MIDDLE = 7.5f;     // of the codes
@@ -71,7 +63,7 @@ struct A4 {
     static constexpr int MTILES = 2 * NB;
     static constexpr bool PURE = G == 32;                     // a group is one block: see kword()
     static constexpr int PART = D * A4_HEADS + 16;            // floats of a partial result
-    static constexpr int CTAS = NB <= 4 ? A4_C4 : NB <= 5 ? 3 : 2;
+    static constexpr int CTAS = NB <= 4 ? 4 : NB <= 5 ? 3 : 2;
     static constexpr int RING = A4_WARPS * A4_STAGES * STAGE;
     static constexpr int JOIN = A4_WARPS * D * A4_HEADS * 4;  // the warps' results
     static constexpr int SMEM = RING > JOIN ? RING : JOIN;    // in turn
@@ -878,7 +870,7 @@ static int attn4_launch_as(const char *name, const Attn4Args &A, long max_units,
     static OncePerDevice once;
     cudaError_t e = once.run([&] { return cudaFuncSetAttribute(attn4_kernel<NB, NG>, cudaFuncAttributeMaxDynamicSharedMemorySize, X::SMEM); });
     if (e != cudaSuccess) return fail((int)e, "%s: shared memory %d: %s", name, X::SMEM, cudaGetErrorString(e));
-    const int wave = min(sm_count() * X::CTAS * A4_WAVES, A4_MAX_CTAS);
+    const int wave = min(sm_count() * X::CTAS, A4_MAX_CTAS);
     launch_kernel(attn4_kernel<NB, NG>, dim3((unsigned)min(max_units, (long)wave)), dim3(A4_THREADS), X::SMEM, st, A);
     return launch_status(name);
 }

@@ -362,9 +362,10 @@ static int kv4_append_launch(const char *name, const T *nk, const T *nv, const K
     B200K_REQUIRE(nk && nv && first, B200K_E_NULL, "%s: NULL pointer", name);
     int rc = kv4_check(name, C, batch, paged);
     if (rc) return rc;
-    B200K_REQUIRE(tokens >= 0 && (long)tokens * C.heads < (1l << 30) && stride_kt >= C.heads * C.d && stride_vt >= C.heads * C.d, B200K_E_SHAPE,
-                  "%s: tokens %d (tokens * heads below 2^30), strides %d and %d (at least heads * head_dim = %d)", name, tokens, stride_kt, stride_vt,
-                  C.heads * C.d);
+    B200K_REQUIRE(tokens >= 0 && (long)tokens * C.heads < (1l << 30) && stride_kt >= (long)C.heads * C.d && stride_vt >= (long)C.heads * C.d,
+                  B200K_E_SHAPE,
+                  "%s: tokens %d (tokens * heads below 2^30), strides %d and %d (at least heads * head_dim = %ld)", name, tokens, stride_kt, stride_vt,
+                  (long)C.heads * C.d);
     B200K_REQUIRE(aligned16(nk) && aligned16(nv) && stride_kt % 8 == 0 && stride_vt % 8 == 0, B200K_E_ALIGN,
                   "%s: new_keys and new_values must be 16-byte aligned, their token strides multiples of 8", name);
     if (batch == 0 || tokens == 0) return 0;
