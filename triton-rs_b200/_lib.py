@@ -12,6 +12,12 @@ import ctypes
 import re
 from pathlib import Path
 
+try:
+    from .fastcall import load as load_calls, types_of
+except ImportError:      # loaded by path, without its package (build.py reads the prototypes)
+    def load_calls():
+        return None
+
 HERE = Path(__file__).resolve().parent
 HEADER = HERE.parent / "include" / "b200_kernels.h"
 LIB_PATH = HERE / "libb200_kernels.so"
@@ -75,6 +81,7 @@ class Library:
         self.protos = parse_header()
         self._fns = {}
         self._callers = {}
+        self._compiled = load_calls()
         missing = []
         for name, (ret, args) in self.protos.items():
             try:
@@ -101,6 +108,16 @@ class Library:
         fn = self._callers.get(name)
         if fn is None:
             ret, proto = self.protos[name]
+
+            def fail(rc):
+                raise B200KError(name, rc, self.last_error())
+            status = ret == "int" and name not in _NOT_STATUS
+            if self._compiled is not None and ret in ("int", "size_t"):
+                fn = self._compiled.caller(name, types_of(proto), ctypes.cast(self._fns[name], ctypes.c_void_p).value, tensor_type,
+                                           lambda at, a: self._pointer(name, proto[at][1], a), self._stream, fail if status else None)
+                if fn is not None:
+                    self._callers[name] = fn
+                    return fn
             conv = []
             for ty, an in proto:
                 if ty == "ptr":
@@ -111,11 +128,8 @@ class Library:
                     conv.append(f"{an} if {an}.__class__ is float else float({an})")
                 else:
                     conv.append(f"{an} if {an}.__class__ is int else int({an})")
-            check = "    if rc: E(rc)\n" if ret == "int" and name not in _NOT_STATUS else ""
+            check = "    if rc: E(rc)\n" if status else ""
             src = f"def caller({', '.join(an for _, an in proto)}):\n    rc = F({', '.join(conv)})\n{check}    return rc\n"
-
-            def fail(rc):
-                raise B200KError(name, rc, self.last_error())
             space = {"T": tensor_type, "F": self._fns[name], "P": lambda a, an: self._pointer(name, an, a), "S": self._stream, "E": fail}
             exec(compile(src, f"<{name}>", "exec"), space)
             fn = self._callers[name] = space["caller"]

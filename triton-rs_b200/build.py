@@ -29,8 +29,19 @@ def _stale() -> bool:
     if not LIB.exists():
         return True
     t = LIB.stat().st_mtime
-    deps = list(CSRC.glob("*.cu")) + list(CSRC.glob("*.cuh")) + [HERE.parent / "include" / "b200_kernels.h", Path(__file__)]
+    deps = list(CSRC.glob("*.cu")) + list(CSRC.glob("*.cuh")) + [HERE.parent / "include" / "b200_kernels.h", Path(__file__), HERE / "fastcall.py"]
     return any(d.stat().st_mtime > t for d in deps)
+
+
+def _build_calls(obj_dir):
+    """The compiled argument conversion of the Python mirror (optional: without it the mirror converts in Python)."""
+    import importlib.util
+    mods = []
+    for name in ("_lib", "fastcall"):
+        spec = importlib.util.spec_from_file_location(f"b200k_{name}", HERE / f"{name}.py")
+        mods.append(importlib.util.module_from_spec(spec))
+        spec.loader.exec_module(mods[-1])
+    mods[1].build(mods[0].parse_header(), obj_dir)
 
 
 def build(force: bool = False, verbose: bool = False) -> Path:
@@ -56,6 +67,7 @@ def build(force: bool = False, verbose: bool = False) -> Path:
         failed |= p.returncode != 0
     if failed:
         raise RuntimeError("nvcc failed")
+    _build_calls(obj_dir)
     link = [nvcc, "-shared", "-o", str(LIB), *map(str, objs), "-lcudart"]
     subprocess.run(link, check=True)
     return LIB
