@@ -106,6 +106,13 @@ def test_refusals(pkg, call, kw, code):
     assert e.value.code == code, e.value.message
 
 
+def test_head_counts_whose_sum_passes_32_bits(pkg):
+    for hq, heads in ((2 ** 31 - 1, 2 ** 30), (2 ** 31 - 1, 2 ** 30 + 8), (2 ** 30, 8), (32, 2 ** 31 - 1)):
+        with pytest.raises(pkg.B200KError) as e:
+            _rope(pkg.lib(), hq=hq, heads=heads)
+        assert e.value.code == SHAPE
+
+
 def test_layer_cache_refusals(pkg):
     L = pkg.lib()
     for args, code in ([(None, PTR, PTR, PTR, PTR, 64), NULL], [(PTR, None, PTR, PTR, PTR, 64), NULL], [(PTR, PTR, PTR, PTR, None, 64), NULL],

@@ -13,10 +13,15 @@ template <typename T> struct Kv4Pair;
 template <> struct Kv4Pair<__half> {
     using type = __half2;
     __device__ static float2 wide(uint32_t w) { return h2_to_f2(w); }
+    __device__ static uint32_t pack(float a, float b) { return f2_to_h2(a, b); }
 };
 template <> struct Kv4Pair<__nv_bfloat16> {
     using type = __nv_bfloat162;
     __device__ static float2 wide(uint32_t w) { return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)); }
+    __device__ static uint32_t pack(float a, float b) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+        return *reinterpret_cast<const uint32_t *>(&h);
+    }
 };
 // minimum and maximum of both halves; a NaN stays
 template <typename T> __device__ __forceinline__ uint32_t pair_min(uint32_t a, uint32_t b) {
@@ -44,8 +49,7 @@ __device__ __forceinline__ float kv4_quotient(float a, float b, float y) {
 // three shuffles, over the eight threads, all of which call this; `row` < 0 stores nothing.
 // A quotient on the border of two codes is common in 16-bit data and has to go to the even code, which a product with the
 // reciprocal can miss; see kv4_quotient.  A sum with 1.5 * 2^23 then rounds it.  6 instructions an element where the compiler's
-// division, good for all operands, takes some 20: with it the append was bound by the issue of instructions (8192 tokens of
-// 8 heads: 65 us, 6.5 us being the floor).  Groups that need a clamp somewhere take the division.
+// division, good for all operands, takes some 20.  Groups that need a clamp somewhere take the division.
 template <typename T>
 __device__ __noinline__ uint32_t kv4_codes_clamped(uint32_t x0, uint32_t x1, float base, float scale) {
     const float2 a = Kv4Pair<T>::wide(x0), c = Kv4Pair<T>::wide(x1);
@@ -147,6 +151,10 @@ __device__ __forceinline__ void kv4_load_row(uint32_t (&x)[2 * NB], const T *row
 
 // New rows [batch, tokens, heads, D] (token pitch stride_t elements) -> cache rows first[b] + t.  Eight threads a row of K and the
 // same row of V, rows of a sequence (blockIdx.y) numbered (t, h).
+// One sequence, 8192 tokens of 8 heads, D 128, bf16, groups of 128: 11.9 us, 6.6 us being the bytes at copy bandwidth; the schedulers
+// issue in 72 of 100 cycles (some 7 instructions for each element of a thread's 16), so it is the quantisation that bounds it.
+// With K and V in threads of their own, which search for their place twice, 16.4 us.  One token each of 64 sequences: 2.2 us,
+// the time of a launch.
 template <typename T, int NB, int BPG>
 __global__ void __launch_bounds__(128)
 kv4_append_kernel(const T *__restrict__ nk, const T *__restrict__ nv, Kv4Cache C, const int32_t *__restrict__ first,
@@ -192,6 +200,7 @@ kv4_append_kernel(const T *__restrict__ nk, const T *__restrict__ nv, Kv4Cache C
 // the key that is quantised does not depend on which of them a compiler contracts, and the key is rounded to its type
 // first, as in the unfused sequence.  Eight threads a head; the other half of a pair is the same thread's where the
 // number of blocks is even, and loaded again (from L1) where it is odd.
+// 64 sequences of 32 + 2 x 8 heads: 2.0 us, 512 sequences 4.7 us: launch and three dependent loads (position, table row, qkv) bound it.
 template <typename T, int NB, int BPG>
 __global__ void __launch_bounds__(128)
 kv4_rope_append_kernel(const T *__restrict__ qkv, const float *__restrict__ cos_t, const float *__restrict__ sin_t,
@@ -251,7 +260,7 @@ kv4_rope_append_kernel(const T *__restrict__ qkv, const float *__restrict__ cos_
                 const float2 f = Kv4Pair<T>::wide(x[2 * j + e]), o = Kv4Pair<T>::wide(other[2 * j + e]);
                 const float a0 = __fmul_rn(f.x, c[2 * e]), z0 = __fmul_rn(o.x, s[2 * e]);
                 const float a1 = __fmul_rn(f.y, c[2 * e + 1]), z1 = __fmul_rn(o.y, s[2 * e + 1]);
-                out[2 * j + e] = Kv4Elem<T>::pack(upper ? __fadd_rn(a0, z0) : __fsub_rn(a0, z0), upper ? __fadd_rn(a1, z1) : __fsub_rn(a1, z1));
+                out[2 * j + e] = Kv4Pair<T>::pack(upper ? __fadd_rn(a0, z0) : __fsub_rn(a0, z0), upper ? __fadd_rn(a1, z1) : __fsub_rn(a1, z1));
             }
         }
 #pragma unroll
@@ -270,6 +279,8 @@ kv4_rope_append_kernel(const T *__restrict__ qkv, const float *__restrict__ cos_
 // Rows first[b] + i of the cache, i < out_len and below context_lens[b] -> out [batch, heads, out_len, D]; rows behind
 // them are left as they were.  Four threads a row of K or V: a thread's quarter of the codes (NB words) holds eight
 // neighbouring dims of every block, 16 bytes of the output.
+// 4 sequences of 8192 positions, 8 heads, D 128, fp16: 29 us, 0.9 of the copy bandwidth, which bounds it; a few hundred rows a sequence
+// (paged, 16 sequences): 7 to 8 us against 4 us of bytes, the start of the launch and the way through table, codes and parameters.
 template <typename T, int NB, int BPG>
 __global__ void __launch_bounds__(256)
 kv4_read_kernel(Kv4Cache C, const int32_t *__restrict__ first, const int32_t *__restrict__ lens, T *__restrict__ k_out, T *__restrict__ v_out,
@@ -331,8 +342,8 @@ kv4_read_kernel(Kv4Cache C, const int32_t *__restrict__ first, const int32_t *__
                 f[n] = fmaf(c.x, p.x, p.y);
                 f[n + 4] = fmaf(c.y, p.x, p.y);
             }
-            *reinterpret_cast<uint4 *>(to + 32 * j) = make_uint4(Kv4Elem<T>::pack(f[0], f[1]), Kv4Elem<T>::pack(f[2], f[3]), Kv4Elem<T>::pack(f[4], f[5]),
-                                                                 Kv4Elem<T>::pack(f[6], f[7]));
+            *reinterpret_cast<uint4 *>(to + 32 * j) = make_uint4(Kv4Pair<T>::pack(f[0], f[1]), Kv4Pair<T>::pack(f[2], f[3]), Kv4Pair<T>::pack(f[4], f[5]),
+                                                                 Kv4Pair<T>::pack(f[6], f[7]));
         }
     }
 }
@@ -385,7 +396,7 @@ static int kv4_rope_append_launch(const char *name, const T *qkv, const float *c
     B200K_REQUIRE(qkv && cos_t && sin_t && positions && q_out, B200K_E_NULL, "%s: NULL pointer", name);
     int rc = kv4_check(name, C, batch, false);
     if (rc) return rc;
-    B200K_REQUIRE(hq > 0, B200K_E_SHAPE, "%s: num_q_heads %d", name, hq);
+    B200K_REQUIRE(hq > 0 && hq + 2l * C.heads < (1l << 30), B200K_E_SHAPE, "%s: num_q_heads %d, num_kv_heads %d", name, hq, C.heads);
     B200K_REQUIRE(aligned16(qkv) && aligned16(q_out), B200K_E_ALIGN, "%s: qkv and q_out must be 16-byte aligned", name);
     if (batch == 0) return 0;
     int *status = status_word();

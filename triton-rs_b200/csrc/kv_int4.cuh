@@ -74,28 +74,4 @@ static inline Kv4Cache kv4_pool(const int32_t *kc, const b200k_half *kp, const i
     return C;
 }
 
-// 16-bit element types of activations: four elements of a unit <-> fp32
-template <typename T> struct Kv4Elem;
-template <> struct Kv4Elem<__half> {
-    __device__ static void load(const __half *p, float (&f)[4]) {
-        const uint2 u = *reinterpret_cast<const uint2 *>(p);
-        const float2 a = h2_to_f2(u.x), b = h2_to_f2(u.y);
-        f[0] = a.x; f[1] = a.y; f[2] = b.x; f[3] = b.y;
-    }
-    __device__ static uint32_t pack(float a, float b) { return f2_to_h2(a, b); }
-    __device__ static float round(float v) { return __half2float(__float2half_rn(v)); }
-};
-template <> struct Kv4Elem<__nv_bfloat16> {
-    __device__ static void load(const __nv_bfloat16 *p, float (&f)[4]) {
-        const uint2 u = *reinterpret_cast<const uint2 *>(p);
-        f[0] = __uint_as_float(u.x << 16); f[1] = __uint_as_float(u.x & 0xFFFF0000u);
-        f[2] = __uint_as_float(u.y << 16); f[3] = __uint_as_float(u.y & 0xFFFF0000u);
-    }
-    __device__ static uint32_t pack(float a, float b) {
-        const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
-        return *reinterpret_cast<const uint32_t *>(&h);
-    }
-    __device__ static float round(float v) { return __bfloat162float(__float2bfloat16_rn(v)); }
-};
-
 }  // namespace b200k
