@@ -20,8 +20,9 @@
 //
 // Work is dealt out on the device, from the lengths, so a captured graph follows them; see the kernel's first part.  Each warp
 // streams two 16-position tiles a stage through a ring of cp.async stages of its own, without a barrier between warps: four
-// warps a CTA, four CTAs an SM at head_dim 128 keep 74 KB under way.  (Three stages instead of two: 92 instead of 64 us, the
-// shared memory then leaves no room for the fourth CTA.  One tile a stage: 66 us.)  Rows behind the context are not read.
+// warps a CTA, four CTAs an SM at head_dim 128 keep 74 KB under way.  (Where two stages of two tiles took 64 us, before the sums
+// were centred, three stages took 92: the shared memory then leaves no room for the fourth CTA; one tile a stage 68.)  Rows
+// behind the context are not read.
 #include "kv_int4.cuh"
 #include "tma.cuh"
 

@@ -151,7 +151,7 @@ __device__ __forceinline__ void kv4_load_row(uint32_t (&x)[2 * NB], const T *row
 
 // New rows [batch, tokens, heads, D] (token pitch stride_t elements) -> cache rows first[b] + t.  Eight threads a row of K and the
 // same row of V, rows of a sequence (blockIdx.y) numbered (t, h).
-// One sequence, 8192 tokens of 8 heads, D 128, bf16, groups of 128: 11.9 us, 6.6 us being the bytes at copy bandwidth; the schedulers
+// One sequence, 8192 tokens of 8 heads, D 128, bf16, groups of 128: 11.9 us, 6.5 us being the bytes at copy bandwidth; the schedulers
 // issue in 72 of 100 cycles (some 7 instructions for each element of a thread's 16), so it is the quantisation that bounds it.
 // With K and V in threads of their own, which search for their place twice, 16.4 us.  One token each of 64 sequences: 2.2 us,
 // the time of a launch.
