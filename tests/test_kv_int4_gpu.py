@@ -266,6 +266,37 @@ def test_read_back(P, pkg, oracle, dtype, heads, d, g, block):
                     assert (np.abs(got[:, :n] - ref) <= half_step(dtype, ref)).all()
 
 
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("heads,d,g,block", [(8, 128, 64, 0), (8, 128, 32, 16), (2, 96, 32, 7), (1, 64, 64, 0), (3, 32, 32, 4), (4, 256, 128, 64),
+                                             (1, 224, 32, 0)])
+def test_read_back_of_many_rows(P, pkg, oracle, dtype, heads, d, g, block):
+    """K and V by the same threads: rows of a large call against those of small ones, and a sample against the oracle."""
+    b, rng = 4, np.random.default_rng(heads + d)
+    n = 40000 // (b * heads) + 3                     # 8 b n heads threads are more than the machine holds at once
+    c = big_cache(oracle, b, heads, d, g, n, 7, block)
+    lens = t(np.array([n, n // 2 + 1, 0, 17], np.int32))
+    part = n // 4 + 1
+
+    def read(first, out_len):
+        ko = torch.full((b, heads, out_len, d), 9.0, dtype=TYPES[dtype], device=DEV)
+        vo = ko.clone()
+        c.read(P, dtype, t(np.full(b, first, np.int32)), lens, ko, vo)
+        return ko, vo
+    status(pkg)
+    whole = read(0, n)
+    parts = [read(f, part) for f in range(0, n, part)]
+    assert status(pkg) == 0
+    for i, o in enumerate(whole):
+        assert torch.equal(o.view(torch.int16), torch.cat([x[i] for x in parts], 2)[:, :, :n].contiguous().view(torch.int16))
+        for s, m in enumerate(lens.tolist()):
+            assert (o[s, :, m:] == 9).all()
+            w, p = c.words[i].cpu().numpy(), c.params[i].cpu().numpy()
+            for pos in rng.integers(0, m, 20 if m else 0):
+                at = c.where(s, int(pos))
+                ref = oracle.kv4_values(w[at], p[at])
+                assert (np.abs(as64(o[s, :, pos]) - ref) <= half_step(dtype, ref)).all()
+
+
 def test_read_lengths_and_starts_outside_are_reported(P, pkg, oracle):
     c = Cache(3, 1, 64, 64, 10)
     x = as64(values((3, 1, 10, 64), "f16", 1))

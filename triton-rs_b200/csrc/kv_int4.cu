@@ -43,13 +43,34 @@ __device__ __forceinline__ float kv4_quotient(float a, float b, float y) {
     return fmaf(fmaf(-q, b, a), y, q);
 }
 
+// two fp32 numbers in a register pair, each operation one instruction for both
+struct Kv4Two {
+    unsigned long long v;
+    __device__ Kv4Two(unsigned long long v) : v(v) {}
+    __device__ Kv4Two(float a, float b) { asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b)); }
+    __device__ explicit Kv4Two(float2 a) : Kv4Two(a.x, a.y) {}
+    __device__ friend Kv4Two operator+(Kv4Two a, Kv4Two b) { asm("add.rn.f32x2 %0, %1, %2;" : "=l"(a.v) : "l"(a.v), "l"(b.v)); return a; }
+    __device__ friend Kv4Two operator*(Kv4Two a, Kv4Two b) { asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(a.v) : "l"(a.v), "l"(b.v)); return a; }
+    __device__ uint32_t low() const { return (uint32_t)v; }
+    __device__ uint32_t high() const { return (uint32_t)(v >> 32); }
+};
+__device__ __forceinline__ Kv4Two kv4_fma(Kv4Two a, Kv4Two b, Kv4Two c) {
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(a.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+    return a;
+}
+// the same quotients of two numbers: `minus_b` holds -b
+__device__ __forceinline__ Kv4Two kv4_quotient(Kv4Two a, Kv4Two minus_b, Kv4Two y) {
+    const Kv4Two q = a * y;
+    return kv4_fma(kv4_fma(q, minus_b, a), y, q);
+}
+
 // ---- one row by eight neighbouring threads ----------------------------------------------------------------------------
 // Thread r has the units (j, r) of all NB 32-dim blocks j: dims 32 j + 4 r .. + 3, x[2 j] and x[2 j + 1] in pairs.  Its codes
 // are 2 NB neighbouring bytes of the stored row.  The range of a group is the minimum of (x, -x) over its blocks and, by
 // three shuffles, over the eight threads, all of which call this; `row` < 0 stores nothing.
 // A quotient on the border of two codes is common in 16-bit data and has to go to the even code, which a product with the
-// reciprocal can miss; see kv4_quotient.  A sum with 1.5 * 2^23 then rounds it.  6 instructions an element where the compiler's
-// division, good for all operands, takes some 20.  Groups that need a clamp somewhere take the division.
+// reciprocal can miss; see kv4_quotient.  A sum with 1.5 * 2^23 then rounds it.  5 instructions for two elements where the
+// compiler's division, good for all operands, takes some 20 for each.  Groups that need a clamp somewhere take the division.
 template <typename T>
 __device__ __noinline__ uint32_t kv4_codes_clamped(uint32_t x0, uint32_t x1, float base, float scale) {
     const float2 a = Kv4Pair<T>::wide(x0), c = Kv4Pair<T>::wide(x1);
@@ -83,10 +104,11 @@ __device__ __forceinline__ void kv4_store_row(const uint32_t (&x)[2 * NB], long 
                 upper[j] = pair_max<T>(upper[j], upper[j + step]);
             }
     uint32_t bits[NB];
-    float base = 0.f, scale = 0.f, inv = 0.f;
-    bool plain = true;                       // BPG blocks are a group
+    float bases[NB / BPG], scales[NB / BPG], inv = 0.f;      // BPG blocks are a group
+    unsigned clamped = 0;                    // groups
 #pragma unroll
     for (int j = 0; j < NB; ++j) {
+        float &base = bases[j / BPG], &scale = scales[j / BPG];
         if (j % BPG == 0) {                  // a new group
             // (minimum, -maximum) in one register
             uint32_t lo = pair_min<T>(range[j], range[j] >> 16 | range[j] << 16);
@@ -104,24 +126,24 @@ __device__ __forceinline__ void kv4_store_row(const uint32_t (&x)[2 * NB], long 
             const __half scale_h = __float2half_rn(kv4_quotient(most - base, 15.f, 1.f / 15.f));
             scale = __half2float(scale_h);
             // nothing to clamp: values inside the limits, and a scale that is rounded by 2^-11 at most
-            plain = least == f.x && most == -f.y && scale >= 1.f / 8192.f;
+            clamped |= least == f.x && most == -f.y && scale >= 1.f / 8192.f ? 0u : 1u << (j / BPG);
             asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(scale));
             if (row >= 0 && r == j / BPG) reinterpret_cast<__half2 *>(params)[row * (NB / BPG) + j / BPG] = __halves2half2(scale_h, base_h);
         }
-        float f[4];
-        {
-            const float2 a = Kv4Pair<T>::wide(x[2 * j]), c = Kv4Pair<T>::wide(x[2 * j + 1]);
-            f[0] = a.x; f[1] = a.y; f[2] = c.x; f[3] = c.y;
-        }
         uint32_t code = 0;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float c = kv4_quotient(f[i] - base, scale, inv) + MAGIC;
-            code += __float_as_uint(c) * (1u << (4 * i));      // the low bits of MAGIC are 0: only the nibble reaches the low 16 bits
+        for (int i = 0; i < 2; ++i) {
+            const Kv4Two a = Kv4Two(Kv4Pair<T>::wide(x[2 * j + i])) + Kv4Two(-base, -base);
+            const Kv4Two c = kv4_quotient(a, Kv4Two(-scale, -scale), Kv4Two(inv, inv)) + Kv4Two(MAGIC, MAGIC);
+            // the low bits of MAGIC are 0: only the nibble reaches the low 16 bits
+            code += c.low() * (1u << (8 * i)) + c.high() * (16u << (8 * i));
         }
-        if (!plain) code = kv4_codes_clamped<T>(x[2 * j], x[2 * j + 1], base, scale);
         bits[j] = code;
     }
+    if (clamped)
+#pragma unroll
+        for (int j = 0; j < NB; ++j)
+            if (clamped >> (j / BPG) & 1) bits[j] = kv4_codes_clamped<T>(x[2 * j], x[2 * j + 1], bases[j / BPG], scales[j / BPG]);
     if (row < 0) return;
     unsigned char *to = reinterpret_cast<unsigned char *>(codes) + row * (16 * NB) + r * (2 * NB);
     if constexpr (NB % 2) {
@@ -151,10 +173,10 @@ __device__ __forceinline__ void kv4_load_row(uint32_t (&x)[2 * NB], const T *row
 
 // New rows [batch, tokens, heads, D] (token pitch stride_t elements) -> cache rows first[b] + t.  Eight threads a row of K and the
 // same row of V, rows of a sequence (blockIdx.y) numbered (t, h).
-// One sequence, 8192 tokens of 8 heads, D 128, bf16, groups of 128: 11.9 us, 6.5 us being the bytes at copy bandwidth; the schedulers
-// issue in 72 of 100 cycles (some 7 instructions for each element of a thread's 16), so it is the quantisation that bounds it.
-// With K and V in threads of their own, which search for their place twice, 16.4 us.  One token each of 64 sequences: 2.2 us,
-// the time of a launch.
+// One sequence, 8192 tokens of 8 heads, D 128, bf16, groups of 128: 10.8 us, 6.5 us being the bytes at copy bandwidth; the issue of
+// instructions bounds it (each element's quantisation, and a third of them for places and ranges).  With K and V in threads of
+// their own, which search for their place twice, 16.4 us; with every operation of the quantisation on one number 11.9.  One token
+// each of 64 sequences: 2.1 us, the time of a launch.
 template <typename T, int NB, int BPG>
 __global__ void __launch_bounds__(128)
 kv4_append_kernel(const T *__restrict__ nk, const T *__restrict__ nv, Kv4Cache C, const int32_t *__restrict__ first,
@@ -200,7 +222,7 @@ kv4_append_kernel(const T *__restrict__ nk, const T *__restrict__ nv, Kv4Cache C
 // the key that is quantised does not depend on which of them a compiler contracts, and the key is rounded to its type
 // first, as in the unfused sequence.  Eight threads a head; the other half of a pair is the same thread's where the
 // number of blocks is even, and loaded again (from L1) where it is odd.
-// 64 sequences of 32 + 2 x 8 heads: 2.0 us, 512 sequences 4.7 us: launch and three dependent loads (position, table row, qkv) bound it.
+// 64 sequences of 32 + 2 x 8 heads: 2.0 us, 512 sequences 4.4 us: launch and three dependent loads (position, table row, qkv) bound it.
 template <typename T, int NB, int BPG>
 __global__ void __launch_bounds__(128)
 kv4_rope_append_kernel(const T *__restrict__ qkv, const float *__restrict__ cos_t, const float *__restrict__ sin_t,
@@ -277,15 +299,17 @@ kv4_rope_append_kernel(const T *__restrict__ qkv, const float *__restrict__ cos_
 }
 
 // Rows first[b] + i of the cache, i < out_len and below context_lens[b] -> out [batch, heads, out_len, D]; rows behind
-// them are left as they were.  Four threads a row of K or V: a thread's quarter of the codes (NB words) holds eight
-// neighbouring dims of every block, 16 bytes of the output.
-// 4 sequences of 8192 positions, 8 heads, D 128, fp16: 29 us, 0.9 of the copy bandwidth, which bounds it; a few hundred rows a sequence
-// (paged, 16 sequences): 7 to 8 us against 4 us of bytes, the start of the launch and the way through table, codes and parameters.
-template <typename T, int NB, int BPG>
+// them are left as they were.  Four threads a row: a thread's quarter of the codes (NB words) holds eight neighbouring dims of
+// every block, 16 bytes of the output.  BOTH: of K and of V in turn, so that a place is looked up once and twice the bytes are under
+// way; in a small launch K and V have threads of their own (kv4_read_launch).
+// 4 sequences of 8192 positions, 8 heads, D 128, fp16: 29 us, 0.9 of the copy bandwidth, which bounds it; one of them 8.2 us (9.2
+// not BOTH), 6.5 us being the bytes; a few hundred rows a sequence (paged, 16 sequences) 7.5 us (8.1) against 4 us of bytes, the
+// start of the launch and the way through table, codes and parameters.
+template <typename T, int NB, int BPG, bool BOTH>
 __global__ void __launch_bounds__(256)
 kv4_read_kernel(Kv4Cache C, const int32_t *__restrict__ first, const int32_t *__restrict__ lens, T *__restrict__ k_out, T *__restrict__ v_out,
                 int out_len, int *status) {
-    constexpr int D = 32 * NB;
+    constexpr int D = 32 * NB, TENSORS = BOTH ? 2 : 1;
     pdl_wait();
     pdl_launch_dependents();
     const int b = blockIdx.y, t = threadIdx.x & 3;
@@ -295,13 +319,14 @@ kv4_read_kernel(Kv4Cache C, const int32_t *__restrict__ first, const int32_t *__
         if (blockIdx.x == 0 && threadIdx.x == 0) atomicOr(status, KV4_BAD_POSITION);
     }
     const long start = first ? (long)first[b] : 0l;
-    const unsigned rows = (unsigned)max(min((long)out_len, len - start), 0l);     // of a head, times K and V, times heads:
-    const long total = 2l * rows * C.heads;
-    for (long i2 = ((long)blockIdx.x * blockDim.x + threadIdx.x) >> 2; i2 < total; i2 += gridDim.x * blockDim.x >> 2) {
-        const bool is_v = i2 & 1;
+    const unsigned rows = (unsigned)max(min((long)out_len, len - start), 0l);     // of a head
+    const long total = (long)rows * C.heads * (2 / TENSORS);
+    for (long n = ((long)blockIdx.x * blockDim.x + threadIdx.x) >> 2; n < total; n += gridDim.x * blockDim.x >> 2) {
+        const bool is_v = !BOTH && n & 1;
+        const long hi = BOTH ? n : n >> 1;
         // (head, row) of a number below 2^32 by a 32-bit division, beyond that by a 64-bit one
-        const int h = total >> 33 ? (int)((i2 >> 1) / rows) : (int)((unsigned)(i2 >> 1) / rows);
-        const unsigned i = (unsigned)((i2 >> 1) - (long)h * rows);
+        const int h = total >> 32 ? (int)(hi / rows) : (int)((unsigned)hi / rows);
+        const unsigned i = (unsigned)(hi - (long)h * rows);
         const long pos = start + i;
         if (pos < 0) {
             if (t == 0) atomicOr(status, KV4_BAD_POSITION);
@@ -312,38 +337,48 @@ kv4_read_kernel(Kv4Cache C, const int32_t *__restrict__ first, const int32_t *__
             if (t == 0) atomicOr(status, KV4_BAD_BLOCK);
             continue;
         }
-        uint32_t w[NB];
-        const uint32_t *from = reinterpret_cast<const uint32_t *>(is_v ? C.v_codes : C.k_codes) + row * (4 * NB) + t * NB;
-        if constexpr (NB % 4 == 0) {
+        uint32_t w[TENSORS][NB];
+        __half2 params[TENSORS][NB / BPG];
 #pragma unroll
-            for (int j = 0; j < NB; j += 4) {
-                const uint4 u = ldg_nc_v4(from + j);
-                w[j] = u.x; w[j + 1] = u.y; w[j + 2] = u.z; w[j + 3] = u.w;
+        for (int v = 0; v < TENSORS; ++v) {
+            const uint32_t *from = reinterpret_cast<const uint32_t *>(v || is_v ? C.v_codes : C.k_codes) + row * (4 * NB) + t * NB;
+            if constexpr (NB % 4 == 0) {
+#pragma unroll
+                for (int j = 0; j < NB; j += 4) {
+                    const uint4 u = ldg_nc_v4(from + j);
+                    w[v][j] = u.x; w[v][j + 1] = u.y; w[v][j + 2] = u.z; w[v][j + 3] = u.w;
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < NB; ++j) w[v][j] = from[j];
             }
-        } else {
+            const __half2 *at = reinterpret_cast<const __half2 *>(v || is_v ? C.v_params : C.k_params) + row * (NB / BPG);
 #pragma unroll
-            for (int j = 0; j < NB; ++j) w[j] = from[j];
+            for (int g = 0; g < NB / BPG; ++g) params[v][g] = at[g];
         }
-        const __half2 *params = reinterpret_cast<const __half2 *>(is_v ? C.v_params : C.k_params) + row * (NB / BPG);
-        T *to = (is_v ? v_out : k_out) + (((long)b * C.heads + h) * out_len + i) * D + 8 * t;
-        float2 p = make_float2(0.f, 0.f);
+        const long to_row = (((long)b * C.heads + h) * out_len + i) * D + 8 * t;
 #pragma unroll
-        for (int j = 0; j < NB; ++j) {
-            if (j % BPG == 0) {
-                p = __half22float2(params[j / BPG]);
-                p.x *= 16777216.f;           // the codes come as fp16 subnormals, c 2^-24: exact either way
-            }
-            // units (2 t, j) and (2 t + 1, j): dims 8 t .. + 3 in the low half, + 4 .. + 7 in the high one
-            const uint32_t u = __byte_perm(w[j >> 1], w[(NB + j) >> 1], (j & 1 ? 0x32 : 0x10) | ((NB + j & 1 ? 0x76 : 0x54) << 8));
-            float f[8];
+        for (int v = 0; v < TENSORS; ++v) {
+            T *to = (v || is_v ? v_out : k_out) + to_row;
+            float2 p = make_float2(0.f, 0.f);
 #pragma unroll
-            for (int n = 0; n < 4; ++n) {
-                const float2 c = h2_to_f2((u >> (4 * n)) & 0x000f000fu);
-                f[n] = fmaf(c.x, p.x, p.y);
-                f[n + 4] = fmaf(c.y, p.x, p.y);
+            for (int j = 0; j < NB; ++j) {
+                if (j % BPG == 0) {
+                    p = __half22float2(params[v][j / BPG]);
+                    p.x *= 16777216.f;       // the codes come as fp16 subnormals, c 2^-24: exact either way
+                }
+                // units (2 t, j) and (2 t + 1, j): dims 8 t .. + 3 in the low half, + 4 .. + 7 in the high one
+                const uint32_t u = __byte_perm(w[v][j >> 1], w[v][(NB + j) >> 1], (j & 1 ? 0x32 : 0x10) | ((NB + j & 1 ? 0x76 : 0x54) << 8));
+                float f[8];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float2 c = h2_to_f2((u >> (4 * e)) & 0x000f000fu);
+                    f[e] = fmaf(c.x, p.x, p.y);
+                    f[e + 4] = fmaf(c.y, p.x, p.y);
+                }
+                *reinterpret_cast<uint4 *>(to + 32 * j) = make_uint4(Kv4Pair<T>::pack(f[0], f[1]), Kv4Pair<T>::pack(f[2], f[3]),
+                                                                     Kv4Pair<T>::pack(f[4], f[5]), Kv4Pair<T>::pack(f[6], f[7]));
             }
-            *reinterpret_cast<uint4 *>(to + 32 * j) = make_uint4(Kv4Pair<T>::pack(f[0], f[1]), Kv4Pair<T>::pack(f[2], f[3]), Kv4Pair<T>::pack(f[4], f[5]),
-                                                                 Kv4Pair<T>::pack(f[6], f[7]));
         }
     }
 }
@@ -421,10 +456,15 @@ static int kv4_read_launch(const char *name, const Kv4Cache &C, bool paged, cons
     if (batch == 0 || out_len == 0) return 0;
     int *status = status_word();
     if (!status) return B200K_E_WORKSPACE;
-    const int threads = 8l * out_len * C.heads <= 128 ? 64 : 256;       // a few rows a sequence: small blocks
-    const dim3 grid(kv4_grid(2l * out_len * C.heads, threads / 4, batch), batch);
+    // K and V in threads of their own while these fit the machine at once (2048 an SM): latency counts then.  64 sequences of one
+    // position of 8 heads 2.3 us (2.9 with both in a thread), 512 of four 3.4 (3.8); beyond that 8 of 1000 positions 6.7 us (6.0).
+    const bool apart = 8.0 * batch * out_len * C.heads <= 2048.0 * sm_count();
+    const long rows = (apart ? 2l : 1l) * out_len * C.heads;
+    const int threads = 4 * rows <= 128 ? 64 : 256;             // a few rows a sequence: small blocks
+    const dim3 grid(kv4_grid(rows, threads / 4, batch), batch);
     kv4_by_shape(C.d, C.g, [&](auto nb, auto bpg) {
-        launch_kernel(kv4_read_kernel<T, nb(), bpg()>, grid, dim3(threads), 0, to_stream(stream), C, first, lens, k_out, v_out, out_len, status);
+        launch_kernel(apart ? kv4_read_kernel<T, nb(), bpg(), false> : kv4_read_kernel<T, nb(), bpg(), true>, grid, dim3(threads), 0, to_stream(stream),
+                      C, first, lens, k_out, v_out, out_len, status);
     });
     return launch_status(name);
 }
