@@ -456,6 +456,46 @@ def test_attention_nan_stays_with_its_head(P, oracle):
     assert torch.isnan(out[0, 4:]).all() and torch.isfinite(out[0, :4]).all() and torch.isfinite(out[1]).all()
 
 
+@pytest.mark.parametrize("d,g", [(128, 32), (256, 64)])
+@pytest.mark.parametrize("kspread,vspread,kmean,vmean,scale", [
+    (1.0, 1.0, 0.0, 0.0, 0.09), (1.0, 1e-4, 0.0, 0.0, 0.09), (30.0, 1000.0, 0.0, 0.0, 0.02), (1.0, 1.0, 50.0, -100.0, 0.09), (1.0, 8000.0, 0.0, 20000.0, 0.09),
+    (1.0, 0.0, 0.0, 3.0, 0.09), (0.0, 1.0, 2.0, 0.0, 1.0), (1.0, 1.0, 0.0, 0.0, -0.1), (1.0, 1.0, 0.0, 0.0, 0.0)])
+def test_attention_with_four_groups(P, oracle, d, g, kspread, vspread, kmean, vmean, scale):
+    """Their bases go through matrix instructions: far off-centre, tiny, huge and constant keys and values."""
+    b, hq, hkv, n = 3, 10, 2, 420
+    lens = [n, n - 7, 5]
+    c = Cache(b, hkv, d, g, n)
+    k = as64((values((b, hkv, n, d), "f16", 31, kspread).float() + kmean).half())
+    v = as64((values((b, hkv, n, d), "f16", 32, vspread).float() + vmean).clamp(-60000, 60000).half())
+    c.fill(k, v, lens, oracle)
+    q = values((b, hq, d), "f16", 33)
+    out = torch.empty((b, hq, d), dtype=torch.float16, device=DEV)
+    c.attend(P, "f16", q, t(np.array(lens, np.int32)), out, scale)
+    check_attention(oracle, c, q, lens, out, scale, "f16")
+
+
+@pytest.mark.parametrize("d,g", [(128, 32), (128, 64)])
+@pytest.mark.parametrize("vspread,vmean", [(1.0, 0.0), (8000.0, 20000.0), (1e-3, 5.0)])
+def test_one_position_over_many_small_ones(P, oracle, d, g, vspread, vmean):
+    """Probabilities 2^-16.6 of the largest, whose sum counts: none may vanish in 16 bits.  600 contexts, so that a warp has 512
+    positions of one; the value scales grow on the way."""
+    b, n = 600, 2000
+    c = Cache(b, 1, d, g, n)
+    gen = torch.Generator(device=DEV).manual_seed(5)
+    k = torch.zeros(b, n, 1, d, dtype=torch.float16, device=DEV)
+    k[:, 0, 0, :] = 11.5 / d
+    v = (torch.randn(b, n, 1, d, device=DEV, generator=gen) * vspread * torch.linspace(0.01, 1.0, n, device=DEV)[None, :, None, None] + vmean).half()
+    c.append(P, "f16", k, v, t(np.zeros(b, np.int32)), None, n)
+    q = torch.ones(b, 2, d, dtype=torch.float16, device=DEV)
+    out = torch.empty_like(q)
+    c.attend(P, "f16", q, t(np.full(b, n, np.int32)), out, 1.0)
+    for s in (0, 311, 599):
+        (kw, kp), (vw, vp) = c.rows(0, s, n), c.rows(1, s, n)
+        ref, mag, smag = oracle.kv4_decode_attention(as64(q[s]), kw, kp, vw, vp, 1.0)
+        bound = half_step("f16", ref) + (2.0 ** -11 + 2.0 ** -19 + 2 * 2.0 ** -20 * smag) * mag
+        assert (np.abs(as64(out[s]) - ref) <= bound).all()
+
+
 def big_cache(oracle, b, hkv, d, g, n, seed, block=0):
     """A long cache: random words and params straight on the device."""
     c = Cache(b, hkv, d, g, n, block, seed)

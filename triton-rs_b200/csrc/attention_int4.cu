@@ -16,7 +16,7 @@
 // 236 us, 0.91 of the copy bandwidth), and just below that the issue of instructions: about 250 a warp for 16 positions of K
 // and V, half of them on the integer pipe, at 0.6 a cycle and scheduler; HBM delivers 16 positions to an SM every 96 cycles.
 // At 64 x 4096 positions (46 us of bytes) 66 us: starting takes 4 us, the joins of the CTAs 4, and the rest is the issue
-// rate.  Groups of 32 take a third more instructions (83 us), groups of 128 a tenth fewer (57 us).
+// rate.  Groups of 32 take a fifth more instructions (78 us), groups of 128 a tenth fewer (57 us).
 //
 // Work is dealt out on the device, from the lengths, so a captured graph follows them; see the kernel's first part.  Each warp
 // streams two 16-position tiles a stage through a ring of cp.async stages of its own, without a barrier between warps: four
@@ -63,6 +63,10 @@ struct A4 {
     static constexpr int STAGE = A4_SUBS * SUB;
     static constexpr int MTILES = 2 * NB;
     static constexpr bool PURE = G == 32;                     // a group is one block: see kword()
+    // With four groups the bases go through matrix instructions as well (a row's params are the 16 bytes that these want): two of
+    // them, and 14 others, for 48 on scalars.  D 128, groups of 32, 64 x 4096: 78 us, 84 without; with two groups, where 16
+    // instructions replace 24, 65.9 and 66.6, which is not worth rounding the probabilities that meet the bases to fp16.
+    static constexpr bool BASES = NG == 4;
     static constexpr int PART = D * A4_HEADS + 16;            // floats of a partial result
     static constexpr int CTAS = NB <= 4 ? 4 : NB <= 5 ? 3 : 2;
     static constexpr int RING = A4_WARPS * A4_STAGES * STAGE;
@@ -115,6 +119,9 @@ __device__ __forceinline__ void a4_lds(uint32_t *w, uint32_t at) {    // N words
 #pragma unroll
         for (int i = 0; i < N; ++i) asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w[i]) : "r"(at + 4 * i) : "memory");
     }
+}
+__device__ __forceinline__ void a4_ldm_trans(uint32_t &a, uint32_t &b, uint32_t at) {     // two 8 x 8 matrices of halves, transposed
+    asm volatile("ldmatrix.sync.aligned.m8n8.x2.trans.shared.b16 {%0, %1}, [%2];" : "=r"(a), "=r"(b) : "r"(at) : "memory");
 }
 __device__ __forceinline__ uint32_t a4_lds16(uint32_t at) {
     uint16_t h;
@@ -359,6 +366,9 @@ attn4_kernel(const __grid_constant__ Attn4Args A) {
     const uint32_t at_p = a4_keep(ring + 2 * A4_TILE * X::ROW + kpos * 2 * X::PROW);
     auto piece_at = [&](int pos) { return ring + (A4_TILE + pos) * X::ROW + (((2 * NB * r >> 4) ^ X::swizzle(pos)) << 4) + (2 * NB * r & 15); };
     const uint32_t at_v0 = a4_keep(piece_at(t)), at_v1 = a4_keep(piece_at(4 + (t ^ 1)));
+    // BASES: the params of V as a matrix [MMA index][scale, base of each group], and K's word of group t
+    const uint32_t at_b = X::BASES ? a4_keep(ring + 2 * A4_TILE * X::ROW + (2 * a4_pos(lane & 15) + 1) * X::PROW) : 0;
+    const uint32_t at_kz = X::BASES ? a4_keep(at_p + 4 * t) : 0;
 
     // ---- streaming a piece: tile i of this warp goes to stage i % STAGES ------------------------------------------------------------
     // 16 neighbouring rows are one linear part of the cache, so a tile that is whole and lies in one block takes nothing but
@@ -488,18 +498,33 @@ attn4_kernel(const __grid_constant__ Attn4Args A) {
             if (warp == 0 && t == 0) sm_fac[r] = r >= d.heads ? 0.f : big < INFINITY ? fabsf(A.scale_log2e) / fabsf(up) * 16777216.f : NAN;
         }
         __syncthreads();
-        float qsum[NG][2], fac[2];             // of heads 2t and 2t + 1
+        float qsum[NG][2];                     // of heads 2t and 2t + 1
+        const float fac[2] = {sm_fac[2 * t], sm_fac[2 * t + 1]};
+        uint32_t qz0 = 0, qz1 = 0;
+        if constexpr (X::BASES) {
+            // sum_g z_g (sum q) in one instruction: its k indices 2 t and 2 t + 1 meet (scale, base) of group t, so the operand has 0 and
+            // the sum of q there, as two fp16 numbers (22 bits; 2^10 larger, so that the second is no subnormal) one after the other
+            float sum = 0.f;
 #pragma unroll
-        for (int e2 = 0; e2 < 2; ++e2) {
-            fac[e2] = sm_fac[2 * t + e2];
+            for (int i = 0; i < NB; ++i)
+                if (a4_kgroup<NB, NG, X::PURE>(i) == t) sum += sm_qsum[i][r];
+            sum *= 1024.f;
+            const __half hi = __float2half_rn(sum), lo = __float2half_rn(sum - __half2float(hi));
+            qz0 = (uint32_t)__half_as_ushort(hi) << 16;
+            qz1 = (uint32_t)__half_as_ushort(lo) << 16;
+        } else {
 #pragma unroll
-            for (int g = 0; g < NG; ++g) qsum[g][e2] = 0.f;
+            for (int e2 = 0; e2 < 2; ++e2) {
 #pragma unroll
-            for (int i = 0; i < NB; ++i) qsum[a4_kgroup<NB, NG, X::PURE>(i)][e2] += sm_qsum[i][2 * t + e2];
+                for (int g = 0; g < NG; ++g) qsum[g][e2] = 0.f;
+#pragma unroll
+                for (int i = 0; i < NB; ++i) qsum[a4_kgroup<NB, NG, X::PURE>(i)][e2] += sm_qsum[i][2 * t + e2];
+            }
         }
 
         // sacc: the sum of w (below), group 2 i in the first two registers, 2 i + 1 in the others
-        float oacc[X::MTILES][4], sacc[(NG + 1) / 2][4], zacc[NG][2], l[2] = {0.f, 0.f};
+        // zacc: the sum of p (z + 7.5 s); BASES: in bacc that of lift p times scale (even r) or base (odd r) of group r / 2
+        float oacc[X::MTILES][4], sacc[(NG + 1) / 2][4], zacc[NG][2], bacc[2] = {0.f, 0.f}, lift = 0.f, l[2] = {0.f, 0.f};
 #pragma unroll
         for (int i = 0; i < X::MTILES; ++i)
 #pragma unroll
@@ -549,6 +574,15 @@ attn4_kernel(const __grid_constant__ Attn4Args A) {
                     a4_lds<NB>(w0, at_k + st);
                     a4_lds<NB>(w1, at_k + st + 8 * X::ROW);
                 }
+                if constexpr (X::BASES) {
+                    uint32_t z0, z1;
+                    float zq[4];
+                    a4_lds<1>(&z0, at_kz + st);
+                    a4_lds<1>(&z1, at_kz + st + 16 * X::PROW);
+                    a4_mma0(zq, z0, z1, z0, z1, qz0, qz1);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) s[i] = zq[i] * (1.f / 1024.f);
+                }
                 float s0[NG], z0[NG], s1[NG], z1[NG];
                 a4_params<NG>(s0, z0, pw0);
                 a4_params<NG>(s1, z1, pw1);
@@ -569,10 +603,16 @@ attn4_kernel(const __grid_constant__ Attn4Args A) {
                         begun = true;
                         a4_mma(acc, x2, y2, x3, y3, q4.z, q4.w);
                     }
-                    s[0] = fmaf(s0[g], acc[0], fmaf(z0[g], qsum[g][0], s[0]));
-                    s[1] = fmaf(s0[g], acc[1], fmaf(z0[g], qsum[g][1], s[1]));
-                    s[2] = fmaf(s1[g], acc[2], fmaf(z1[g], qsum[g][0], s[2]));
-                    s[3] = fmaf(s1[g], acc[3], fmaf(z1[g], qsum[g][1], s[3]));
+                    if constexpr (!X::BASES) {
+                        s[0] = fmaf(z0[g], qsum[g][0], s[0]);
+                        s[1] = fmaf(z0[g], qsum[g][1], s[1]);
+                        s[2] = fmaf(z1[g], qsum[g][0], s[2]);
+                        s[3] = fmaf(z1[g], qsum[g][1], s[3]);
+                    }
+                    s[0] = fmaf(s0[g], acc[0], s[0]);
+                    s[1] = fmaf(s0[g], acc[1], s[1]);
+                    s[2] = fmaf(s1[g], acc[2], s[2]);
+                    s[3] = fmaf(s1[g], acc[3], s[3]);
                 }
             }
             constexpr int VW = NB % 2 == 0 ? NB / 2 : 1;
@@ -608,6 +648,7 @@ attn4_kernel(const __grid_constant__ Attn4Args A) {
                     n1 = fmaxf(n1, __shfl_xor_sync(0xffffffffu, n1, o));
                     vmax = fmaxf(vmax, __shfl_xor_sync(0xffffffffu, vmax, o));
                 }
+                const float e_was = e;
                 if (vmax > most) {
                     // 2^e vmax in [2^2, 2^3): vmax is a positive fp16 number, so its exponent lies in -24 .. 15
                     const int ex = (int)(__float_as_uint(vmax) >> 23) - 127;
@@ -623,6 +664,12 @@ attn4_kernel(const __grid_constant__ Attn4Args A) {
                 ref[1] = r1;
                 l[0] *= a0;
                 l[1] *= a1;
+                if constexpr (X::BASES) {
+                    const float back = a4_exp2(e_was - e);
+                    bacc[0] *= a0 * back;
+                    bacc[1] *= a1 * back;
+                    lift = a4_exp2(9.f - e);
+                }
 #pragma unroll
                 for (int g = 0; g < NG; ++g) {
                     zacc[g][0] *= a0;
@@ -650,17 +697,29 @@ attn4_kernel(const __grid_constant__ Attn4Args A) {
             // other tile adds -w (15 - c) in place of w c: the codes are not centred, their sum would grow with the context, and
             // the tensor cores truncate.  Output error relative to 64 bits, fp16: 64 contexts of 4096 positions 6.3e-4 without
             // either, 3.1e-4 with the first or both, 2.1e-4 being what rounding the output alone leaves; one of 131071 positions
-            // 9.4e-4, 4.4e-4 with the first, 3.1e-4 with both.
+            // 9.4e-4, 4.4e-4 with the first, 3.1e-4 with both.  BASES: for the bases p is rounded to fp16 too, as
+            // 2^9 of the largest (2^15 at most) whatever e is; the sums over a tile go to fp32, so that they do not grow in the
+            // tensor cores either.
             constexpr uint32_t ONES = 0x3c003c00u;
             const float sign = sub & 1 ? -1.f : 1.f;
             uint32_t pb[NG][2];
+            if constexpr (X::BASES) {
+                uint32_t b0, b1;
+                float x[4];
+                a4_ldm_trans(b0, b1, at_b + st);
+                a4_mma0(x, b0, 0u, b1, 0u, a4_transpose(f2_to_h2(p[0] * lift, p[1] * lift)), a4_transpose(f2_to_h2(p[2] * lift, p[3] * lift)));
+                bacc[0] += x[0];
+                bacc[1] += x[1];
+            }
 #pragma unroll
             for (int g = 0; g < NG; ++g) {
                 const float y0 = fmaf(vs0[g], A4_MIDDLE, vz0[g]), y1 = fmaf(vs1[g], A4_MIDDLE, vz1[g]);
                 pb[g][0] = a4_transpose(f2_to_h2(p[0] * (sign * vs0[g]), p[1] * (sign * vs0[g])));
                 pb[g][1] = a4_transpose(f2_to_h2(p[2] * (sign * vs1[g]), p[3] * (sign * vs1[g])));
-                zacc[g][0] = fmaf(p[0], y0, fmaf(p[2], y1, zacc[g][0]));
-                zacc[g][1] = fmaf(p[1], y0, fmaf(p[3], y1, zacc[g][1]));
+                if constexpr (!X::BASES) {
+                    zacc[g][0] = fmaf(p[0], y0, fmaf(p[2], y1, zacc[g][0]));
+                    zacc[g][1] = fmaf(p[1], y0, fmaf(p[3], y1, zacc[g][1]));
+                }
                 if (g & 1) a4_mma(sacc[g / 2], 0u, ONES, 0u, ONES, pb[g][0], pb[g][1]);
                 else a4_mma(sacc[g / 2], ONES, 0u, ONES, 0u, pb[g][0], pb[g][1]);
             }
@@ -695,11 +754,22 @@ attn4_kernel(const __grid_constant__ Attn4Args A) {
         for (int o = 4; o <= 16; o <<= 1) {
             l[0] += __shfl_xor_sync(0xffffffffu, l[0], o);
             l[1] += __shfl_xor_sync(0xffffffffu, l[1], o);
+            if constexpr (!X::BASES)
 #pragma unroll
-            for (int g = 0; g < NG; ++g) {
-                zacc[g][0] += __shfl_xor_sync(0xffffffffu, zacc[g][0], o);
-                zacc[g][1] += __shfl_xor_sync(0xffffffffu, zacc[g][1], o);
-            }
+                for (int g = 0; g < NG; ++g) {
+                    zacc[g][0] += __shfl_xor_sync(0xffffffffu, zacc[g][0], o);
+                    zacc[g][1] += __shfl_xor_sync(0xffffffffu, zacc[g][1], o);
+                }
+        }
+        if constexpr (X::BASES) {
+            const float back = a4_exp2(e - 9.f);
+#pragma unroll
+            for (int g = 0; g < NG; ++g)
+#pragma unroll
+                for (int e2 = 0; e2 < 2; ++e2) {
+                    const int from = 8 * g + t;            // the lane that has the scale's sum; the base's is 4 on
+                    zacc[g][e2] = fmaf(__shfl_sync(0xffffffffu, bacc[e2], from), A4_MIDDLE, __shfl_sync(0xffffffffu, bacc[e2], from + 4)) * back;
+                }
         }
         if (lane < 4) {
             // a warp without positions has no say in the maximum
