@@ -496,6 +496,21 @@ def test_one_position_over_many_small_ones(P, oracle, d, g, vspread, vmean):
         assert (np.abs(as64(out[s]) - ref) <= bound).all()
 
 
+@pytest.mark.parametrize("d,g", [(128, 32), (128, 64), (256, 64), (96, 32), (64, 32)])
+def test_value_nan_stays_with_its_group(P, oracle, d, g):
+    hq, hkv, n = 4, 1, 90
+    k, v = as64(values((1, hkv, n, d), "f16", 61)), as64(values((1, hkv, n, d), "f16", 62))
+    v[0, 0, 70, 40] = np.nan
+    c = Cache(1, hkv, d, g, n)
+    c.fill(k, v, [n], oracle)
+    q = values((1, hq, d), "f16", 63)
+    out = torch.empty((1, hq, d), dtype=torch.float16, device=DEV)
+    c.attend(P, "f16", q, t(np.array([n], np.int32)), out, 0.088)
+    bad = torch.zeros(d, dtype=torch.bool, device=DEV)
+    bad[40 // g * g:40 // g * g + g] = True
+    assert torch.isnan(out[..., bad]).all() and torch.isfinite(out[..., ~bad]).all()
+
+
 def big_cache(oracle, b, hkv, d, g, n, seed, block=0):
     """A long cache: random words and params straight on the device."""
     c = Cache(b, hkv, d, g, n, block, seed)

@@ -99,6 +99,11 @@ __device__ __forceinline__ float a4_exp2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
     return r;
 }
+__device__ __forceinline__ float a4_max_nan(float a, float b) {      // a NaN stays
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
 template <int BYTES>
 __device__ __forceinline__ void a4_copy(uint32_t dst, const void *src, int bytes) {   // bytes = BYTES, or 0: zeros
     if constexpr (BYTES == 16)
@@ -638,9 +643,19 @@ attn4_kernel(const __grid_constant__ Attn4Args A) {
             }
             float vmax = 0.f;
 #pragma unroll
-            for (int g = 0; g < NG; ++g) vmax = fmaxf(vmax, fmaxf(vs0[g], vs1[g]));
-            if (__any_sync(0xffffffffu, fmaxf(s[0], s[2]) > bar[0] || fmaxf(s[1], s[3]) > bar[1] || vmax > most)) {
-                // a score or a value scale has outgrown what the probabilities are held against
+            for (int g = 0; g < NG; ++g) vmax = a4_max_nan(vmax, a4_max_nan(vs0[g], vs1[g]));
+            if (__any_sync(0xffffffffu, fmaxf(s[0], s[2]) > bar[0] || fmaxf(s[1], s[3]) > bar[1] || !(vmax <= most))) {
+                // a score or a value scale has outgrown what the probabilities are held against, or a value is NaN.  That must reach
+                // its own group alone, but two groups share sacc and 0 NaN is NaN: through the bases, which are apart.
+                if (vmax != vmax) {
+                    vmax = 0.f;
+#pragma unroll
+                    for (int g = 0; g < NG; ++g) {
+                        if (vs0[g] != vs0[g]) { vz0[g] = vs0[g]; vs0[g] = 0.f; }
+                        if (vs1[g] != vs1[g]) { vz1[g] = vs1[g]; vs1[g] = 0.f; }
+                        vmax = fmaxf(vmax, fmaxf(vs0[g], vs1[g]));
+                    }
+                }
                 float n0 = fmaxf(top[0], fmaxf(s[0], s[2])), n1 = fmaxf(top[1], fmaxf(s[1], s[3]));
 #pragma unroll
                 for (int o = 4; o <= 16; o <<= 1) {
