@@ -54,3 +54,41 @@ def test_counts_and_sizes_are_not_statuses(library, pkg):
     size = library.caller("b200k_gemm_workspace_bytes", Cuda)(16, 4096, 4096)
     assert size == pkg.lib().call("b200k_gemm_workspace_bytes", 16, 4096, 4096) > 0
     assert library.caller("b200k_layer_launches_per_forward", Cuda)(None) == 0
+
+
+def test_the_stream_may_be_left_out_or_named(library, pkg):
+    seen = []
+
+    def current():
+        seen.append(1)
+        return 0
+    f = library.caller("rms_norm_f16", Cuda, current)
+    args = (Cuda(), Cuda(), Cuda(), 4, 0.25, 1e-5, 0)
+    assert f(*args) == 0 and len(seen) == 1
+    assert f(*args, stream=None) == 0 and len(seen) == 2
+    stream = type("Stream", (), {"cuda_stream": 0})()
+    assert f(*args, stream=stream) == 0 and f(*args, 0) == 0 and f(*args, None) == 0 and len(seen) == 2
+    assert f.__name__ == "rms_norm_f16" and "rms_norm_f16" in f.__doc__
+    for bad, named in ((args[:-1], {}), ((*args, 0, 0), {}), (args, {"other": 0}), (args, {"stream": 0, "other": 0})):
+        with pytest.raises(TypeError):
+            f(*bad, **named)
+    with pytest.raises(TypeError):                   # no stream provider, no name
+        library.caller("rms_norm_f16", Cuda)(*args, stream=0)
+    with pytest.raises(TypeError):
+        library.caller("rms_norm_f16", Cuda)(*args)
+
+    def broken():
+        raise RuntimeError("no stream")
+    with pytest.raises(RuntimeError, match="no stream"):
+        library.caller("rms_norm_f16", Cuda, broken)(*args)
+    assert library.caller("rms_norm_f16", Cuda, current) is f
+
+
+def test_prelude_functions_are_callers(pkg):
+    f = pkg.prelude.rms_norm_f32
+    assert f is pkg.prelude.rms_norm_f32 and f.__name__ == "rms_norm_f32"
+    with pytest.raises(TypeError):
+        f(None)
+    with pytest.raises(pkg.B200KError) as e:
+        f(None, None, None, 4, 0.25, 1e-5, 1, 0)
+    assert e.value.code == -1

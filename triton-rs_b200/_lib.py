@@ -101,11 +101,12 @@ class Library:
     def raw(self, name: str):
         return self._fns[name]
 
-    def caller(self, name: str, tensor_type):
+    def caller(self, name: str, tensor_type, current=None):
         """A function of `name`'s arguments that does what `call` does, with the conversions written out for its prototype: a
         decode step makes a dozen calls of a few microseconds each, and the loop in `call` takes as long as a kernel.
-        `tensor_type` is torch.Tensor (this module does not import torch); anything else goes the way of `call`."""
-        fn = self._callers.get(name)
+        `tensor_type` is torch.Tensor (this module does not import torch); anything else goes the way of `call`.  With `current`, a
+        function, the stream (the last argument) may be left out or given by name; `current()` then says which."""
+        fn = self._callers.get((name, current))
         if fn is None:
             ret, proto = self.protos[name]
 
@@ -114,9 +115,9 @@ class Library:
             status = ret == "int" and name not in _NOT_STATUS
             if self._compiled is not None and ret in ("int", "size_t"):
                 fn = self._compiled.caller(name, types_of(proto), ctypes.cast(self._fns[name], ctypes.c_void_p).value, tensor_type,
-                                           lambda at, a: self._pointer(name, proto[at][1], a), self._stream, fail if status else None)
+                                           lambda at, a: self._pointer(name, proto[at][1], a), self._stream, fail if status else None, current)
                 if fn is not None:
-                    self._callers[name] = fn
+                    self._callers[(name, current)] = fn
                     return fn
             conv = []
             for ty, an in proto:
@@ -129,10 +130,23 @@ class Library:
                 else:
                     conv.append(f"{an} if {an}.__class__ is int else int({an})")
             check = "    if rc: E(rc)\n" if status else ""
-            src = f"def caller({', '.join(an for _, an in proto)}):\n    rc = F({', '.join(conv)})\n{check}    return rc\n"
+            src = f"def caller({', '.join([an for _, an in proto] + ['/'] * bool(proto))}):\n    rc = F({', '.join(conv)})\n{check}    return rc\n"
             space = {"T": tensor_type, "F": self._fns[name], "P": lambda a, an: self._pointer(name, an, a), "S": self._stream, "E": fail}
             exec(compile(src, f"<{name}>", "exec"), space)
-            fn = self._callers[name] = space["caller"]
+            fn = space["caller"]
+            if current is not None:
+                fn = self._streamed(name, len(proto), fn, current)
+            self._callers[(name, current)] = fn
+        return fn
+
+    @staticmethod
+    def _streamed(name, nargs, call, current):
+        def fn(*args, stream=None):
+            if len(args) == nargs - 1:
+                return call(*args, current() if stream is None else stream)
+            return call(*args)
+        fn.__name__ = name
+        fn.__doc__ = f"C ABI `{name}`; see include/b200_kernels.h for the argument list."
         return fn
 
     @staticmethod

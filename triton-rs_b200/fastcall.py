@@ -21,6 +21,7 @@ _CTYPE = {"ptr": "void *", "int": "int", "float": "float", "size_t": "size_t", "
 _FIELD = {"ptr": "p", "int": "i", "float": "f", "size_t": "u", "b200k_stream": "p", "uint64_t": "u", "int64_t": "i"}
 _CODE = {"ptr": "p", "int": "i", "float": "f", "size_t": "u", "b200k_stream": "s", "uint64_t": "u", "int64_t": "l"}
 _RET = {"int": "int", "size_t": "size_t"}
+EDITION = 2          # of the arguments that the extension's caller() takes
 
 _BODY = r"""
 #define PY_SSIZE_T_CLEAN
@@ -45,9 +46,10 @@ typedef struct {
     Py_ssize_t count;
     PyTypeObject *tensor;                 /* exact type whose data_ptr() is taken */
     PyObject *pointer, *stream, *error;   /* what Python does with other arguments, and with a status that is not 0 (or None) */
+    PyObject *current;                    /* None, or what gives the stream of a call that leaves it out */
 } Caller;
 
-static PyObject *s_is_cuda, *s_data_ptr;
+static PyObject *s_is_cuda, *s_data_ptr, *s_stream;
 
 static int convert(Caller *c, PyObject *o, Py_ssize_t at, Arg *a) {
     PyObject *v = NULL;
@@ -103,14 +105,24 @@ static int convert(Caller *c, PyObject *o, Py_ssize_t at, Arg *a) {
 
 static PyObject *caller_call(PyObject *self, PyObject *const *args, size_t nargsf, PyObject *kwnames) {
     Caller *c = (Caller *)self;
-    const Py_ssize_t n = PyVectorcall_NARGS(nargsf);
-    if (n != c->count || (kwnames && PyTuple_GET_SIZE(kwnames))) {
-        PyErr_Format(PyExc_TypeError, "%%s takes %%zd arguments, got %%zd", c->proto->name, c->count, n);
+    const Py_ssize_t n = PyVectorcall_NARGS(nargsf), named = kwnames ? PyTuple_GET_SIZE(kwnames) : 0;
+    const int may = c->current != Py_None;
+    if (!(n == c->count || (may && n == c->count - 1)) || named > may ||
+        (named && PyUnicode_Compare(PyTuple_GET_ITEM(kwnames, 0), s_stream))) {
+        if (!PyErr_Occurred())
+            PyErr_Format(PyExc_TypeError, "%%s takes %%zd arguments%%s, got %%zd", c->proto->name, c->count, may ? " (the stream may be left out or named)" : "", n);
         return NULL;
     }
     Arg a[MOST];
     for (Py_ssize_t i = 0; i < n; ++i)
         if (convert(c, args[i], i, &a[i])) return NULL;
+    if (n < c->count) {
+        PyObject *own = named && args[n] != Py_None ? Py_NewRef(args[n]) : PyObject_CallNoArgs(c->current);
+        if (!own) return NULL;
+        const int bad = convert(c, own, n, &a[n]);
+        Py_DECREF(own);
+        if (bad) return NULL;
+    }
     long long rc;
     Py_BEGIN_ALLOW_THREADS
     rc = c->proto->call(c->address, a);
@@ -129,20 +141,29 @@ static void caller_free(PyObject *self) {
     Py_CLEAR(c->pointer);
     Py_CLEAR(c->stream);
     Py_CLEAR(c->error);
+    Py_CLEAR(c->current);
     Py_TYPE(self)->tp_free(self);
 }
+
+static PyObject *caller_name(PyObject *self, void *unused) { return PyUnicode_FromString(((Caller *)self)->proto->name); }
+static PyObject *caller_doc(PyObject *self, void *unused) {
+    return PyUnicode_FromFormat("C ABI `%%s`; see include/b200_kernels.h for the argument list.", ((Caller *)self)->proto->name);
+}
+static PyGetSetDef caller_has[] = {{"__name__", caller_name}, {"__doc__", caller_doc}, {NULL}};
 
 static PyTypeObject CallerType = {
     PyVarObject_HEAD_INIT(NULL, 0).tp_name = "_b200_call.Caller", .tp_basicsize = sizeof(Caller), .tp_dealloc = caller_free,
     .tp_flags = Py_TPFLAGS_DEFAULT | Py_TPFLAGS_HAVE_VECTORCALL, .tp_vectorcall_offset = offsetof(Caller, vectorcall), .tp_call = PyVectorcall_Call,
-    .tp_doc = "A library function with its arguments converted in C."};
+    .tp_getset = caller_has};
 
-/* caller(name, types, address, tensor type, pointer, stream, error): None when this build has no such prototype */
+/* caller(name, types, address, tensor type, pointer, stream, error, current): None when this build has no such prototype */
 static PyObject *make_caller(PyObject *self, PyObject *args) {
     const char *name, *types;
     unsigned long long address;
-    PyObject *tensor, *pointer, *stream, *error;
-    if (!PyArg_ParseTuple(args, "ssKOOOO", &name, &types, &address, &tensor, &pointer, &stream, &error)) return NULL;
+    PyObject *tensor, *pointer, *stream, *error, *current;
+    if (!PyArg_ParseTuple(args, "ssKOOOOO", &name, &types, &address, &tensor, &pointer, &stream, &error, &current)) return NULL;
+    const size_t count = strlen(types);
+    if (current != Py_None && (!count || types[count - 1] != 's')) Py_RETURN_NONE;
     for (int i = 0; i < COUNT; ++i)
         if (!strcmp(protos[i].name, name) && !strcmp(protos[i].types, types) && PyType_Check(tensor)) {
             Caller *c = (Caller *)CallerType.tp_alloc(&CallerType, 0);
@@ -150,11 +171,12 @@ static PyObject *make_caller(PyObject *self, PyObject *args) {
             c->vectorcall = caller_call;
             c->proto = &protos[i];
             c->address = (void *)(uintptr_t)address;
-            c->count = (Py_ssize_t)strlen(types);
+            c->count = (Py_ssize_t)count;
             c->tensor = (PyTypeObject *)Py_NewRef(tensor);
             c->pointer = Py_NewRef(pointer);
             c->stream = Py_NewRef(stream);
             c->error = Py_NewRef(error);
+            c->current = Py_NewRef(current);
             return (PyObject *)c;
         }
     Py_RETURN_NONE;
@@ -165,8 +187,11 @@ static struct PyModuleDef module = {PyModuleDef_HEAD_INIT, "_b200_call", "Argume
 PyMODINIT_FUNC PyInit__b200_call(void) {
     s_is_cuda = PyUnicode_InternFromString("is_cuda");
     s_data_ptr = PyUnicode_InternFromString("data_ptr");
-    if (!s_is_cuda || !s_data_ptr || PyType_Ready(&CallerType) < 0) return NULL;
-    return PyModule_Create(&module);
+    s_stream = PyUnicode_InternFromString("stream");
+    if (!s_is_cuda || !s_data_ptr || !s_stream || PyType_Ready(&CallerType) < 0) return NULL;
+    PyObject *m = PyModule_Create(&module);
+    if (m && PyModule_AddIntConstant(m, "EDITION", %(edition)d)) Py_CLEAR(m);
+    return m;
 }
 """
 
@@ -186,7 +211,7 @@ def source(protos) -> str:
         conv = ", ".join(f"({_CTYPE[ty]})a[{i}].{_FIELD[ty]}" if ty != "float" else f"a[{i}].f" for i, (ty, _) in enumerate(args))
         calls.append(f"static long long call_{name}(void *f, const Arg *a) {{ return (long long)(({_RET[ret]} (*)({sig}))f)({conv}); }}")
         table.append(f'    {{"{name}", "{types_of(args)}", call_{name}}},')
-    return _BODY % {"calls": "\n".join(calls), "table": "\n".join(table) + "\n", "most": most}
+    return _BODY % {"edition": EDITION, "calls": "\n".join(calls), "table": "\n".join(table) + "\n", "most": most}
 
 
 def build(protos, obj_dir: Path) -> Path | None:
@@ -213,6 +238,6 @@ def load():
         spec = importlib.util.spec_from_file_location("_b200_call", OUT)
         mod = importlib.util.module_from_spec(spec)
         spec.loader.exec_module(mod)
-        return mod
+        return mod if getattr(mod, "EDITION", 1) == EDITION else None
     except ImportError:
         return None

@@ -26,23 +26,12 @@ if hasattr(torch._C, "_cuda_getCurrentRawStream"):   # the same stream without b
         return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
 
 
-def _make(name, nargs):
-    def fn(*args, stream=None):
-        call = lib().caller(name, torch.Tensor)
-        if len(args) == nargs - 1:  # stream omitted
-            return call(*args, _current_stream() if stream is None else stream)
-        return call(*args)
-    fn.__name__ = name
-    fn.__doc__ = f"C ABI `{name}`; see include/b200_kernels.h for the argument list."
-    return fn
-
-
 def __getattr__(name):
     protos = lib().protos
     if name in protos:
         ret, args = protos[name]
         if args and args[-1][0] == "b200k_stream":
-            f = _make(name, len(args))
+            f = lib().caller(name, torch.Tensor, _current_stream)
         else:
             def f(*a, _n=name):
                 return lib().call(_n, *a)
