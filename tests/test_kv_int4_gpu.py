@@ -511,6 +511,23 @@ def test_value_nan_stays_with_its_group(P, oracle, d, g):
     assert torch.isnan(out[..., bad]).all() and torch.isfinite(out[..., ~bad]).all()
 
 
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("hq,hkv,d,g,block", [(3, 3, 32, 32, 4), (4, 4, 64, 32, 0), (6, 2, 64, 64, 7), (9, 1, 96, 32, 0), (16, 2, 128, 32, 0), (32, 8, 128, 64, 16),
+                                              (32, 2, 128, 128, 0), (8, 2, 160, 32, 0), (4, 1, 192, 64, 0), (4, 2, 192, 32, 32), (2, 1, 224, 32, 16),
+                                              (7, 1, 256, 32, 16), (4, 1, 256, 64, 0), (10, 2, 256, 128, 0)])
+def test_attention_cut_and_whole_contexts(P, oracle, dtype, hq, hkv, d, g, block):
+    """Every shape with contexts that several CTAs share and, in a call of their own, with ones that one CTA has."""
+    c = Cache(3, hkv, d, g, 700, block, seed=d)
+    lens = [700, 385, 1]
+    k, v = as64(values((3, hkv, 700, d), dtype, 24)), as64(values((3, hkv, 700, d), dtype, 25))
+    c.fill(k, v, lens, oracle)
+    q = values((3, hq, d), dtype, 26)
+    for now in (lens, [256, 129, 1]):
+        out = torch.full((3, hq, d), float("nan"), dtype=TYPES[dtype], device=DEV)
+        c.attend(P, dtype, q, t(np.array(now, np.int32)), out, d ** -0.5)
+        check_attention(oracle, c, q, now, out, d ** -0.5, dtype)
+
+
 def big_cache(oracle, b, hkv, d, g, n, seed, block=0):
     """A long cache: random words and params straight on the device."""
     c = Cache(b, hkv, d, g, n, block, seed)

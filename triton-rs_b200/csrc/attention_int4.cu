@@ -13,9 +13,9 @@
 // of a GQA group the 8 columns; one query token a sequence cannot fill a 128-row tcgen05 tile.
 //
 // What bounds it: the bytes of the cache where contexts are long (74 x 8 contexts of 16384 positions, D 128, groups of 64:
-// 236 us, 0.91 of the copy bandwidth), and just below that the issue of instructions: about 250 a warp for 16 positions of K
+// 238 us, 0.9 of the copy bandwidth), and just below that the issue of instructions: about 250 a warp for 16 positions of K
 // and V, half of them on the integer pipe, at 0.6 a cycle and scheduler; HBM delivers 16 positions to an SM every 96 cycles.
-// At 64 x 4096 positions (46 us of bytes) 66 us: starting takes 4 us, the joins of the CTAs 4, and the rest is the issue
+// At 64 x 4096 positions (46 us of bytes) 67 us: starting takes 4 us, the joins of the CTAs 4, and the rest is the issue
 // rate.  Groups of 32 take a fifth more instructions (78 us), groups of 128 a tenth fewer (57 us).
 //
 // Work is dealt out on the device, from the lengths, so a captured graph follows them; see the kernel's first part.  Each warp
@@ -33,6 +33,7 @@ constexpr int A4_TILE = 16, A4_SUBS = 2;                // positions of a tile (
 constexpr int A4_STEP = A4_SUBS * A4_TILE, A4_UNIT = A4_WARPS * A4_STEP;       // positions of a warp's stage, of a unit of work
 constexpr int A4_MAX_CTAS = 640;                               // CTAs of a launch: one wave
 constexpr int A4_FAN = 16;                                     // partial results that are joined at a time
+constexpr unsigned A4_WHOLE = 2;                               // units of contexts that are never cut
 constexpr int A4_HEADS = 8;                                    // columns of one MMA
 constexpr float A4_MIDDLE = 7.5f;     // of the codes
 constexpr float A4_LAZY = 6.f;        // the running maximum moves when a score passes it by 2^6: probabilities stay below 2^6
@@ -285,6 +286,9 @@ attn4_kernel(const __grid_constant__ Attn4Args A) {
         contexts = __reduce_add_sync(0xffffffffu, contexts) * per_seq;
         longest = __reduce_max_sync(0xffffffffu, longest);
         share = max((total + gridDim.x - 1) / gridDim.x, 1u);
+        // contexts of one or two units stay whole: nothing to join.  236 positions, 1 / 8 / 32 sequences: 6.9 / 9.6 / 10.7 us, cut
+        // 8.1 / 10.1 / 11.6; three units 7.9 / 11.4 / 12.7 against 8.2 / 10.2 / 13.6, four 8.7 / 13.1 / 14.5 against 8.1 / 10.4 / 14.3
+        if (longest <= A4_WHOLE && contexts <= gridDim.x) share = A4_WHOLE;
         bool cut = contexts > gridDim.x;                   // pieces will not do
         for (unsigned s = share; !cut && share > 1;) {     // with a unit for every CTA, units are the pieces
             unsigned pieces = 0;
