@@ -296,14 +296,15 @@ attn4_kernel(const __grid_constant__ Attn4Args A) {
             for (int b = lane; b < A.batch; b += 32) pieces += (units_of(b) + s - 1) / s;
             pieces = __reduce_add_sync(0xffffffffu, pieces) * per_seq;
             if (pieces <= gridDim.x) {
-                share = s;
+                cut = s > share + share / 6 + 2 && 5 * pieces < 4 * gridDim.x;
+                if (!cut) share = s;
                 break;
             }
             // a piece fewer for the longest context
             const unsigned parts = (longest + s - 1) / s;
             cut = parts < 2;
             if (!cut) s = (longest + parts - 2) / (parts - 1);
-            cut = cut || s > share + share / 6 + 2;
+            cut = cut || s > share + share / 6 + (2 * contexts > gridDim.x ? 12 : 2);
         }
         // the sequence that this CTA's first unit, or its piece, belongs to
         if (cut) {
