@@ -242,10 +242,13 @@ attn4_kernel(const __grid_constant__ Attn4Args A) {
     pdl_launch_dependents();
 
     // ---- the share of this CTA, by warp 0 (the host made sure that 32 bits hold all units) ----------------------------------------
-    // Either one piece of one context, all contexts being cut into pieces of at most `share` units, no more pieces than CTAs; or,
-    // where the largest piece would be over a sixth more than an equal share, units [at, end) of all, which may begin and end
-    // within contexts: a CTA then joins and starts anew wherever it passes from one to the next.  One context of 131071
-    // positions: 38.7 us in pieces, 43 cut evenly; 32 of 512 to 8192 positions, the pieces up to a third larger: 58.5 and 57.2.
+    // Either one piece of one context, all contexts being cut into pieces of at most `share` units, no more pieces than CTAs; or
+    // units [at, end) of all, which may begin and end within contexts: a CTA then joins and starts anew wherever it passes from
+    // one to the next.  Pieces are taken where the largest is a sixth (and two units) over an equal share at most: one context of
+    // 131071 positions 38.7 us in pieces, 43 cut evenly; 32 of 512 to 8192 positions, the pieces a third larger, groups of 32: 56 and
+    // 54.7.  Twelve units over it are still better where more than every other CTA would start anew and four of five have a
+    // piece: 40 sequences of 100 to 4000 positions 38.7 and 42.2 us, 100 of 4 kv heads up to 5000 44.6 and 50; but 50 of 1000 to
+    // 3000, whole contexts for two of three CTAs, 46.4 and 38.9.
     const unsigned per_seq = C.heads * A.head_blocks;      // contexts of a sequence
     auto units_of = [&](int b) { return (unsigned)(max(min(A.lens[b], C.capacity), 0) + A4_UNIT - 1) / A4_UNIT; };
     auto place_heads = [&](Attn4Segment &d, unsigned ctx) {
