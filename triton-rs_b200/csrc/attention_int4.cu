@@ -226,7 +226,10 @@ struct Attn4Segment {
     unsigned share, at, end;        // units of a CTA; those that follow this segment in this CTA: [at, end)
 };
 
-template <int NB, int NG>
+// SPLIT: the q heads of a kv head, 4 or fewer, stand in both halves of the columns.  The second half takes what the first half's
+// probabilities times scales lose when they are rounded to fp16: nothing is lost then, and no instruction but those that
+// part them is added.  For fp16 outputs; a bf16 output's own rounding is eight times larger.
+template <int NB, int NG, bool SPLIT>
 __global__ void __launch_bounds__(A4_THREADS, A4<NB, NG>::CTAS)
 attn4_kernel(const __grid_constant__ Attn4Args A) {
     using X = A4<NB, NG>;
@@ -459,13 +462,16 @@ attn4_kernel(const __grid_constant__ Attn4Args A) {
         src_v = (const unsigned char *)C.v_codes + row0 * X::ROW + lane * 16;
         src_p = (const unsigned char *)(lane < 16 ? C.k_params : C.v_params) + (row0 + (lane & 15)) * X::PROW;
         bool edge = issue(d, 0, 0);
+        const uint32_t w_flip = t >= 2 ? 0x80000000u : 0u;
+        const float w_all = t >= 2 ? 1.f : 0.f;
 
         // ---- q as the B operand, a word by each warp; scaled by a power of two to [2^14, 2^15) -------------------------------------------
         // (any 16-bit type then fits fp16 with all its bits, down to 2^-25 of the head's largest element; nibbles 1 and 3 carry
         // 2^4 more than 0 and 2, so their q is divided by 16)
         {
             // head r, lane t's dims: of operand word i 4 + 4 (two blocks), or 8 in a row (one block)
-            const uint16_t *qrow = (const uint16_t *)A.q + ((long)d.b * A.hq + d.h0 + (r < d.heads ? r : 0)) * X::D;
+            const int hr = SPLIT ? r & 3 : r;
+            const uint16_t *qrow = (const uint16_t *)A.q + ((long)d.b * A.hq + d.h0 + (hr < d.heads ? hr : 0)) * X::D;
             auto word = [&](int i) {
                 int lo, hi;
                 a4_kdims<NB, X::PURE>(i, 0, t, lo, hi);
@@ -484,7 +490,7 @@ attn4_kernel(const __grid_constant__ Attn4Args A) {
             top2 = max(top2, __shfl_xor_sync(0xffffffffu, top2, 2));
             const float big = A.bf16 ? __uint_as_float(top2 << 16) : __half2float(__ushort_as_half((unsigned short)top2));
             const int k = min(14 - ((int)(__float_as_uint(big) >> 23) - 127), 126);
-            const float up = r < d.heads ? copysignf(__uint_as_float((uint32_t)(k + 127) << 23), A.scale_log2e) : 0.f, up16 = up * 0.0625f;
+            const float up = hr < d.heads ? copysignf(__uint_as_float((uint32_t)(k + 127) << 23), A.scale_log2e) : 0.f, up16 = up * 0.0625f;
 #pragma unroll 1
             for (int i = warp; i < NB; i += A4_WARPS) {
                 const uint4 u = word(i);       // u.x, u.y: dims 0-3 of the low half, u.z, u.w of the high one
@@ -500,7 +506,7 @@ attn4_kernel(const __grid_constant__ Attn4Args A) {
                 }
 #pragma unroll
                 for (int e2 = 0; e2 < 8; ++e2) f[e2] *= e2 & 1 ? up16 : up;
-                if (r >= d.heads) f[0] = f[1] = f[2] = f[3] = f[4] = f[5] = f[6] = f[7] = 0.f;     // another head's row stood in
+                if (hr >= d.heads) f[0] = f[1] = f[2] = f[3] = f[4] = f[5] = f[6] = f[7] = 0.f;     // another head's row stood in
                 sm_q[i][lane] = make_uint4(f2_to_h2(f[0], f[4]), f2_to_h2(f[1], f[5]), f2_to_h2(f[2], f[6]), f2_to_h2(f[3], f[7]));
                 float sum = fmaf((f[1] + f[5]) + (f[3] + f[7]), 16.f, (f[0] + f[4]) + (f[2] + f[6]));
                 sum += __shfl_xor_sync(0xffffffffu, sum, 1);
@@ -508,7 +514,7 @@ attn4_kernel(const __grid_constant__ Attn4Args A) {
                 if (t == 0) sm_qsum[i][r] = sum * (1.f / 16777216.f);
             }
             // what a score is multiplied by; a q with an infinity or a NaN has no finite score: NaN
-            if (warp == 0 && t == 0) sm_fac[r] = r >= d.heads ? 0.f : big < INFINITY ? fabsf(A.scale_log2e) / fabsf(up) * 16777216.f : NAN;
+            if (warp == 0 && t == 0) sm_fac[r] = hr >= d.heads ? 0.f : big < INFINITY ? fabsf(A.scale_log2e) / fabsf(up) * 16777216.f : NAN;
         }
         __syncthreads();
         float qsum[NG][2];                     // of heads 2t and 2t + 1
@@ -714,13 +720,15 @@ attn4_kernel(const __grid_constant__ Attn4Args A) {
             }
             l[0] += p[0] + p[2];
             l[1] += p[1] + p[3];
-            // w = probability x value scale, rounded to fp16, is the B operand.  With it
+            // w = probability x value scale, rounded to fp16, is the B operand (SPLIT: its upper 11 bits in one column, the rest in
+            // another).  With it
             //   sum p v = sum w (c - 7.5) + sum p (z + 7.5 s) = sum w c - 7.5 sum w + sum p (z + 7.5 s)
             // so that its rounding meets a code's distance from the middle, not the code; a product with ones gives sum w.  Every
             // other tile adds -w (15 - c) in place of w c: the codes are not centred, their sum would grow with the context, and
             // the tensor cores truncate.  Output error relative to 64 bits, fp16: 64 contexts of 4096 positions 6.3e-4 without
-            // either, 3.1e-4 with the first or both, 2.1e-4 being what rounding the output alone leaves; one of 131071 positions
-            // 9.4e-4, 4.4e-4 with the first, 3.1e-4 with both.  BASES: for the bases p is rounded to fp16 too, as
+            // either, 3.1e-4 with the first or both, 2.1e-4 with SPLIT too, which is what rounding the output alone leaves; one of
+            // 131071 positions 9.4e-4, 4.4e-4 with the first, 3.1e-4 with both, 2.1e-4 with SPLIT too.  SPLIT costs 4.5 % (64 x 4096: 67 ->
+            // 70 us; as a branch in one kernel 72 and slower for every other call).  BASES: for the bases p is rounded to fp16 too, as
             // 2^9 of the largest (2^15 at most) whatever e is; the sums over a tile go to fp32, so that they do not grow in the
             // tensor cores either.
             constexpr uint32_t ONES = 0x3c003c00u;
@@ -737,8 +745,12 @@ attn4_kernel(const __grid_constant__ Attn4Args A) {
 #pragma unroll
             for (int g = 0; g < NG; ++g) {
                 const float y0 = fmaf(vs0[g], A4_MIDDLE, vz0[g]), y1 = fmaf(vs1[g], A4_MIDDLE, vz1[g]);
-                pb[g][0] = a4_transpose(f2_to_h2(p[0] * (sign * vs0[g]), p[1] * (sign * vs0[g])));
-                pb[g][1] = a4_transpose(f2_to_h2(p[2] * (sign * vs1[g]), p[3] * (sign * vs1[g])));
+                float w[4] = {p[0] * (sign * vs0[g]), p[1] * (sign * vs0[g]), p[2] * (sign * vs1[g]), p[3] * (sign * vs1[g])};
+                if constexpr (SPLIT)           // upper 11 bits, or x minus these
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) w[i] = fmaf(w[i], w_all, __uint_as_float((__float_as_uint(w[i]) & 0xffffe000u) ^ w_flip));
+                pb[g][0] = a4_transpose(f2_to_h2(w[0], w[1]));
+                pb[g][1] = a4_transpose(f2_to_h2(w[2], w[3]));
                 if constexpr (!X::BASES) {
                     zacc[g][0] = fmaf(p[0], y0, fmaf(p[2], y1, zacc[g][0]));
                     zacc[g][1] = fmaf(p[1], y0, fmaf(p[3], y1, zacc[g][1]));
@@ -821,15 +833,20 @@ attn4_kernel(const __grid_constant__ Attn4Args A) {
                 *reinterpret_cast<float2 *>(&sm_sum[2 * t]) = make_float2(L[0], L[1]);
             }
             float *o0 = so + (warp * X::D + r) * A4_HEADS + 2 * t;
+            const float own = SPLIT && t >= 2 ? 0.f : 1.f;         // the bases count once
 #pragma unroll
             for (int m = 0; m < X::MTILES; ++m) {
                 const int g = (m / 2) * NG / NB;
-                const float za = fmaf(sacc[g / 2][2 * (g & 1)], -A4_MIDDLE, zacc[g][0]) * wgt[0];
-                const float zb = fmaf(sacc[g / 2][2 * (g & 1) + 1], -A4_MIDDLE, zacc[g][1]) * wgt[1];
-                *reinterpret_cast<float2 *>(o0 + m * 16 * A4_HEADS) =
-                    make_float2(fmaf(oacc[m][0], 16777216.f * wgt[0], za), fmaf(oacc[m][1], 16777216.f * wgt[1], zb));
-                *reinterpret_cast<float2 *>(o0 + (m * 16 + 8) * A4_HEADS) =
-                    make_float2(fmaf(oacc[m][2], 1048576.f * wgt[0], za), fmaf(oacc[m][3], 1048576.f * wgt[1], zb));
+                const float za = fmaf(sacc[g / 2][2 * (g & 1)], -A4_MIDDLE, zacc[g][0] * own) * wgt[0];
+                const float zb = fmaf(sacc[g / 2][2 * (g & 1) + 1], -A4_MIDDLE, zacc[g][1] * own) * wgt[1];
+                float2 lo = make_float2(fmaf(oacc[m][0], 16777216.f * wgt[0], za), fmaf(oacc[m][1], 16777216.f * wgt[1], zb));
+                float2 hi = make_float2(fmaf(oacc[m][2], 1048576.f * wgt[0], za), fmaf(oacc[m][3], 1048576.f * wgt[1], zb));
+                if constexpr (SPLIT) {
+                    lo.x += __shfl_xor_sync(0xffffffffu, lo.x, 2); lo.y += __shfl_xor_sync(0xffffffffu, lo.y, 2);
+                    hi.x += __shfl_xor_sync(0xffffffffu, hi.x, 2); hi.y += __shfl_xor_sync(0xffffffffu, hi.y, 2);
+                }
+                *reinterpret_cast<float2 *>(o0 + m * 16 * A4_HEADS) = lo;
+                *reinterpret_cast<float2 *>(o0 + (m * 16 + 8) * A4_HEADS) = hi;
             }
         }
         __syncthreads();
@@ -959,15 +976,21 @@ attn4_kernel(const __grid_constant__ Attn4Args A) {
 constexpr size_t A4_COUNTERS_OFF = 256, A4_PARTS_OFF = 128 * 1024;
 static size_t attn4_ws_bytes(int d) { return A4_PARTS_OFF + (size_t)A4_MAX_CTAS * 2 * (d * A4_HEADS + 16) * sizeof(float); }
 
-template <int NB, int NG>
+template <int NB, int NG, bool SPLIT>
 static int attn4_launch_as(const char *name, const Attn4Args &A, long max_units, cudaStream_t st) {
     using X = A4<NB, NG>;
     static OncePerDevice once;
-    cudaError_t e = once.run([&] { return cudaFuncSetAttribute(attn4_kernel<NB, NG>, cudaFuncAttributeMaxDynamicSharedMemorySize, X::SMEM); });
+    cudaError_t e = once.run([&] { return cudaFuncSetAttribute(attn4_kernel<NB, NG, SPLIT>, cudaFuncAttributeMaxDynamicSharedMemorySize, X::SMEM); });
     if (e != cudaSuccess) return fail((int)e, "%s: shared memory %d: %s", name, X::SMEM, cudaGetErrorString(e));
     const int wave = min(sm_count() * X::CTAS, A4_MAX_CTAS);
-    launch_kernel(attn4_kernel<NB, NG>, dim3((unsigned)min(max_units, (long)wave)), dim3(A4_THREADS), X::SMEM, st, A);
+    launch_kernel(attn4_kernel<NB, NG, SPLIT>, dim3((unsigned)min(max_units, (long)wave)), dim3(A4_THREADS), X::SMEM, st, A);
     return launch_status(name);
+}
+
+template <int NB, int NG>
+static int attn4_launch_shape(const char *name, const Attn4Args &A, long max_units, cudaStream_t st) {
+    const bool split = !A.bf16 && A.hq / A.C.heads <= 4;
+    return split ? attn4_launch_as<NB, NG, true>(name, A, max_units, st) : attn4_launch_as<NB, NG, false>(name, A, max_units, st);
 }
 
 static int attn4_launch(const char *name, const void *q, const Kv4Cache &C, bool paged, const int32_t *lens, void *out, int batch, int hq,
@@ -997,20 +1020,20 @@ static int attn4_launch(const char *name, const void *q, const Kv4Cache &C, bool
     B200K_REQUIRE(max_units < (1l << 31), B200K_E_SHAPE, "%s: batch * num_kv_heads * ceil(gqa / 8) * ceil(positions / 128) = %ld exceeds 31 bits", name, max_units);
     cudaStream_t st = to_stream(stream);
     switch (C.d / 32 * 1000 + C.d / C.g) {
-        case 1001: return attn4_launch_as<1, 1>(name, A, max_units, st);
-        case 2001: return attn4_launch_as<2, 1>(name, A, max_units, st);
-        case 2002: return attn4_launch_as<2, 2>(name, A, max_units, st);
-        case 3003: return attn4_launch_as<3, 3>(name, A, max_units, st);
-        case 4001: return attn4_launch_as<4, 1>(name, A, max_units, st);
-        case 4002: return attn4_launch_as<4, 2>(name, A, max_units, st);
-        case 4004: return attn4_launch_as<4, 4>(name, A, max_units, st);
-        case 5005: return attn4_launch_as<5, 5>(name, A, max_units, st);
-        case 6003: return attn4_launch_as<6, 3>(name, A, max_units, st);
-        case 6006: return attn4_launch_as<6, 6>(name, A, max_units, st);
-        case 7007: return attn4_launch_as<7, 7>(name, A, max_units, st);
-        case 8002: return attn4_launch_as<8, 2>(name, A, max_units, st);
-        case 8004: return attn4_launch_as<8, 4>(name, A, max_units, st);
-        case 8008: return attn4_launch_as<8, 8>(name, A, max_units, st);
+        case 1001: return attn4_launch_shape<1, 1>(name, A, max_units, st);
+        case 2001: return attn4_launch_shape<2, 1>(name, A, max_units, st);
+        case 2002: return attn4_launch_shape<2, 2>(name, A, max_units, st);
+        case 3003: return attn4_launch_shape<3, 3>(name, A, max_units, st);
+        case 4001: return attn4_launch_shape<4, 1>(name, A, max_units, st);
+        case 4002: return attn4_launch_shape<4, 2>(name, A, max_units, st);
+        case 4004: return attn4_launch_shape<4, 4>(name, A, max_units, st);
+        case 5005: return attn4_launch_shape<5, 5>(name, A, max_units, st);
+        case 6003: return attn4_launch_shape<6, 3>(name, A, max_units, st);
+        case 6006: return attn4_launch_shape<6, 6>(name, A, max_units, st);
+        case 7007: return attn4_launch_shape<7, 7>(name, A, max_units, st);
+        case 8002: return attn4_launch_shape<8, 2>(name, A, max_units, st);
+        case 8004: return attn4_launch_shape<8, 4>(name, A, max_units, st);
+        case 8008: return attn4_launch_shape<8, 8>(name, A, max_units, st);
     }
     return fail(B200K_E_SHAPE, "%s: head_dim %d, group_size %d", name, C.d, C.g);
 }
