@@ -13,10 +13,10 @@
 // of a GQA group the 8 columns; one query token a sequence cannot fill a 128-row tcgen05 tile.
 //
 // What bounds it: the bytes of the cache where contexts are long (74 x 8 contexts of 16384 positions, D 128, groups of 64:
-// 238 us, 0.9 of the copy bandwidth), and just below that the issue of instructions: about 250 a warp for 16 positions of K
+// 246 us, 0.87 of the copy bandwidth), and just below that the issue of instructions: about 265 a warp for 16 positions of K
 // and V, half of them on the integer pipe, at 0.6 a cycle and scheduler; HBM delivers 16 positions to an SM every 96 cycles.
-// At 64 x 4096 positions (46 us of bytes) 67 us: starting takes 4 us, the joins of the CTAs 4, and the rest is the issue
-// rate.  Groups of 32 take a fifth more instructions (78 us), groups of 128 a tenth fewer (57 us).
+// At 64 x 4096 positions (46 us of bytes) 69 us: starting takes 4 us, the joins of the CTAs 4, and the rest is the issue
+// rate.  Groups of 32 take a fifth more instructions (86 us), groups of 128 a tenth fewer (59 us).
 //
 // Work is dealt out on the device, from the lengths, so a captured graph follows them; see the kernel's first part.  Each warp
 // streams two 16-position tiles a stage through a ring of cp.async stages of its own, without a barrier between warps: four
@@ -65,8 +65,8 @@ struct A4 {
     static constexpr int MTILES = 2 * NB;
     static constexpr bool PURE = G == 32;                     // a group is one block: see kword()
     // With four groups the bases go through matrix instructions as well (a row's params are the 16 bytes that these want): two of
-    // them, and 14 others, for 48 on scalars.  D 128, groups of 32, 64 x 4096: 78 us, 84 without; with two groups, where 16
-    // instructions replace 24, 65.9 and 66.6, which is not worth rounding the probabilities that meet the bases to fp16.
+    // them, and 14 others, for 48 on scalars.  D 128, groups of 32, 64 x 4096: 78 us, 84 without (neither with SPLIT); with two
+    // groups, where 16 instructions replace 24, 65.9 and 66.6, which is not worth rounding the probabilities that meet the bases to fp16.
     static constexpr bool BASES = NG == 4;
     static constexpr int PART = D * A4_HEADS + 16;            // floats of a partial result
     static constexpr int CTAS = NB <= 4 ? 4 : NB <= 5 ? 3 : 2;
@@ -228,11 +228,14 @@ struct Attn4Segment {
 
 // SPLIT: the q heads of a kv head, 4 or fewer, stand in both halves of the columns.  The second half takes what the first half's
 // probabilities times scales lose when they are rounded to fp16: nothing is lost then, and no instruction but those that
-// part them is added.  For fp16 outputs; a bf16 output's own rounding is eight times larger.
-template <int NB, int NG, bool SPLIT>
+// part them is added.  For fp16 outputs; a bf16 output's own rounding is eight times larger.  With more heads an fp16 output is
+// 3.0e-4 off (2.1e-4 from its own rounding), 3.1e-4 if the bases met rounded probabilities too.
+enum { A4_PLAIN, A4_SPLIT, A4_EXACT_BASES };      // A4_EXACT_BASES: fp16 outputs of more than 4 heads do without BASES
+template <int NB, int NG, int MODE>
 __global__ void __launch_bounds__(A4_THREADS, A4<NB, NG>::CTAS)
 attn4_kernel(const __grid_constant__ Attn4Args A) {
     using X = A4<NB, NG>;
+    constexpr bool SPLIT = MODE == A4_SPLIT, BASES = X::BASES && MODE != A4_EXACT_BASES;
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ __align__(16) float sm_ref[A4_WARPS][A4_HEADS], sm_l[A4_WARPS][A4_HEADS], sm_top[A4_HEADS], sm_sum[A4_HEADS];
     __shared__ __align__(16) uint4 sm_q[NB][32];       // q as the B operand: word i of all lanes
@@ -383,8 +386,8 @@ attn4_kernel(const __grid_constant__ Attn4Args A) {
     auto piece_at = [&](int pos) { return ring + (A4_TILE + pos) * X::ROW + (((2 * NB * r >> 4) ^ X::swizzle(pos)) << 4) + (2 * NB * r & 15); };
     const uint32_t at_v0 = a4_keep(piece_at(t)), at_v1 = a4_keep(piece_at(4 + (t ^ 1)));
     // BASES: the params of V as a matrix [MMA index][scale, base of each group], and K's word of group t
-    const uint32_t at_b = X::BASES ? a4_keep(ring + 2 * A4_TILE * X::ROW + (2 * a4_pos(lane & 15) + 1) * X::PROW) : 0;
-    const uint32_t at_kz = X::BASES ? a4_keep(at_p + 4 * t) : 0;
+    const uint32_t at_b = BASES ? a4_keep(ring + 2 * A4_TILE * X::ROW + (2 * a4_pos(lane & 15) + 1) * X::PROW) : 0;
+    const uint32_t at_kz = BASES ? a4_keep(at_p + 4 * t) : 0;
 
     // ---- streaming a piece: tile i of this warp goes to stage i % STAGES ------------------------------------------------------------
     // 16 neighbouring rows are one linear part of the cache, so a tile that is whole and lies in one block takes nothing but
@@ -520,7 +523,7 @@ attn4_kernel(const __grid_constant__ Attn4Args A) {
         float qsum[NG][2];                     // of heads 2t and 2t + 1
         const float fac[2] = {sm_fac[2 * t], sm_fac[2 * t + 1]};
         uint32_t qz0 = 0, qz1 = 0;
-        if constexpr (X::BASES) {
+        if constexpr (BASES) {
             // sum_g z_g (sum q) in one instruction: its k indices 2 t and 2 t + 1 meet (scale, base) of group t, so the operand has 0 and
             // the sum of q there, as two fp16 numbers (22 bits; 2^10 larger, so that the second is no subnormal) one after the other
             float sum = 0.f;
@@ -593,7 +596,7 @@ attn4_kernel(const __grid_constant__ Attn4Args A) {
                     a4_lds<NB>(w0, at_k + st);
                     a4_lds<NB>(w1, at_k + st + 8 * X::ROW);
                 }
-                if constexpr (X::BASES) {
+                if constexpr (BASES) {
                     uint32_t z0, z1;
                     float zq[4];
                     a4_lds<1>(&z0, at_kz + st);
@@ -622,7 +625,7 @@ attn4_kernel(const __grid_constant__ Attn4Args A) {
                         begun = true;
                         a4_mma(acc, x2, y2, x3, y3, q4.z, q4.w);
                     }
-                    if constexpr (!X::BASES) {
+                    if constexpr (!BASES) {
                         s[0] = fmaf(z0[g], qsum[g][0], s[0]);
                         s[1] = fmaf(z0[g], qsum[g][1], s[1]);
                         s[2] = fmaf(z1[g], qsum[g][0], s[2]);
@@ -693,7 +696,7 @@ attn4_kernel(const __grid_constant__ Attn4Args A) {
                 ref[1] = r1;
                 l[0] *= a0;
                 l[1] *= a1;
-                if constexpr (X::BASES) {
+                if constexpr (BASES) {
                     const float back = a4_exp2(e_was - e);
                     bacc[0] *= a0 * back;
                     bacc[1] *= a1 * back;
@@ -734,7 +737,7 @@ attn4_kernel(const __grid_constant__ Attn4Args A) {
             constexpr uint32_t ONES = 0x3c003c00u;
             const float sign = sub & 1 ? -1.f : 1.f;
             uint32_t pb[NG][2];
-            if constexpr (X::BASES) {
+            if constexpr (BASES) {
                 uint32_t b0, b1;
                 float x[4];
                 a4_ldm_trans(b0, b1, at_b + st);
@@ -751,7 +754,7 @@ attn4_kernel(const __grid_constant__ Attn4Args A) {
                     for (int i = 0; i < 4; ++i) w[i] = fmaf(w[i], w_all, __uint_as_float((__float_as_uint(w[i]) & 0xffffe000u) ^ w_flip));
                 pb[g][0] = a4_transpose(f2_to_h2(w[0], w[1]));
                 pb[g][1] = a4_transpose(f2_to_h2(w[2], w[3]));
-                if constexpr (!X::BASES) {
+                if constexpr (!BASES) {
                     zacc[g][0] = fmaf(p[0], y0, fmaf(p[2], y1, zacc[g][0]));
                     zacc[g][1] = fmaf(p[1], y0, fmaf(p[3], y1, zacc[g][1]));
                 }
@@ -789,14 +792,14 @@ attn4_kernel(const __grid_constant__ Attn4Args A) {
         for (int o = 4; o <= 16; o <<= 1) {
             l[0] += __shfl_xor_sync(0xffffffffu, l[0], o);
             l[1] += __shfl_xor_sync(0xffffffffu, l[1], o);
-            if constexpr (!X::BASES)
+            if constexpr (!BASES)
 #pragma unroll
                 for (int g = 0; g < NG; ++g) {
                     zacc[g][0] += __shfl_xor_sync(0xffffffffu, zacc[g][0], o);
                     zacc[g][1] += __shfl_xor_sync(0xffffffffu, zacc[g][1], o);
                 }
         }
-        if constexpr (X::BASES) {
+        if constexpr (BASES) {
             const float back = a4_exp2(e - 9.f);
 #pragma unroll
             for (int g = 0; g < NG; ++g)
@@ -976,21 +979,23 @@ attn4_kernel(const __grid_constant__ Attn4Args A) {
 constexpr size_t A4_COUNTERS_OFF = 256, A4_PARTS_OFF = 128 * 1024;
 static size_t attn4_ws_bytes(int d) { return A4_PARTS_OFF + (size_t)A4_MAX_CTAS * 2 * (d * A4_HEADS + 16) * sizeof(float); }
 
-template <int NB, int NG, bool SPLIT>
+template <int NB, int NG, int MODE>
 static int attn4_launch_as(const char *name, const Attn4Args &A, long max_units, cudaStream_t st) {
     using X = A4<NB, NG>;
     static OncePerDevice once;
-    cudaError_t e = once.run([&] { return cudaFuncSetAttribute(attn4_kernel<NB, NG, SPLIT>, cudaFuncAttributeMaxDynamicSharedMemorySize, X::SMEM); });
+    cudaError_t e = once.run([&] { return cudaFuncSetAttribute(attn4_kernel<NB, NG, MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, X::SMEM); });
     if (e != cudaSuccess) return fail((int)e, "%s: shared memory %d: %s", name, X::SMEM, cudaGetErrorString(e));
     const int wave = min(sm_count() * X::CTAS, A4_MAX_CTAS);
-    launch_kernel(attn4_kernel<NB, NG, SPLIT>, dim3((unsigned)min(max_units, (long)wave)), dim3(A4_THREADS), X::SMEM, st, A);
+    launch_kernel(attn4_kernel<NB, NG, MODE>, dim3((unsigned)min(max_units, (long)wave)), dim3(A4_THREADS), X::SMEM, st, A);
     return launch_status(name);
 }
 
 template <int NB, int NG>
 static int attn4_launch_shape(const char *name, const Attn4Args &A, long max_units, cudaStream_t st) {
-    const bool split = !A.bf16 && A.hq / A.C.heads <= 4;
-    return split ? attn4_launch_as<NB, NG, true>(name, A, max_units, st) : attn4_launch_as<NB, NG, false>(name, A, max_units, st);
+    if (!A.bf16 && A.hq / A.C.heads <= 4) return attn4_launch_as<NB, NG, A4_SPLIT>(name, A, max_units, st);
+    if constexpr (A4<NB, NG>::BASES)
+        if (!A.bf16) return attn4_launch_as<NB, NG, A4_EXACT_BASES>(name, A, max_units, st);
+    return attn4_launch_as<NB, NG, A4_PLAIN>(name, A, max_units, st);
 }
 
 static int attn4_launch(const char *name, const void *q, const Kv4Cache &C, bool paged, const int32_t *lens, void *out, int batch, int hq,
