@@ -528,6 +528,25 @@ def test_attention_cut_and_whole_contexts(P, oracle, dtype, hq, hkv, d, g, block
         check_attention(oracle, c, q, now, out, d ** -0.5, dtype)
 
 
+@pytest.mark.parametrize("hq,hkv,d,g", [(8, 2, 128, 64), (4, 4, 128, 128), (3, 1, 64, 64), (8, 2, 96, 32), (6, 3, 256, 128)])
+def test_attention_of_few_heads_loses_nothing_but_the_output_rounding(P, oracle, hq, hkv, d, g):
+    """Up to 4 q heads a kv head, fp16: 22 bits of a probability times a scale count (2^-22), so of the general bound's 2^-11 there
+    remains what the exponential and the fp32 sums are off (2^-19, and 2^-19 for what the tensor cores cut off)."""
+    b, n = 2, 420
+    c = Cache(b, hkv, d, g, n)
+    lens = [n, n - 130]
+    k, v = as64(values((b, hkv, n, d), "f16", 71)), as64(values((b, hkv, n, d), "f16", 72))
+    c.fill(k, v, lens, oracle)
+    q = values((b, hq, d), "f16", 73)
+    out = torch.empty((b, hq, d), dtype=torch.float16, device=DEV)
+    c.attend(P, "f16", q, t(np.array(lens, np.int32)), out, d ** -0.5)
+    for s, m in enumerate(lens):
+        (kw, kp), (vw, vp) = c.rows(0, s, m), c.rows(1, s, m)
+        ref, mag, smag = oracle.kv4_decode_attention(as64(q[s]), kw, kp, vw, vp, d ** -0.5)
+        bound = half_step("f16", ref) + (2.0 ** -22 + 2.0 ** -18 + 2 * 2.0 ** -20 * smag) * mag
+        assert (np.abs(as64(out[s]) - ref) <= bound).all()
+
+
 def big_cache(oracle, b, hkv, d, g, n, seed, block=0):
     """A long cache: random words and params straight on the device."""
     c = Cache(b, hkv, d, g, n, block, seed)
