@@ -562,7 +562,9 @@ int kv_cache_read_paged_int4_f16(const int32_t *k_codes, const b200k_half *k_par
                                  int out_len, b200k_stream stream);
 /* batched_decode_attention_hm_f16 over a 4-bit cache: q / output [batch, num_q_heads, head_dim], context_lens [batch] int32
  * (0 or less: a zero output row), any GQA group size.  The cache's values are never rounded; scores, softmax statistics and sums
- * are fp32, and what is rounded to fp16 on the way is each probability times its value scale.  The `_ws` editions take a
+ * are fp32.  On the way a probability times its value scale is rounded to fp16, but for fp16 outputs with up to 4 q heads a kv
+ * head, which keep 22 bits; and, where a row has four groups, the probability that its bases are multiplied by, but for fp16
+ * outputs with more.  The `_ws` editions take a
  * workspace of b200k_attention_int4_workspace_bytes whose first 128 KiB are zero before the first call and then left to the
  * kernels (b200k_workspace_status reads its status word); calls that may run at the same time need one each. */
 size_t b200k_attention_int4_workspace_bytes(int batch, int num_q_heads, int num_kv_heads, int head_dim);
